@@ -46,6 +46,7 @@ extern "C" {
 
 #define OPUS_DTYPE_BF16 0
 #define OPUS_DTYPE_F32 1
+#define OPUS_DTYPE_F16 2 /* the training-step operators alone take it */
 
 /* Library version (OPUS_ABI_VERSION). */
 OPUS_API int opus_abi_version(void);
@@ -338,6 +339,121 @@ OPUS_API int opus_gemm_bf16(const void* a, const void* a_lo, const void* b, int 
 OPUS_API int64_t opus_muon_S_workspace_bytes(int d_out, int d_in);
 OPUS_API int opus_muon_S(const void* m, int m_dtype, int d_out, int d_in, void* workspace, int64_t workspace_bytes,
                          void* S, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Operators of the training step around the capture layers (no counterpart
+ * in the reference's selection modules; its training driver leaves them to
+ * torch).  Arrays are bf16, f16 or f32 (OPUS_DTYPE_*); sums are held in f32 or
+ * wider and every result is rounded once.
+ */
+
+/*
+ * Embedding lookup with scaling: out[i] = scale * weight[tokens[i]], n rows of
+ * d elements of weight's type.  weight is [vocab, d] with rows row_stride
+ * elements apart; tokens are int32 or int64 (token_bits 32 or 64).  A token
+ * outside [0, vocab) gives a row of zeros and records 0x202 in the device
+ * error word.  n and vocab up to 2^31 - 1, d up to 65536.
+ */
+OPUS_API int opus_embedding(const void* tokens, int token_bits, int64_t n, const void* weight, int dtype,
+                            int64_t vocab, int64_t row_stride, int d, float scale, void* out, void* stream);
+
+/*
+ * Its gradient by sorted tokens: grad_weight[v] (+)= scale * sum of grad_out[i]
+ * over the i with tokens[i] = v, in the order of the i (the same bits from
+ * every call).  grad_out has n rows of d elements, row_stride apart;
+ * grad_weight is [vocab, d], contiguous, of grad_out's type or f32.  Without
+ * accumulate every row is written, zeros where no token names it; with it only
+ * rows that a token names are touched.  Tokens equal to padding_idx (-1: none)
+ * and tokens outside [0, vocab) (recorded as above) add nothing.  workspace:
+ * opus_embedding_grad_workspace_bytes of device memory, 256-byte aligned.
+ */
+OPUS_API int64_t opus_embedding_grad_workspace_bytes(int64_t n, int64_t vocab, int d);
+OPUS_API int opus_embedding_grad(const void* grad_out, int grad_dtype, int64_t row_stride, const void* tokens,
+                                 int token_bits, int64_t n, int64_t vocab, int d, float scale, int64_t padding_idx,
+                                 void* grad_weight, int out_dtype, int accumulate, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
+/*
+ * The joint between two blocks of a residual network: the norm after the one,
+ * its gate, the scaled residual sum and the norm before the next.
+ *
+ *   z = y, or with `post` N(y) * post_weight + post_bias
+ *   h = residual_scale * x + gate * z        rounded to x's type
+ *   n = N(h) * weight + bias                 rounded to y's type
+ *
+ * N is an RMS norm (kind 0: v / sqrt(mean v^2 + eps)) or a layer norm (kind 1:
+ * (v - mean) / sqrt(variance + eps)) over d elements, of the h that is stored.
+ * NULL parameters are ones (weights, gate) and zeros (biases).  The gate is one
+ * row of d (gate_rows 1) or one for each run of rows / gate_rows rows.  y may
+ * be NULL (no block output): h = residual_scale * x.  h may be NULL when y is
+ * and residual_scale is 1: then h is x.
+ * x, h: x_dtype, f32 or y_dtype; y, n: y_dtype; parameters: each of its own
+ * type.  x, y, h, n and their gradients are [rows, d] with the stated row
+ * strides (in elements; outputs are contiguous).  d up to 16384.
+ */
+typedef struct {
+  int64_t rows;
+  int d;
+  int kind;            /* 0 RMS norm, 1 layer norm */
+  int post;            /* 1: y is normed first */
+  int x_dtype, y_dtype;
+  float eps, residual_scale;
+  const void* x;       /* forward */
+  const void* y;
+  int64_t x_stride, y_stride;
+  const void *weight, *bias, *post_weight, *post_bias, *gate;
+  int weight_dtype, bias_dtype, post_weight_dtype, post_bias_dtype, gate_dtype;
+  int64_t gate_rows;
+  void* h;             /* forward: written; backward: read, contiguous or with h_stride */
+  int64_t h_stride;
+  void* n;             /* forward: written */
+  float* stats;        /* [rows, 4] f32: mean and 1/sd of h, mean and 1/sd of y; written, then read */
+  /* backward */
+  const void* grad_n;  /* y_dtype, NULL: zeros */
+  const void* grad_h;  /* x_dtype, NULL: zeros (the gradient of h as an output of its own) */
+  int64_t grad_n_stride, grad_h_stride;
+  void* grad_x;        /* x_dtype */
+  void* grad_y;        /* y_dtype, NULL exactly when y is */
+  void *grad_weight, *grad_bias, *grad_post_weight, *grad_post_bias, *grad_gate; /* of the parameter's type; NULL:
+                          not wanted (and where there is no such parameter) */
+} opus_residual_norm_args;
+
+OPUS_API int opus_residual_norm(const opus_residual_norm_args* args, void* stream);
+
+/*
+ * Gradients of the same.  The parameters' gradients are sums over the rows in
+ * a fixed order (the same bits from every call on one device).  workspace:
+ * opus_residual_norm_grad_workspace_bytes of device memory, 256-byte aligned.
+ */
+OPUS_API int64_t opus_residual_norm_grad_workspace_bytes(const opus_residual_norm_args* args);
+OPUS_API int opus_residual_norm_grad(const opus_residual_norm_args* args, void* workspace, int64_t workspace_bytes,
+                                     void* stream);
+
+/*
+ * Global gradient norm over `count` tensors, and clipping by it.  grads, outs,
+ * numels, dtypes and out_dtypes are arrays in HOST memory (of device
+ * addresses, lengths and types), read before the call returns; a captured
+ * graph keeps them.  Tensors are runs of elements without gaps; their order
+ * inside a tensor does not matter.
+ *
+ * opus_grad_norm: *norm (f32, on the device) = sqrt of the sum of all squares
+ * (norm_kind 2) or the largest magnitude (norm_kind 0).  0 for an empty list.
+ * opus_clip_grads: the same, then outs[j] = c * grads[j] with
+ * c = min(1, max_norm / (*norm + 1e-6)), the rule of
+ * torch.nn.utils.clip_grad_norm_; a NaN norm gives NaN, an infinite one zeros
+ * (and NaN where the element is infinite).  outs[j] is grads[j] (in place), or memory that
+ * overlaps no list member, of any of the types.
+ * opus_scale_grads: the second half for a *norm that the caller has.
+ * workspace: opus_grad_norm_workspace_bytes(count), 8-byte aligned.
+ */
+OPUS_API int64_t opus_grad_norm_workspace_bytes(int count);
+OPUS_API int opus_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int count,
+                            int norm_kind, void* workspace, int64_t workspace_bytes, float* norm, void* stream);
+OPUS_API int opus_clip_grads(const void* const* grads, const int* dtypes, void* const* outs, const int* out_dtypes,
+                             const int64_t* numels, int count, int norm_kind, float max_norm, void* workspace,
+                             int64_t workspace_bytes, float* norm, void* stream);
+OPUS_API int opus_scale_grads(const void* const* grads, const int* dtypes, void* const* outs, const int* out_dtypes,
+                              const int64_t* numels, int count, float max_norm, const float* norm, void* stream);
 
 /* Number of kernels this library has launched in the process so far (all
  * devices).  Instrumentation with no counterpart in the reference: the

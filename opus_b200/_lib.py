@@ -21,8 +21,30 @@ OPUS_ERR_DEVICE = 4
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_F16 = 2
 
 _c_int, _c_i64, _c_f32, _c_f64, _c_p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_void_p
+
+
+
+class ResidualNormArgs(ctypes.Structure):
+    """opus_residual_norm_args of include/opus_b200.h, field by field."""
+    _fields_ = [
+        ("rows", _c_i64), ("d", _c_int), ("kind", _c_int), ("post", _c_int), ("x_dtype", _c_int),
+        ("y_dtype", _c_int), ("eps", _c_f32), ("residual_scale", _c_f32),
+        ("x", _c_p), ("y", _c_p), ("x_stride", _c_i64), ("y_stride", _c_i64),
+        ("weight", _c_p), ("bias", _c_p), ("post_weight", _c_p), ("post_bias", _c_p), ("gate", _c_p),
+        ("weight_dtype", _c_int), ("bias_dtype", _c_int), ("post_weight_dtype", _c_int),
+        ("post_bias_dtype", _c_int), ("gate_dtype", _c_int), ("gate_rows", _c_i64),
+        ("h", _c_p), ("h_stride", _c_i64), ("n", _c_p), ("stats", _c_p),
+        ("grad_n", _c_p), ("grad_h", _c_p), ("grad_n_stride", _c_i64), ("grad_h_stride", _c_i64),
+        ("grad_x", _c_p), ("grad_y", _c_p),
+        ("grad_weight", _c_p), ("grad_bias", _c_p), ("grad_post_weight", _c_p), ("grad_post_bias", _c_p),
+        ("grad_gate", _c_p),
+    ]
+
+
+_norm_args = ctypes.POINTER(ResidualNormArgs)
 
 # name -> (restype, argtypes); mirrors include/opus_b200.h
 SIGNATURES: dict[str, tuple] = {
@@ -58,6 +80,17 @@ SIGNATURES: dict[str, tuple] = {
     "opus_muon_S": (_c_int, [_c_p, _c_int, _c_int, _c_int, _c_p, _c_i64, _c_p, _c_p]),
     "opus_kernel_launches": (_c_i64, []),
     "opus_adam_diag": (_c_int, [_c_p, _c_f32, _c_i64, _c_p, _c_p]),
+    "opus_embedding": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_int, _c_i64, _c_i64, _c_int, _c_f32, _c_p, _c_p]),
+    "opus_embedding_grad_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_int]),
+    "opus_embedding_grad": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_int, _c_i64, _c_i64, _c_int, _c_f32, _c_i64, _c_p,
+                                     _c_int, _c_int, _c_p, _c_i64, _c_p]),
+    "opus_residual_norm": (_c_int, [_norm_args, _c_p]),
+    "opus_residual_norm_grad_workspace_bytes": (_c_i64, [_norm_args]),
+    "opus_residual_norm_grad": (_c_int, [_norm_args, _c_p, _c_i64, _c_p]),
+    "opus_grad_norm_workspace_bytes": (_c_i64, [_c_int]),
+    "opus_grad_norm": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_int, _c_p, _c_i64, _c_p, _c_p]),
+    "opus_clip_grads": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_f32, _c_p, _c_i64, _c_p, _c_p]),
+    "opus_scale_grads": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_f32, _c_p, _c_p]),
     "opus_sketch_dense_rows": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_i64, _c_int, _c_p, _c_int, _c_p]),
 }
 
@@ -67,7 +100,8 @@ _timer = None  # the active KernelTimer, if any
 
 # entry points that launch no kernel of their own or only query state
 _UNTIMED = {"opus_abi_version", "opus_last_error", "opus_device_error", "opus_sketch_table_entries",
-            "opus_muon_S_workspace_bytes", "opus_kernel_launches"}
+            "opus_muon_S_workspace_bytes", "opus_kernel_launches", "opus_embedding_grad_workspace_bytes",
+            "opus_residual_norm_grad_workspace_bytes", "opus_grad_norm_workspace_bytes"}
 
 
 class KernelTimer:

@@ -1,0 +1,373 @@
+// Global gradient norm over many tensors, and clipping by it.
+//
+//   opus_grad_norm    |g| = sqrt(sum_j sum_i g_ji^2), or max_ji |g_ji|
+//   opus_clip_grads   the same, then out_j = c g_j with c = min(1, max_norm / (|g| + 1e-6))
+//   opus_scale_grads  the second half alone, for a norm that the caller has (joined over ranks, say)
+//
+// Mathematics.  A thread sums the squares of the up to 32 elements of one
+// round of loads in f32 and adds the result to a double, so the rounding error
+// of the whole is that of 32 f32 additions however long the list is.  Where
+// such a partial sum leaves [1e-25, 1e30] (squares that overflow, or vanish,
+// in f32) the same registers are summed again in double.  Partial sums meet in
+// a fixed order: the norm is the same for every run on one device.
+//
+// Bound: HBM bandwidth, reads once for the norm and once more (with the
+// writes) to scale; a list of one type below the bound is not written at all
+// in place, since c = 1 would write what is there.
+//
+// Layout: the list travels as a kernel parameter (addresses, lengths, types:
+// no copy to the device, and a captured graph holds its own), cut into chunks
+// that blocks take in turn; a block finds a chunk's tensor by bisection.
+#include <limits>
+
+#include "elements.cuh"
+
+namespace opus {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlocksPerSm = 8;
+constexpr int64_t kChunk = 16384;  // elements
+constexpr int kMaxTensors = 1024;  // of one launch: its table stays below the 32764 bytes of parameters
+constexpr float kNormEps = 1e-6f;  // as torch.nn.utils.clip_grad_norm_ has it
+
+struct GradTable {
+  const void* in[kMaxTensors];
+  void* out[kMaxTensors];
+  int64_t n[kMaxTensors];
+  int first_chunk[kMaxTensors];
+  uint8_t types[kMaxTensors];  // type in | type out << 4
+  int count;
+  int chunks;
+};
+static_assert(sizeof(GradTable) <= 32000, "kernel parameters");
+
+__device__ __forceinline__ int find_tensor(const GradTable& t, int chunk) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first_chunk[mid] <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Sum (kind 2) or maximum (kind 0: the infinity norm, NaN wins) of doubles.
+__device__ __forceinline__ double join(double a, double b, int kind) {
+  if (kind == 2) return a + b;
+  return (a != a || a > b) ? a : b;
+}
+
+// Every thread's value joined over the block, in a fixed order; valid in all threads.
+__device__ double block_join(double v, int kind) {
+  __shared__ double warp_part[kThreads / 32];
+  __syncthreads();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_down_sync(0xffffffffu, v, o), kind);
+  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = warp_part[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) s = join(s, warp_part[w], kind);
+  return s;
+}
+
+// What one group of elements adds to a thread's partial sum.
+template <int N>
+__device__ __forceinline__ double group_part(const float (&x)[N], int kind) {
+  if (kind != 2) {
+    double m = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = join(m, static_cast<double>(fabsf(x[i])), 0);
+    return m;
+  }
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i & 3] = fmaf(x[i], x[i], s[i & 3]);
+  const float f = (s[0] + s[1]) + (s[2] + s[3]);
+  if (f > 1e-25f && f < 1e30f) return static_cast<double>(f);
+  double d = 0.0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) d = fma(static_cast<double>(x[i]), static_cast<double>(x[i]), d);
+  return d;
+}
+
+template <typename T>
+__device__ double chunk_part(const T* p, int n, int kind) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int U = 4;
+  double acc = 0.0;
+  int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T));
+  head = head < n ? head : n;
+  const int vecs = (n - head) / V;
+  const T* body = p + head;
+  for (int b = threadIdx.x; b < vecs; b += kThreads * U) {
+    float x[U * V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float r[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) r[i] = 0.f;
+      if (b + u * kThreads < vecs) load_vec<T, V>(body + static_cast<int64_t>(b + u * kThreads) * V, r);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[u * V + i] = r[i];
+    }
+    acc = join(acc, group_part(x, kind), kind);
+  }
+  // the up to V - 1 elements before the first 16-byte boundary and after the last
+  const int tail = head + vecs * V;
+  const int i = static_cast<int>(threadIdx.x);
+  const int at = i < head ? i : tail + (i - head);
+  if (at < n) {
+    const float x[1] = {to_f32(p[at])};
+    acc = join(acc, group_part(x, kind), kind);
+  }
+  return acc;
+}
+
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ GradTable t, int kind,
+                                                        double* __restrict__ partial) {
+  double acc = 0.0;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int j = find_tensor(t, c);
+    const int64_t at = static_cast<int64_t>(c - t.first_chunk[j]) * kChunk;
+    const int n = static_cast<int>(t.n[j] - at < kChunk ? t.n[j] - at : kChunk);
+    const int type = t.types[j] & 15;
+    double d;
+    if (type == OPUS_DTYPE_F32) d = chunk_part(static_cast<const float*>(t.in[j]) + at, n, kind);
+    else if (type == OPUS_DTYPE_F16) d = chunk_part(static_cast<const __half*>(t.in[j]) + at, n, kind);
+    else d = chunk_part(static_cast<const __nv_bfloat16*>(t.in[j]) + at, n, kind);
+    acc = join(acc, d, kind);
+  }
+  acc = block_join(acc, kind);
+  if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+// The norm from the blocks' partial sums: every block of the launch does the
+// same additions in the same order.
+__device__ float whole_norm(const double* __restrict__ partial, int parts, int kind) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kThreads) s = join(s, partial[i], kind);
+  s = block_join(s, kind);
+  return static_cast<float>(kind == 2 ? sqrt(s) : s);
+}
+
+__global__ void __launch_bounds__(kThreads) norm_join_kernel(const double* __restrict__ partial, int parts, int kind,
+                                                             float* __restrict__ norm) {
+  const float n = whole_norm(partial, parts, kind);
+  if (threadIdx.x == 0) *norm = n;
+}
+
+template <typename TI, typename TO>
+__device__ void chunk_scale(const TI* p, TO* q, int n, float c) {
+  constexpr int V = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));
+  constexpr int U = 4;
+  int head = static_cast<int>((V * sizeof(TI) - (reinterpret_cast<uintptr_t>(p) & (V * sizeof(TI) - 1))) &
+                              (V * sizeof(TI) - 1)) / static_cast<int>(sizeof(TI));
+  head = head < n ? head : n;
+  // both sides reach their boundaries together, or the chunk goes element by element
+  if ((reinterpret_cast<uintptr_t>(q + head) & (V * sizeof(TO) - 1)) != 0) head = n;
+  const int vecs = (n - head) / V;
+  for (int b = threadIdx.x; b < vecs; b += kThreads * U) {
+    float x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (b + u * kThreads < vecs) load_vec<TI, V>(p + head + static_cast<int64_t>(b + u * kThreads) * V, x[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (b + u * kThreads < vecs) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[u][i] *= c;
+        store_vec<TO, V>(q + head + static_cast<int64_t>(b + u * kThreads) * V, x[u]);
+      }
+  }
+  const int tail = head + vecs * V;
+  for (int i = threadIdx.x; i < head + (n - tail); i += kThreads) {
+    const int at = i < head ? i : tail + (i - head);
+    q[at] = from_f32<TO>(to_f32(p[at]) * c);
+  }
+}
+
+template <typename TI>
+__device__ void chunk_scale_to(const TI* p, void* q, int64_t at, int type, int n, float c) {
+  if (type == OPUS_DTYPE_F32) chunk_scale(p, static_cast<float*>(q) + at, n, c);
+  else if (type == OPUS_DTYPE_F16) chunk_scale(p, static_cast<__half*>(q) + at, n, c);
+  else chunk_scale(p, static_cast<__nv_bfloat16*>(q) + at, n, c);
+}
+
+// parts > 0: the norm is joined from partial sums here (and block 0 writes it); otherwise it is read.
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ GradTable t, int kind,
+                                                         const double* __restrict__ partial, int parts,
+                                                         float max_norm, float* __restrict__ norm) {
+  float n;
+  if (parts > 0) {
+    n = whole_norm(partial, parts, kind);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
+  } else {
+    n = *norm;
+  }
+  float c = max_norm / (n + kNormEps);
+  c = c > 1.0f ? 1.0f : c;  // a NaN stays
+  for (int k = blockIdx.x; k < t.chunks; k += gridDim.x) {
+    const int j = find_tensor(t, k);
+    if (c == 1.0f && t.in[j] == t.out[j]) continue;  // in place: there already
+    const int64_t at = static_cast<int64_t>(k - t.first_chunk[j]) * kChunk;
+    const int len = static_cast<int>(t.n[j] - at < kChunk ? t.n[j] - at : kChunk);
+    const int type = t.types[j] & 15, to = t.types[j] >> 4;
+    if (type == OPUS_DTYPE_F32) chunk_scale_to(static_cast<const float*>(t.in[j]) + at, t.out[j], at, to, len, c);
+    else if (type == OPUS_DTYPE_F16) chunk_scale_to(static_cast<const __half*>(t.in[j]) + at, t.out[j], at, to, len, c);
+    else chunk_scale_to(static_cast<const __nv_bfloat16*>(t.in[j]) + at, t.out[j], at, to, len, c);
+  }
+}
+
+struct Lists {
+  const void* const* in;
+  void* const* out;
+  const int64_t* n;
+  const int* in_types;
+  const int* out_types;
+  int count;
+};
+
+int check_lists(const char* what, const Lists& l, bool outs) {
+  if (l.count < 0) return set_error(OPUS_ERR_INVALID, "%s: %d tensors", what, l.count);
+  if (l.count > 0 && (!l.in || !l.n || !l.in_types || (outs && (!l.out || !l.out_types))))
+    return set_error(OPUS_ERR_INVALID, "%s: NULL list", what);
+  int64_t chunks = 0;
+  for (int i = 0; i < l.count; ++i) {
+    if (l.n[i] < 0) return set_error(OPUS_ERR_INVALID, "%s: tensor %d has %lld elements", what, i, (long long)l.n[i]);
+    if (!dtype_ok(l.in_types[i]) || (outs && !dtype_ok(l.out_types[i])))
+      return set_error(OPUS_ERR_UNSUPPORTED, "%s: tensor %d is neither bf16, f16 nor f32", what, i);
+    if (l.n[i] > 0 && (!l.in[i] || (outs && !l.out[i])))
+      return set_error(OPUS_ERR_INVALID, "%s: tensor %d is NULL", what, i);
+    if (reinterpret_cast<uintptr_t>(l.in[i]) % dtype_bytes(l.in_types[i]) != 0 ||
+        (outs && reinterpret_cast<uintptr_t>(l.out[i]) % dtype_bytes(l.out_types[i]) != 0))
+      return set_error(OPUS_ERR_INVALID, "%s: tensor %d is not aligned to its elements", what, i);
+    chunks += l.n[i] / kChunk + 1;
+    if (l.n[i] > std::numeric_limits<int64_t>::max() / 8 || chunks > std::numeric_limits<int>::max() / 2)
+      return set_error(OPUS_ERR_UNSUPPORTED, "%s: the list is too long", what);
+  }
+  return OPUS_OK;
+}
+
+// Tensors [at, ...) of the list as one launch's table; returns the index of the first that did not fit.
+int fill_table(const Lists& l, int at, GradTable* t) {
+  t->count = 0;
+  int64_t chunks = 0;
+  for (; at < l.count && t->count < kMaxTensors; ++at) {
+    if (l.n[at] == 0) continue;
+    const int k = t->count++;
+    t->in[k] = l.in[at];
+    t->out[k] = l.out ? l.out[at] : nullptr;
+    t->n[k] = l.n[at];
+    t->first_chunk[k] = static_cast<int>(chunks);
+    t->types[k] = static_cast<uint8_t>(l.in_types[at] | (l.out ? l.out_types[at] << 4 : 0));
+    chunks += (l.n[at] + kChunk - 1) / kChunk;
+  }
+  t->chunks = static_cast<int>(chunks);
+  return at;
+}
+
+int grid_of(const GradTable& t) {
+  const int most = sm_count() * kBlocksPerSm;
+  return t.chunks < most ? t.chunks : most;
+}
+
+int launches_of(int count) { return (count + kMaxTensors - 1) / kMaxTensors; }
+
+// Partial sums of every launch side by side; *parts is their number.
+int launch_norm(const Lists& l, int kind, double* partial, int* parts, cudaStream_t st) {
+  GradTable t;
+  *parts = 0;
+  for (int at = 0; at < l.count;) {
+    at = fill_table(l, at, &t);
+    if (t.chunks == 0) continue;
+    const int grid = grid_of(t);
+    norm_kernel<<<grid, kThreads, 0, st>>>(t, kind, partial + *parts);
+    note_launch();
+    OPUS_CUDA_TRY(cudaGetLastError());
+    *parts += grid;
+  }
+  return OPUS_OK;
+}
+
+int launch_scale(const Lists& l, int kind, const double* partial, int parts, float max_norm, float* norm,
+                 cudaStream_t st) {
+  GradTable t;
+  for (int at = 0; at < l.count;) {
+    at = fill_table(l, at, &t);
+    if (t.chunks == 0) continue;
+    scale_kernel<<<grid_of(t), kThreads, 0, st>>>(t, kind, partial, parts, max_norm, norm);
+    note_launch();
+    OPUS_CUDA_TRY(cudaGetLastError());
+  }
+  return OPUS_OK;
+}
+
+int launch_join(const double* partial, int parts, int kind, float* norm, cudaStream_t st) {
+  norm_join_kernel<<<1, kThreads, 0, st>>>(partial, parts, kind, norm);
+  note_launch();
+  OPUS_CUDA_TRY(cudaGetLastError());
+  return OPUS_OK;
+}
+
+int check_norm_args(const char* what, int kind, const void* workspace, int64_t bytes, int count, const float* norm) {
+  if (kind != 2 && kind != 0) return set_error(OPUS_ERR_INVALID, "%s: norm kind %d is neither 2 nor 0 (infinity)", what, kind);
+  if (!workspace || !norm) return set_error(OPUS_ERR_INVALID, "%s: NULL pointer", what);
+  const int64_t need = opus_grad_norm_workspace_bytes(count);
+  if (bytes < need)
+    return set_error(OPUS_ERR_INVALID, "%s: workspace of %lld bytes, need %lld", what, (long long)bytes, (long long)need);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 7) != 0)
+    return set_error(OPUS_ERR_INVALID, "%s: workspace must be 8-byte aligned", what);
+  return OPUS_OK;
+}
+
+}  // namespace
+}  // namespace opus
+
+using namespace opus;
+
+extern "C" int64_t opus_grad_norm_workspace_bytes(int count) {
+  return static_cast<int64_t>(launches_of(count > 0 ? count : 1)) * sm_count() * kBlocksPerSm * 8;
+}
+
+extern "C" int opus_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int count,
+                              int norm_kind, void* workspace, int64_t workspace_bytes, float* norm, void* stream) {
+  const Lists l{grads, nullptr, numels, dtypes, nullptr, count};
+  int rc = check_lists("grad_norm", l, false);
+  if (rc) return rc;
+  rc = check_norm_args("grad_norm", norm_kind, workspace, workspace_bytes, count, norm);
+  if (rc) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  int parts = 0;
+  rc = launch_norm(l, norm_kind, partial, &parts, st);
+  if (rc) return rc;
+  return launch_join(partial, parts, norm_kind, norm, st);
+}
+
+extern "C" int opus_scale_grads(const void* const* grads, const int* dtypes, void* const* outs, const int* out_dtypes,
+                                const int64_t* numels, int count, float max_norm, const float* norm, void* stream) {
+  const Lists l{grads, outs, numels, dtypes, out_dtypes, count};
+  int rc = check_lists("scale_grads", l, true);
+  if (rc) return rc;
+  if (!norm) return set_error(OPUS_ERR_INVALID, "scale_grads: NULL pointer");
+  return launch_scale(l, 2, nullptr, 0, max_norm, const_cast<float*>(norm), reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int opus_clip_grads(const void* const* grads, const int* dtypes, void* const* outs, const int* out_dtypes,
+                               const int64_t* numels, int count, int norm_kind, float max_norm, void* workspace,
+                               int64_t workspace_bytes, float* norm, void* stream) {
+  const Lists l{grads, outs, numels, dtypes, out_dtypes, count};
+  int rc = check_lists("clip_grads", l, true);
+  if (rc) return rc;
+  rc = check_norm_args("clip_grads", norm_kind, workspace, workspace_bytes, count, norm);
+  if (rc) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  int parts = 0;
+  rc = launch_norm(l, norm_kind, partial, &parts, st);
+  if (rc) return rc;
+  if (parts == 0) return launch_join(partial, 0, norm_kind, norm, st);
+  return launch_scale(l, norm_kind, partial, parts, max_norm, norm, st);
+}

@@ -47,6 +47,7 @@ enum DeviceError : int {
   kDevTimeoutDrain = 0x105,
   kDevTimeoutSelftest = 0x106,  // opus_selftest_stalled_wait: a wait that nothing releases
   kDevBadBucket = 0x201,
+  kDevBadToken = 0x202,  // opus_embedding(_grad): a token outside [0, vocab)
 };
 
 // 1 second: every wait in these kernels normally completes in microseconds.

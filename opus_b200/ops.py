@@ -8,12 +8,15 @@ from __future__ import annotations
 
 import ctypes
 import math
+from collections.abc import Iterable, Sequence
 
+import numpy as np
 import torch
 
 from . import _lib
 
 _ERR_BAD_PROBS = 0x301
+_ERR_BAD_TOKEN = 0x202
 
 
 def _stream(t: torch.Tensor) -> ctypes.c_void_p:
@@ -41,6 +44,8 @@ def check_device_error(what: str = "opus kernel") -> None:
     code = _lib.device_error()
     if code == _ERR_BAD_PROBS:
         raise ValueError(f"{what}: probabilities do not sum to 1")
+    if code == _ERR_BAD_TOKEN:
+        raise IndexError(f"{what}: token outside the embedding's rows")
     if code:
         raise RuntimeError(f"{what}: device error 0x{code:x}")
 
@@ -620,3 +625,450 @@ def greedy_select(scores: torch.Tensor, sim: torch.Tensor, n_select: int) -> tor
     return out
 
 
+# ------------------------------------------------------- training step: shared
+_TYPE_CODES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16}
+
+
+def _type_code(t: torch.Tensor, name: str) -> int:
+    code = _TYPE_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    return code
+
+
+def _same_device(ref: torch.Tensor, **others: torch.Tensor | None) -> None:
+    """CUDA tensors of one device (checked after shapes and types, so those are checked without a GPU too)."""
+    for name, t in others.items():
+        if t is None:
+            continue
+        _cuda(t, name)
+        if t.device != ref.device:
+            raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """Call an entry point on the device's current stream, with the device current."""
+    fn = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    _lib.check(rc, name)
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """The tensor as rows of its last dimension, and their stride in elements; copied if rows are not evenly spaced."""
+    d = t.shape[-1]
+    if t.is_contiguous():
+        return t, d
+    if t.stride(-1) == 1 and t.numel() > 0:
+        try:
+            v = t.view(-1, d)
+        except RuntimeError:
+            return t.contiguous(), d
+        if v.shape[0] == 1:
+            return v, d
+        if v.stride(0) >= d:
+            return v, v.stride(0)
+    return t.contiguous(), d
+
+
+# ---------------------------------------------------- training step: embedding
+def _tokens(tokens: torch.Tensor) -> tuple[torch.Tensor, int]:
+    if not isinstance(tokens, torch.Tensor):
+        raise TypeError("tokens must be a torch.Tensor")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
+    return _contig(tokens), 64 if tokens.dtype == torch.int64 else 32
+
+
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """scale * weight[tokens]: [*tokens.shape, d] of weight's type, the product rounded once.
+
+    weight [V, d] in bf16, f16 or f32 (rows may be apart: a column slice of a
+    wider table is read in place).  A token outside [0, V) gives a row of
+    zeros, and the next check_device_error() raises IndexError.
+    """
+    tokens, bits = _tokens(tokens)
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"weight must be [V, d], got {tuple(weight.shape)}")
+    code = _type_code(weight, "weight")
+    V, d = weight.shape
+    shape = (*tokens.shape, d)
+    if out is not None and (out.shape != shape or out.dtype != weight.dtype or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous {weight.dtype} tensor of shape {shape}")
+    _same_device(weight, weight=weight, tokens=tokens, out=out)
+    weight, stride = _rows(weight)
+    if out is None:
+        out = torch.empty(shape, dtype=weight.dtype, device=weight.device)
+    _call("opus_embedding", weight.device, _ptr(tokens), bits, tokens.numel(), _ptr(weight), code, V, stride, d,
+          float(scale), _ptr(out))
+    return out
+
+
+def embedding_grad(grad_out: torch.Tensor, tokens: torch.Tensor, num_embeddings: int, scale: float = 1.0,
+                   padding_idx: int | None = None, out: torch.Tensor | None = None, accumulate: bool = False,
+                   out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Gradient of embedding() for the weight: out[v] (+)= scale * sum of grad_out over the positions of token v.
+
+    grad_out [*tokens.shape, d] in bf16, f16 or f32; out [num_embeddings, d]
+    of its type or float32 (out_dtype, or the type of out).  The sums run in
+    f32 over the positions in order: every call gives the same bits.  Rows of
+    padding_idx get nothing.  accumulate=True adds into out and touches only
+    rows that a token names; without it the rows of other tokens are zeros.
+    Tokens out of range add nothing and are reported as by embedding().
+    """
+    tokens, bits = _tokens(tokens)
+    V = int(num_embeddings)
+    if V < 1:
+        raise ValueError("num_embeddings must be positive")
+    if grad_out.dim() < 1 or grad_out.shape[:-1] != tokens.shape or grad_out.shape[-1] < 1:
+        raise ValueError(f"grad_out must be [*{tuple(tokens.shape)}, d], got {tuple(grad_out.shape)}")
+    code = _type_code(grad_out, "grad_out")
+    d = grad_out.shape[-1]
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx must be within [-{V}, {V}), got {padding_idx}")
+        padding_idx = padding_idx % V
+    if accumulate and out is None:
+        raise ValueError("accumulate needs out")
+    if out is not None:
+        if out_dtype is not None and out_dtype != out.dtype:
+            raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+        if out.shape != (V, d) or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous tensor of shape {(V, d)}")
+    dtype = out.dtype if out is not None else out_dtype or grad_out.dtype
+    if dtype not in (grad_out.dtype, torch.float32):
+        raise ValueError(f"the gradient is {grad_out.dtype} or float32, not {dtype}")
+    _same_device(grad_out, grad_out=grad_out, tokens=tokens, out=out)
+    grad_out, stride = _rows(grad_out)
+    if out is None:
+        out = torch.empty(V, d, dtype=dtype, device=grad_out.device)
+    n = tokens.numel()
+    ws_bytes = int(_lib.load().opus_embedding_grad_workspace_bytes(n, V, d))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=out.device)
+    _call("opus_embedding_grad", out.device, _ptr(grad_out), code, stride, _ptr(tokens), bits, n, V, d, float(scale),
+          -1 if padding_idx is None else int(padding_idx), _ptr(out), _type_code(out, "out"), int(accumulate), _ptr(ws),
+          ws_bytes)
+    return out
+
+
+# ------------------------------------------------ training step: residual norm
+_NORM_KINDS = {"rms": 0, "layer": 1}
+_NORM_PARAMS = ("weight", "bias", "post_weight", "post_bias", "gate")
+
+
+def _norm_args(like: torch.Tensor, y: torch.Tensor | None, y_dtype: torch.dtype, params: dict, post: bool, kind: str,
+               residual_scale: float) -> tuple[_lib.ResidualNormArgs, dict]:
+    """The C arguments that forward and backward share, and the contiguous parameters they point to."""
+    if kind not in _NORM_KINDS:
+        raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
+    if like.dim() < 1 or like.shape[-1] < 1:
+        raise ValueError(f"rows of at least one element expected, got {tuple(like.shape)}")
+    d = like.shape[-1]
+    a = _lib.ResidualNormArgs()
+    a.rows, a.d, a.kind, a.post = like.numel() // d, d, _NORM_KINDS[kind], int(post)
+    a.x_dtype = _type_code(like, "x")
+    if y_dtype not in _TYPE_CODES or (y_dtype != like.dtype and like.dtype != torch.float32):
+        raise ValueError(f"x must be of y's type (bfloat16, float16 or float32) or float32, got {like.dtype} with "
+                         f"{y_dtype}")
+    a.y_dtype = _TYPE_CODES[y_dtype]
+    a.residual_scale = float(residual_scale)
+    if y is not None and y.shape != like.shape:
+        raise ValueError(f"y must have x's shape {tuple(like.shape)}, got {tuple(y.shape)}")
+    if y is None and (post or params.get("gate") is not None):
+        raise ValueError("a gate or a norm after the block needs y")
+    if not post and (params.get("post_weight") is not None or params.get("post_bias") is not None):
+        raise ValueError("post_weight and post_bias belong to post=True")
+    kept = {}
+    for name in _NORM_PARAMS:
+        p = params.get(name)
+        if p is None:
+            continue
+        code = _type_code(p, name)
+        if name == "gate":
+            a.gate_rows = _gate_rows(p, like)
+        elif p.shape != (d,):
+            raise ValueError(f"{name} must be [{d}], got {tuple(p.shape)}")
+        kept[name] = p = _contig(p.detach())
+        setattr(a, name, p.data_ptr())
+        setattr(a, name + "_dtype", code)
+    return a, kept
+
+
+def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
+    """1 for a gate of [d]; the number of samples for one of [B, d] or [B, 1, ..., d] against x [B, ..., d]."""
+    d = x.shape[-1]
+    if gate.shape == (d,):
+        return 1
+    if x.dim() >= 2 and gate.dim() >= 2 and gate.shape[-1] == d and gate.shape[0] == x.shape[0] \
+            and gate.numel() == x.shape[0] * d and gate.dim() in (2, x.dim()):
+        return max(1, x.shape[0])
+    raise ValueError(f"gate must be [{d}] or one row for each of x's first dimension, got {tuple(gate.shape)} "
+                     f"for x {tuple(x.shape)}")
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, weight: torch.Tensor | None = None,
+                  bias: torch.Tensor | None = None, post_weight: torch.Tensor | None = None,
+                  post_bias: torch.Tensor | None = None, post: bool | None = None, gate: torch.Tensor | None = None,
+                  residual_scale: float = 1.0, kind: str = "rms", eps: float = 1e-6,
+                  out_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The joint between two blocks of a residual network in one kernel: (n, h, stats).
+
+        z = y, or with post its norm N(y) * post_weight + post_bias
+        h = residual_scale * x + gate * z            of x's type: the residual stream
+        n = N(h) * weight + bias                     of y's type: what the next block reads
+
+    x and y [..., d], d up to 16384, in bf16, f16 or f32 (x may be float32 with
+    a 16-bit y); N is an RMS norm (kind "rms") or a layer norm ("layer") over d.
+    Every parameter may be absent (ones, zeros) and has a type of its own.
+    gate is [d], or one row for each of x's first dimension ([B, d] or
+    [B, 1, d] against x [B, T, d]).  post defaults to whether post_weight or
+    post_bias is given.  Without y, h is residual_scale * x (x itself at 1) and
+    n of out_dtype (default x's type).  n is the norm of h as it is stored.
+    stats is what residual_norm_grad needs of the forward.
+    """
+    post = (post_weight is not None or post_bias is not None) if post is None else bool(post)
+    n_dtype = x.dtype if y is None else y.dtype
+    if out_dtype is not None and out_dtype != n_dtype:
+        if y is not None:
+            raise ValueError(f"out_dtype is y's type where y is given ({y.dtype}), got {out_dtype}")
+        n_dtype = out_dtype
+    params = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias, "gate": gate}
+    a, kept = _norm_args(x, y, n_dtype, params, post, kind, residual_scale)
+    a.eps = float(eps)
+    _same_device(x, x=x, y=y, **params)
+    xr, a.x_stride = _rows(x)
+    a.x = xr.data_ptr()
+    if y is not None:
+        yr, a.y_stride = _rows(y)
+        a.y = yr.data_ptr()
+    plain = y is None and a.residual_scale == 1.0
+    h = x if plain else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = torch.empty(x.shape, dtype=n_dtype, device=x.device)
+    stats = torch.empty(a.rows, 4, dtype=torch.float32, device=x.device)
+    a.h, a.h_stride = None if plain else h.data_ptr(), a.d
+    a.n, a.stats = n.data_ptr(), stats.data_ptr()
+    _call("opus_residual_norm", x.device, ctypes.byref(a))
+    return n, h, stats
+
+
+def residual_norm_grad(grad_n: torch.Tensor | None, grad_h: torch.Tensor | None, h: torch.Tensor, stats: torch.Tensor,
+                       y: torch.Tensor | None = None, *, weight: torch.Tensor | None = None,
+                       bias: torch.Tensor | None = None, post_weight: torch.Tensor | None = None,
+                       post_bias: torch.Tensor | None = None, post: bool | None = None,
+                       gate: torch.Tensor | None = None, residual_scale: float = 1.0, kind: str = "rms",
+                       wanted: Iterable[str] | None = None) -> dict[str, torch.Tensor]:
+    """Gradients of residual_norm from those of its outputs n and h (one of them may be None: zeros).
+
+    h and stats are the forward's outputs, the other arguments those it was
+    given.  Returns {"x", "y" (if y), and one entry for each parameter given};
+    wanted restricts the parameters' gradients to the named ones.  Each is of
+    its tensor's type and shape.  Sums over rows run in f32 in a fixed order:
+    every call gives the same bits.
+    """
+    post = (post_weight is not None or post_bias is not None) if post is None else bool(post)
+    if grad_n is None and grad_h is None:
+        raise ValueError("grad_n or grad_h must be given")
+    n_dtype = y.dtype if y is not None else grad_n.dtype if grad_n is not None else h.dtype
+    params = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias, "gate": gate}
+    a, kept = _norm_args(h, y, n_dtype, params, post, kind, residual_scale)
+    for name, t, dtype in (("grad_n", grad_n, n_dtype), ("grad_h", grad_h, h.dtype)):
+        if t is not None and (t.shape != h.shape or t.dtype != dtype):
+            raise ValueError(f"{name} must be {dtype} {tuple(h.shape)}, got {t.dtype} {tuple(t.shape)}")
+    if stats.shape != (a.rows, 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError(f"stats must be the forward's, a contiguous float32 [{a.rows}, 4]")
+    names = set(kept) if wanted is None else set(wanted)
+    if not names <= set(_NORM_PARAMS):
+        raise ValueError(f"wanted names {sorted(names - set(_NORM_PARAMS))}, parameters are {_NORM_PARAMS}")
+    _same_device(h, h=h, stats=stats, y=y, grad_n=grad_n, grad_h=grad_h, **params)
+    keep = []
+
+    def rows(t):
+        r, stride = _rows(t)
+        keep.append(r)
+        return r.data_ptr(), stride
+
+    a.h, a.h_stride = rows(h)
+    out = {"x": torch.empty(h.shape, dtype=h.dtype, device=h.device)}
+    if y is not None:
+        a.y, a.y_stride = rows(y)
+        out["y"] = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        a.grad_y = out["y"].data_ptr()
+    if grad_n is not None:
+        a.grad_n, a.grad_n_stride = rows(grad_n)
+    if grad_h is not None:
+        a.grad_h, a.grad_h_stride = rows(grad_h)
+    a.grad_x, a.stats = out["x"].data_ptr(), stats.data_ptr()
+    for name in _NORM_PARAMS:
+        if name in names and name in kept:
+            out[name] = torch.empty(params[name].shape, dtype=params[name].dtype, device=h.device)
+            setattr(a, "grad_" + name, out[name].data_ptr())
+    ws_bytes = int(_lib.load().opus_residual_norm_grad_workspace_bytes(ctypes.byref(a)))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=h.device)
+    _call("opus_residual_norm_grad", h.device, ctypes.byref(a), _ptr(ws), ws_bytes)
+    return out
+
+
+# ------------------------------------------------ training step: gradient clip
+def _norm_kind(norm_type: float) -> int:
+    if norm_type == 2:
+        return 2
+    if norm_type == math.inf:
+        return 0
+    raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one run of memory without gaps, in whatever order of dimensions."""
+    if t.is_contiguous():
+        return True
+    run = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size == 1:
+            continue
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+def _tensor_list(tensors: torch.Tensor | Iterable[torch.Tensor], name: str) -> list[torch.Tensor]:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if tensors:
+        device = tensors[0].device
+        for t in tensors:
+            if t.dtype not in _TYPE_CODES or t.layout != torch.strided:
+                raise ValueError(f"{name} must be dense bfloat16, float16 or float32 tensors, got {t.dtype} {t.layout}")
+            if t.device != device:
+                raise ValueError(f"{name} are on {device} and {t.device}")
+    return tensors
+
+
+class _HostLists:
+    """Addresses, lengths and types of a list of tensors, as the host arrays of the C ABI."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        self.count = len(tensors)
+        self.ptrs = np.array([t.data_ptr() for t in tensors], dtype=np.int64)
+        self.numels = np.array([t.numel() for t in tensors], dtype=np.int64)
+        self.types = np.array([_TYPE_CODES[t.dtype] for t in tensors], dtype=np.int32)
+
+    def ranges(self) -> tuple[np.ndarray, np.ndarray]:
+        """Byte ranges of the tensors that have elements, sorted by their start."""
+        some = self.numels > 0
+        start = self.ptrs[some]
+        end = start + self.numels[some] * np.where(self.types[some] == _lib.DTYPE_F32, 4, 2)
+        order = np.argsort(start, kind="stable")
+        return start[order], end[order]
+
+
+def _p(a: np.ndarray) -> ctypes.c_void_p:
+    return ctypes.c_void_p(a.ctypes.data)
+
+
+def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """Norm of all elements of a list of tensors as one vector: a float32 scalar on their device.
+
+    norm_type 2 (square root of the sum of squares) or inf (largest
+    magnitude).  bf16, f16 and f32 tensors of any layout, mixed; an empty list
+    gives 0 (on the CPU, as torch does).  Nothing waits for the host.
+    """
+    grads = _tensor_list(grads, "grads")
+    kind = _norm_kind(norm_type)
+    if not grads:
+        return torch.tensor(0.0)
+    _cuda(grads[0], "grads")
+    grads = [t if _dense(t) else t.contiguous() for t in grads]
+    g = _HostLists(grads)
+    device = grads[0].device
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    ws = torch.empty(int(_lib.load().opus_grad_norm_workspace_bytes(g.count)), dtype=torch.uint8, device=device)
+    _call("opus_grad_norm", device, _p(g.ptrs), _p(g.numels), _p(g.types), g.count, kind, _ptr(ws), ws.numel(),
+          _ptr(norm))
+    return norm
+
+
+def _clip_targets(grads, out, name):
+    """(sources, targets, [(tensor, its dense copy)] to write back): in place without out."""
+    grads = _tensor_list(grads, "grads")
+    if out is None:
+        dense = [t if _dense(t) else t.contiguous() for t in grads]
+        back = [(t, c) for t, c in zip(grads, dense) if c is not t]
+        for t, _ in back:
+            if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                raise ValueError(f"{name}: a gradient's elements overlap in memory (an expanded tensor)")
+        return dense, dense, back
+    out = _tensor_list(out, "out")
+    if len(out) != len(grads) or any(o.shape != t.shape for o, t in zip(out, grads)):
+        raise ValueError(f"{name}: out must have a tensor of the same shape for each gradient")
+    if grads and out[0].device != grads[0].device:
+        raise ValueError(f"out is on {out[0].device}, grads on {grads[0].device}")
+    if not all(o.is_contiguous() for o in out):
+        raise ValueError(f"{name}: out must be contiguous tensors")
+    return [_contig(t) for t in grads], out, []
+
+
+def _check_overlap(g: _HostLists, o: _HostLists, name: str) -> None:
+    start, end = o.ranges()
+    if np.any(start[1:] < np.maximum.accumulate(end)[:-1]):
+        raise ValueError(f"{name}: a tensor is written twice (the same gradient, or overlapping ones, in the list)")
+    if g is not o and start.size:
+        g_start, g_end = g.ranges()
+        below = np.searchsorted(g_start, end)  # sources that start before each target ends
+        reach = np.concatenate([[0], np.maximum.accumulate(g_end)])
+        if np.any(reach[below] > start):
+            raise ValueError(f"{name}: out overlaps the gradients (leave it out to clip in place)")
+
+
+def clip_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+               out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
+    """Scale gradients so that their joint norm is at most max_norm; returns the norm they had.
+
+    The rule of torch.nn.utils.clip_grad_norm_: each gradient times
+    min(1, max_norm / (norm + 1e-6)), in place, or written to out (contiguous
+    tensors of the gradients' shapes and any of the types: 16-bit gradients
+    into an optimizer's float32 ones).  The factor is held in f32 and each
+    product rounded once.  Gradients whose norm is within the bound are not
+    written in place.  A NaN norm makes every gradient NaN.  The norm is a
+    float32 scalar on the device, and nothing waits for the host.
+    """
+    kind = _norm_kind(norm_type)
+    src, dst, back = _clip_targets(grads, out, "clip_grads")
+    if not src:
+        return torch.tensor(0.0)
+    g = _HostLists(src)
+    o = g if dst is src else _HostLists(dst)
+    _check_overlap(g, o, "clip_grads")
+    _cuda(src[0], "grads")
+    device = src[0].device
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    ws = torch.empty(int(_lib.load().opus_grad_norm_workspace_bytes(g.count)), dtype=torch.uint8, device=device)
+    _call("opus_clip_grads", device, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels), g.count, kind,
+          float(max_norm), _ptr(ws), ws.numel(), _ptr(norm))
+    for t, c in back:
+        t.copy_(c)
+    return norm
+
+
+def scale_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm: torch.Tensor,
+                out: Sequence[torch.Tensor] | None = None) -> None:
+    """The second half of clip_grads, for a norm that is known: joined over ranks that hold shards, say.
+
+    norm: a float32 scalar on the gradients' device.
+    """
+    src, dst, back = _clip_targets(grads, out, "scale_grads")
+    if norm.numel() != 1 or norm.dtype != torch.float32:
+        raise ValueError(f"norm must be a float32 scalar, got {norm.dtype} {tuple(norm.shape)}")
+    if not src:
+        return
+    g = _HostLists(src)
+    o = g if dst is src else _HostLists(dst)
+    _check_overlap(g, o, "scale_grads")
+    _same_device(src[0], grads=src[0], norm=norm)
+    _call("opus_scale_grads", src[0].device, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels), g.count,
+          float(max_norm), _ptr(norm))
+    for t, c in back:
+        t.copy_(c)

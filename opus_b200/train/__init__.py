@@ -7,6 +7,7 @@ from .data_selection import (
     initialize_projector,
     stochastic_greedy_selection,
 )
+from .grad_clip import clip_grad_norm_
 from .random_projection import GradientProjector
 
 __all__ = [
@@ -17,4 +18,5 @@ __all__ = [
     "greedy_selection",
     "stochastic_greedy_selection",
     "GradientProjector",
+    "clip_grad_norm_",
 ]
