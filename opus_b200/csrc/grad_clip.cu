@@ -16,9 +16,14 @@
 // in place, since c = 1 would write what is there.
 //
 // Layout: the list travels as a kernel parameter (addresses, lengths, types:
-// no copy to the device, and a captured graph holds its own), cut into chunks
-// that blocks take in turn; a block finds a chunk's tensor by bisection.
-#include <limits>
+// no copy to the device, and a captured graph holds its own).  Tensors are cut
+// into units of 2048 elements and every block takes one run of neighbouring
+// units, so blocks share the elements evenly and look a tensor up once.  The
+// scaling launch walks each block's run backwards: what the norm read last is
+// still in L2.
+#include <algorithm>
+#include <new>
+#include <vector>
 
 #include "elements.cuh"
 
@@ -27,29 +32,41 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlocksPerSm = 8;
-constexpr int64_t kChunk = 16384;  // elements
-constexpr int kMaxTensors = 1024;  // of one launch: its table stays below the 32764 bytes of parameters
+constexpr int64_t kUnit = 2048;   // elements
 constexpr float kNormEps = 1e-6f;  // as torch.nn.utils.clip_grad_norm_ has it
 
+// The tensors of one launch.  Most is 960 for long lists (below the 32764 bytes of parameters) and 64 for
+// short ones.
+template <int Most>
 struct GradTable {
-  const void* in[kMaxTensors];
-  void* out[kMaxTensors];
-  int64_t n[kMaxTensors];
-  int first_chunk[kMaxTensors];
-  uint8_t types[kMaxTensors];  // type in | type out << 4
+  const void* in[Most];
+  void* out[Most];
+  int64_t n[Most];
+  int64_t first[Most];  // number of the tensor's first unit
+  uint8_t types[Most];  // type in | type out << 4
   int count;
-  int chunks;
+  int in_place;  // every out is its in
+  int64_t units;
 };
-static_assert(sizeof(GradTable) <= 32000, "kernel parameters");
+constexpr int kShort = 64, kLong = 960;
+static_assert(sizeof(GradTable<kLong>) <= 32000, "kernel parameters");
 
-__device__ __forceinline__ int find_tensor(const GradTable& t, int chunk) {
+template <int Most>
+__device__ __forceinline__ int find_tensor(const GradTable<Most>& t, int64_t unit) {
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (t.first_chunk[mid] <= chunk) lo = mid;
+    if (t.first[mid] <= unit) lo = mid;
     else hi = mid - 1;
   }
   return lo;
+}
+
+// This block's run of units: [*a, *b).
+__device__ __forceinline__ void block_run(int64_t units, int64_t* a, int64_t* b) {
+  const int64_t each = units / gridDim.x, more = units % gridDim.x, k = blockIdx.x;
+  *a = k * each + (k < more ? k : more);
+  *b = *a + each + (k < more ? 1 : 0);
 }
 
 // Sum (kind 2) or maximum (kind 0: the infinity norm, NaN wins) of doubles.
@@ -93,31 +110,31 @@ __device__ __forceinline__ double group_part(const float (&x)[N], int kind) {
 }
 
 template <typename T>
-__device__ double chunk_part(const T* p, int n, int kind) {
+__device__ double run_part(const T* p, int64_t n, int kind) {
   constexpr int V = 16 / sizeof(T);
   constexpr int U = 4;
   double acc = 0.0;
-  int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T));
+  int64_t head = static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T));
   head = head < n ? head : n;
-  const int vecs = (n - head) / V;
+  const int64_t vecs = (n - head) / V;
   const T* body = p + head;
-  for (int b = threadIdx.x; b < vecs; b += kThreads * U) {
+  for (int64_t b = threadIdx.x; b < vecs; b += kThreads * U) {
     float x[U * V];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float r[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) r[i] = 0.f;
-      if (b + u * kThreads < vecs) load_vec<T, V>(body + static_cast<int64_t>(b + u * kThreads) * V, r);
+      if (b + u * kThreads < vecs) load_vec<T, V>(body + (b + u * kThreads) * V, r);
 #pragma unroll
       for (int i = 0; i < V; ++i) x[u * V + i] = r[i];
     }
     acc = join(acc, group_part(x, kind), kind);
   }
   // the up to V - 1 elements before the first 16-byte boundary and after the last
-  const int tail = head + vecs * V;
-  const int i = static_cast<int>(threadIdx.x);
-  const int at = i < head ? i : tail + (i - head);
+  const int64_t tail = head + vecs * V;
+  const int64_t i = threadIdx.x;
+  const int64_t at = i < head ? i : tail + (i - head);
   if (at < n) {
     const float x[1] = {to_f32(p[at])};
     acc = join(acc, group_part(x, kind), kind);
@@ -125,19 +142,23 @@ __device__ double chunk_part(const T* p, int n, int kind) {
   return acc;
 }
 
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ GradTable t, int kind,
+template <int Most>
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ GradTable<Most> t, int kind,
                                                         double* __restrict__ partial) {
   double acc = 0.0;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const int j = find_tensor(t, c);
-    const int64_t at = static_cast<int64_t>(c - t.first_chunk[j]) * kChunk;
-    const int n = static_cast<int>(t.n[j] - at < kChunk ? t.n[j] - at : kChunk);
+  int64_t u, last;
+  block_run(t.units, &u, &last);
+  for (int j = find_tensor(t, u); u < last; ++j) {
+    const int64_t stop = j + 1 < t.count && t.first[j + 1] < last ? t.first[j + 1] : last;
+    const int64_t at = (u - t.first[j]) * kUnit;
+    const int64_t n = t.n[j] - at < (stop - u) * kUnit ? t.n[j] - at : (stop - u) * kUnit;
     const int type = t.types[j] & 15;
     double d;
-    if (type == OPUS_DTYPE_F32) d = chunk_part(static_cast<const float*>(t.in[j]) + at, n, kind);
-    else if (type == OPUS_DTYPE_F16) d = chunk_part(static_cast<const __half*>(t.in[j]) + at, n, kind);
-    else d = chunk_part(static_cast<const __nv_bfloat16*>(t.in[j]) + at, n, kind);
+    if (type == OPUS_DTYPE_F32) d = run_part(static_cast<const float*>(t.in[j]) + at, n, kind);
+    else if (type == OPUS_DTYPE_F16) d = run_part(static_cast<const __half*>(t.in[j]) + at, n, kind);
+    else d = run_part(static_cast<const __nv_bfloat16*>(t.in[j]) + at, n, kind);
     acc = join(acc, d, kind);
+    u = stop;
   }
   acc = block_join(acc, kind);
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
@@ -158,45 +179,41 @@ __global__ void __launch_bounds__(kThreads) norm_join_kernel(const double* __res
   if (threadIdx.x == 0) *norm = n;
 }
 
+// From the run's end to its start.
 template <typename TI, typename TO>
-__device__ void chunk_scale(const TI* p, TO* q, int n, float c) {
+__device__ void run_scale(const TI* p, TO* q, int64_t n, float c) {
   constexpr int V = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));
-  constexpr int U = 4;
-  int head = static_cast<int>((V * sizeof(TI) - (reinterpret_cast<uintptr_t>(p) & (V * sizeof(TI) - 1))) &
-                              (V * sizeof(TI) - 1)) / static_cast<int>(sizeof(TI));
+  constexpr int U = 64 / (V * sizeof(TI));  // 64 bytes of loads a thread in flight
+  constexpr uintptr_t in_mask = V * sizeof(TI) - 1, out_mask = V * sizeof(TO) - 1;
+  int64_t head = static_cast<int64_t>((V * sizeof(TI) - (reinterpret_cast<uintptr_t>(p) & in_mask)) & in_mask) /
+                 static_cast<int>(sizeof(TI));
   head = head < n ? head : n;
-  // both sides reach their boundaries together, or the chunk goes element by element
-  if ((reinterpret_cast<uintptr_t>(q + head) & (V * sizeof(TO) - 1)) != 0) head = n;
-  const int vecs = (n - head) / V;
-  for (int b = threadIdx.x; b < vecs; b += kThreads * U) {
+  // both sides reach their boundaries together, or the run goes element by element
+  if ((reinterpret_cast<uintptr_t>(q + head) & out_mask) != 0) head = n;
+  const int64_t vecs = (n - head) / V;
+  const int64_t tail = head + vecs * V;
+  for (int64_t i = threadIdx.x; i < head + (n - tail); i += kThreads) {
+    const int64_t at = i < head ? i : tail + (i - head);
+    q[at] = from_f32<TO>(to_f32(p[at]) * c);
+  }
+  for (int64_t b = vecs - 1 - threadIdx.x; b >= 0; b -= kThreads * U) {
     float x[U][V];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (b + u * kThreads < vecs) load_vec<TI, V>(p + head + static_cast<int64_t>(b + u * kThreads) * V, x[u]);
+      if (b - u * kThreads >= 0) load_vec<TI, V>(p + head + (b - u * kThreads) * V, x[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (b + u * kThreads < vecs) {
+      if (b - u * kThreads >= 0) {
 #pragma unroll
         for (int i = 0; i < V; ++i) x[u][i] *= c;
-        store_vec<TO, V>(q + head + static_cast<int64_t>(b + u * kThreads) * V, x[u]);
+        store_vec<TO, V>(q + head + (b - u * kThreads) * V, x[u]);
       }
   }
-  const int tail = head + vecs * V;
-  for (int i = threadIdx.x; i < head + (n - tail); i += kThreads) {
-    const int at = i < head ? i : tail + (i - head);
-    q[at] = from_f32<TO>(to_f32(p[at]) * c);
-  }
-}
-
-template <typename TI>
-__device__ void chunk_scale_to(const TI* p, void* q, int64_t at, int type, int n, float c) {
-  if (type == OPUS_DTYPE_F32) chunk_scale(p, static_cast<float*>(q) + at, n, c);
-  else if (type == OPUS_DTYPE_F16) chunk_scale(p, static_cast<__half*>(q) + at, n, c);
-  else chunk_scale(p, static_cast<__nv_bfloat16*>(q) + at, n, c);
 }
 
 // parts > 0: the norm is joined from partial sums here (and block 0 writes it); otherwise it is read.
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ GradTable t, int kind,
+template <typename TI, typename TO, int Most>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ GradTable<Most> t, int kind,
                                                          const double* __restrict__ partial, int parts,
                                                          float max_norm, float* __restrict__ norm) {
   float n;
@@ -208,15 +225,15 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
   }
   float c = max_norm / (n + kNormEps);
   c = c > 1.0f ? 1.0f : c;  // a NaN stays
-  for (int k = blockIdx.x; k < t.chunks; k += gridDim.x) {
-    const int j = find_tensor(t, k);
-    if (c == 1.0f && t.in[j] == t.out[j]) continue;  // in place: there already
-    const int64_t at = static_cast<int64_t>(k - t.first_chunk[j]) * kChunk;
-    const int len = static_cast<int>(t.n[j] - at < kChunk ? t.n[j] - at : kChunk);
-    const int type = t.types[j] & 15, to = t.types[j] >> 4;
-    if (type == OPUS_DTYPE_F32) chunk_scale_to(static_cast<const float*>(t.in[j]) + at, t.out[j], at, to, len, c);
-    else if (type == OPUS_DTYPE_F16) chunk_scale_to(static_cast<const __half*>(t.in[j]) + at, t.out[j], at, to, len, c);
-    else chunk_scale_to(static_cast<const __nv_bfloat16*>(t.in[j]) + at, t.out[j], at, to, len, c);
+  if (c == 1.0f && t.in_place) return;
+  int64_t first, u;
+  block_run(t.units, &first, &u);
+  for (int j = find_tensor(t, u - 1); u > first; --j) {
+    const int64_t from = t.first[j] > first ? t.first[j] : first;
+    const int64_t at = (from - t.first[j]) * kUnit;
+    const int64_t len = t.n[j] - at < (u - from) * kUnit ? t.n[j] - at : (u - from) * kUnit;
+    run_scale(static_cast<const TI*>(t.in[j]) + at, static_cast<TO*>(t.out[j]) + at, len, c);
+    u = from;
   }
 }
 
@@ -229,11 +246,13 @@ struct Lists {
   int count;
 };
 
+constexpr int64_t kMostElements = int64_t{1} << 48;
+
 int check_lists(const char* what, const Lists& l, bool outs) {
   if (l.count < 0) return set_error(OPUS_ERR_INVALID, "%s: %d tensors", what, l.count);
   if (l.count > 0 && (!l.in || !l.n || !l.in_types || (outs && (!l.out || !l.out_types))))
     return set_error(OPUS_ERR_INVALID, "%s: NULL list", what);
-  int64_t chunks = 0;
+  int64_t whole = 0;
   for (int i = 0; i < l.count; ++i) {
     if (l.n[i] < 0) return set_error(OPUS_ERR_INVALID, "%s: tensor %d has %lld elements", what, i, (long long)l.n[i]);
     if (!dtype_ok(l.in_types[i]) || (outs && !dtype_ok(l.out_types[i])))
@@ -243,47 +262,81 @@ int check_lists(const char* what, const Lists& l, bool outs) {
     if (reinterpret_cast<uintptr_t>(l.in[i]) % dtype_bytes(l.in_types[i]) != 0 ||
         (outs && reinterpret_cast<uintptr_t>(l.out[i]) % dtype_bytes(l.out_types[i]) != 0))
       return set_error(OPUS_ERR_INVALID, "%s: tensor %d is not aligned to its elements", what, i);
-    chunks += l.n[i] / kChunk + 1;
-    if (l.n[i] > std::numeric_limits<int64_t>::max() / 8 || chunks > std::numeric_limits<int>::max() / 2)
+    if (l.n[i] <= kMostElements) whole += l.n[i];
+    if (l.n[i] > kMostElements || whole > kMostElements)
       return set_error(OPUS_ERR_UNSUPPORTED, "%s: the list is too long", what);
   }
   return OPUS_OK;
 }
 
-// Tensors [at, ...) of the list as one launch's table; returns the index of the first that did not fit.
-int fill_table(const Lists& l, int at, GradTable* t) {
+// Refuses a list that writes an element twice or writes what it reads elsewhere (outs[j] == grads[j] aside).
+int check_overlap(const char* what, const Lists& l) {
+  struct Range {
+    uintptr_t start, end;
+    bool written;
+  };
+  try {
+    std::vector<Range> r;
+    r.reserve(2 * static_cast<size_t>(l.count));
+    for (int i = 0; i < l.count; ++i) {
+      if (l.n[i] == 0) continue;
+      const uintptr_t in = reinterpret_cast<uintptr_t>(l.in[i]), out = reinterpret_cast<uintptr_t>(l.out[i]);
+      const bool in_place = in == out && l.in_types[i] == l.out_types[i];
+      if (!in_place) r.push_back({in, in + l.n[i] * dtype_bytes(l.in_types[i]), false});
+      r.push_back({out, out + l.n[i] * dtype_bytes(l.out_types[i]), true});
+    }
+    std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.start < b.start; });
+    uintptr_t read = 0, written = 0;  // how far the ranges so far reach
+    for (const Range& x : r) {
+      if (x.start < written || (x.written && x.start < read))
+        return set_error(OPUS_ERR_INVALID, "%s: an element would be written twice, or written and read elsewhere "
+                         "(a tensor listed twice, overlapping views, or outputs that overlap the inputs)", what);
+      uintptr_t& reach = x.written ? written : read;
+      reach = x.end > reach ? x.end : reach;
+    }
+  } catch (const std::bad_alloc&) {
+    return set_error(OPUS_ERR_INVALID, "%s: no host memory for %d tensors", what, l.count);
+  }
+  return OPUS_OK;
+}
+
+// Tensors [at, ...) of the list as one launch's table, those of one pair of types when asked for; returns
+// the index of the first that did not fit.
+template <int Most>
+int fill_table(const Lists& l, int at, int types, GradTable<Most>* t) {
   t->count = 0;
-  int64_t chunks = 0;
-  for (; at < l.count && t->count < kMaxTensors; ++at) {
-    if (l.n[at] == 0) continue;
+  t->in_place = 1;
+  t->units = 0;
+  for (; at < l.count && t->count < Most; ++at) {
+    const int pair = l.in_types[at] | (l.out ? l.out_types[at] << 4 : 0);
+    if (l.n[at] == 0 || (types >= 0 && types != pair)) continue;
     const int k = t->count++;
     t->in[k] = l.in[at];
     t->out[k] = l.out ? l.out[at] : nullptr;
+    t->in_place &= t->in[k] == t->out[k];
     t->n[k] = l.n[at];
-    t->first_chunk[k] = static_cast<int>(chunks);
-    t->types[k] = static_cast<uint8_t>(l.in_types[at] | (l.out ? l.out_types[at] << 4 : 0));
-    chunks += (l.n[at] + kChunk - 1) / kChunk;
+    t->first[k] = t->units;
+    t->types[k] = static_cast<uint8_t>(pair);
+    t->units += (l.n[at] + kUnit - 1) / kUnit;
   }
-  t->chunks = static_cast<int>(chunks);
   return at;
 }
 
-int grid_of(const GradTable& t) {
-  const int most = sm_count() * kBlocksPerSm;
-  return t.chunks < most ? t.chunks : most;
+int grid_of(int64_t units) {
+  const int64_t most = static_cast<int64_t>(sm_count()) * kBlocksPerSm;
+  return static_cast<int>(units < most ? units : most);
 }
 
-int launches_of(int count) { return (count + kMaxTensors - 1) / kMaxTensors; }
-
 // Partial sums of every launch side by side; *parts is their number.
+template <int Most>
 int launch_norm(const Lists& l, int kind, double* partial, int* parts, cudaStream_t st) {
-  GradTable t;
+  GradTable<Most> t;
   *parts = 0;
   for (int at = 0; at < l.count;) {
-    at = fill_table(l, at, &t);
-    if (t.chunks == 0) continue;
-    const int grid = grid_of(t);
-    norm_kernel<<<grid, kThreads, 0, st>>>(t, kind, partial + *parts);
+    at = fill_table(l, at, -1, &t);
+    if (t.units == 0) continue;
+    const int grid = grid_of(t.units);
+    norm_kernel<Most><<<grid, kThreads, 0, st>>>(t, kind, partial + *parts);
     note_launch();
     OPUS_CUDA_TRY(cudaGetLastError());
     *parts += grid;
@@ -291,17 +344,54 @@ int launch_norm(const Lists& l, int kind, double* partial, int* parts, cudaStrea
   return OPUS_OK;
 }
 
-int launch_scale(const Lists& l, int kind, const double* partial, int parts, float max_norm, float* norm,
-                 cudaStream_t st) {
-  GradTable t;
+template <typename TI, typename TO, int Most>
+int launch_scale_pair(const Lists& l, int types, int kind, const double* partial, int parts, float max_norm,
+                      float* norm, cudaStream_t st) {
+  GradTable<Most> t;
   for (int at = 0; at < l.count;) {
-    at = fill_table(l, at, &t);
-    if (t.chunks == 0) continue;
-    scale_kernel<<<grid_of(t), kThreads, 0, st>>>(t, kind, partial, parts, max_norm, norm);
+    at = fill_table(l, at, types, &t);
+    if (t.units == 0) continue;
+    scale_kernel<TI, TO, Most><<<grid_of(t.units), kThreads, 0, st>>>(t, kind, partial, parts, max_norm, norm);
     note_launch();
     OPUS_CUDA_TRY(cudaGetLastError());
   }
   return OPUS_OK;
+}
+
+// One launch for each pair of types in the list (a kernel of all nine pairs takes 238 registers and ran at a
+// quarter of the bandwidth).
+template <int Most>
+int launch_scale_most(const Lists& l, int kind, const double* partial, int parts, float max_norm, float* norm,
+                      cudaStream_t st) {
+  unsigned seen[3] = {0, 0, 0};
+  for (int i = 0; i < l.count; ++i)
+    if (l.n[i] > 0) seen[l.in_types[i]] |= 1u << l.out_types[i];
+  int rc = OPUS_OK;
+#define OPUS_SCALE_PAIR(A, TA, B, TB)          \
+  if (rc == OPUS_OK && (seen[A] & (1u << B)))  \
+    rc = launch_scale_pair<TA, TB, Most>(l, A | B << 4, kind, partial, parts, max_norm, norm, st)
+  OPUS_SCALE_PAIR(OPUS_DTYPE_BF16, __nv_bfloat16, OPUS_DTYPE_BF16, __nv_bfloat16);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_BF16, __nv_bfloat16, OPUS_DTYPE_F32, float);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_BF16, __nv_bfloat16, OPUS_DTYPE_F16, __half);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_F32, float, OPUS_DTYPE_BF16, __nv_bfloat16);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_F32, float, OPUS_DTYPE_F32, float);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_F32, float, OPUS_DTYPE_F16, __half);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_F16, __half, OPUS_DTYPE_BF16, __nv_bfloat16);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_F16, __half, OPUS_DTYPE_F32, float);
+  OPUS_SCALE_PAIR(OPUS_DTYPE_F16, __half, OPUS_DTYPE_F16, __half);
+#undef OPUS_SCALE_PAIR
+  return rc;
+}
+
+int launch_norm(const Lists& l, int kind, double* partial, int* parts, cudaStream_t st) {
+  return l.count <= kShort ? launch_norm<kShort>(l, kind, partial, parts, st)
+                           : launch_norm<kLong>(l, kind, partial, parts, st);
+}
+
+int launch_scale(const Lists& l, int kind, const double* partial, int parts, float max_norm, float* norm,
+                 cudaStream_t st) {
+  return l.count <= kShort ? launch_scale_most<kShort>(l, kind, partial, parts, max_norm, norm, st)
+                           : launch_scale_most<kLong>(l, kind, partial, parts, max_norm, norm, st);
 }
 
 int launch_join(const double* partial, int parts, int kind, float* norm, cudaStream_t st) {
@@ -328,7 +418,8 @@ int check_norm_args(const char* what, int kind, const void* workspace, int64_t b
 using namespace opus;
 
 extern "C" int64_t opus_grad_norm_workspace_bytes(int count) {
-  return static_cast<int64_t>(launches_of(count > 0 ? count : 1)) * sm_count() * kBlocksPerSm * 8;
+  const int64_t launches = count > kLong ? (count + kLong - 1) / kLong : 1;
+  return launches * sm_count() * kBlocksPerSm * 8;
 }
 
 extern "C" int opus_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int count,
@@ -350,6 +441,7 @@ extern "C" int opus_scale_grads(const void* const* grads, const int* dtypes, voi
                                 const int64_t* numels, int count, float max_norm, const float* norm, void* stream) {
   const Lists l{grads, outs, numels, dtypes, out_dtypes, count};
   int rc = check_lists("scale_grads", l, true);
+  if (rc == OPUS_OK) rc = check_overlap("scale_grads", l);
   if (rc) return rc;
   if (!norm) return set_error(OPUS_ERR_INVALID, "scale_grads: NULL pointer");
   return launch_scale(l, 2, nullptr, 0, max_norm, const_cast<float*>(norm), reinterpret_cast<cudaStream_t>(stream));
@@ -360,6 +452,7 @@ extern "C" int opus_clip_grads(const void* const* grads, const int* dtypes, void
                                int64_t workspace_bytes, float* norm, void* stream) {
   const Lists l{grads, outs, numels, dtypes, out_dtypes, count};
   int rc = check_lists("clip_grads", l, true);
+  if (rc == OPUS_OK) rc = check_overlap("clip_grads", l);
   if (rc) return rc;
   rc = check_norm_args("clip_grads", norm_kind, workspace, workspace_bytes, count, norm);
   if (rc) return rc;

@@ -8,9 +8,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from collections.abc import Iterable, Sequence
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -935,38 +935,37 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _tensor_list(tensors: torch.Tensor | Iterable[torch.Tensor], name: str) -> list[torch.Tensor]:
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if tensors:
-        device = tensors[0].device
-        for t in tensors:
-            if t.dtype not in _TYPE_CODES or t.layout != torch.strided:
-                raise ValueError(f"{name} must be dense bfloat16, float16 or float32 tensors, got {t.dtype} {t.layout}")
-            if t.device != device:
-                raise ValueError(f"{name} are on {device} and {t.device}")
-    return tensors
+class _TensorList:
+    """Strided tensors of the three types on one device, and their addresses, lengths and types as the host arrays
+    of the C ABI.  A tensor whose elements do not fill one run of memory is copied (tensors), and named in copied."""
 
-
-class _HostLists:
-    """Addresses, lengths and types of a list of tensors, as the host arrays of the C ABI."""
-
-    def __init__(self, tensors: Sequence[torch.Tensor]):
+    def __init__(self, tensors: torch.Tensor | Iterable[torch.Tensor], name: str, contiguous: bool = False):
+        tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
         self.count = len(tensors)
-        self.ptrs = np.array([t.data_ptr() for t in tensors], dtype=np.int64)
-        self.numels = np.array([t.numel() for t in tensors], dtype=np.int64)
-        self.types = np.array([_TYPE_CODES[t.dtype] for t in tensors], dtype=np.int32)
+        dtypes = {t.dtype for t in tensors}
+        if not dtypes <= _TYPE_CODES.keys():
+            raise ValueError(f"{name} must be bfloat16, float16 or float32 tensors, got {dtypes - _TYPE_CODES.keys()}")
+        if {t.layout for t in tensors} - {torch.strided}:
+            raise ValueError(f"{name} must be dense tensors")
+        devices = set(map(torch.Tensor.get_device, tensors))
+        if len(devices) > 1:
+            raise ValueError(f"{name} are on several devices: {sorted({str(t.device) for t in tensors})}")
+        self.device_index = devices.pop() if devices else -1
+        self.copied = []
+        if not all(map(torch.Tensor.is_contiguous, tensors)):
+            for i, t in enumerate(tensors):
+                if not (t.is_contiguous() if contiguous else _dense(t)):
+                    self.copied.append(t)
+                    tensors[i] = t.contiguous()
+        self.tensors = tensors
+        self.ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
+        self.numels = array("q", map(torch.Tensor.numel, tensors))
+        self.types = array("i", [_TYPE_CODES[t.dtype] for t in tensors] if len(dtypes) > 1 else
+                           [_TYPE_CODES[t] for t in dtypes] * self.count)
 
-    def ranges(self) -> tuple[np.ndarray, np.ndarray]:
-        """Byte ranges of the tensors that have elements, sorted by their start."""
-        some = self.numels > 0
-        start = self.ptrs[some]
-        end = start + self.numels[some] * np.where(self.types[some] == _lib.DTYPE_F32, 4, 2)
-        order = np.argsort(start, kind="stable")
-        return start[order], end[order]
 
-
-def _p(a: np.ndarray) -> ctypes.c_void_p:
-    return ctypes.c_void_p(a.ctypes.data)
+def _p(a: array) -> ctypes.c_void_p:
+    return ctypes.c_void_p(a.buffer_info()[0])
 
 
 def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
@@ -976,14 +975,11 @@ def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2
     magnitude).  bf16, f16 and f32 tensors of any layout, mixed; an empty list
     gives 0 (on the CPU, as torch does).  Nothing waits for the host.
     """
-    grads = _tensor_list(grads, "grads")
     kind = _norm_kind(norm_type)
-    if not grads:
+    g = _TensorList(grads, "grads")
+    if not g.count:
         return torch.tensor(0.0)
-    _cuda(grads[0], "grads")
-    grads = [t if _dense(t) else t.contiguous() for t in grads]
-    g = _HostLists(grads)
-    device = grads[0].device
+    device = _cuda(g.tensors[0], "grads").device
     norm = torch.empty((), dtype=torch.float32, device=device)
     ws = torch.empty(int(_lib.load().opus_grad_norm_workspace_bytes(g.count)), dtype=torch.uint8, device=device)
     _call("opus_grad_norm", device, _p(g.ptrs), _p(g.numels), _p(g.types), g.count, kind, _ptr(ws), ws.numel(),
@@ -991,36 +987,25 @@ def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2
     return norm
 
 
-def _clip_targets(grads, out, name):
-    """(sources, targets, [(tensor, its dense copy)] to write back): in place without out."""
-    grads = _tensor_list(grads, "grads")
+def _clip_targets(grads, out, name: str) -> tuple[_TensorList, _TensorList, list]:
+    """(sources, targets, [(gradient, its dense copy)] to write back): in place without out."""
     if out is None:
-        dense = [t if _dense(t) else t.contiguous() for t in grads]
-        back = [(t, c) for t, c in zip(grads, dense) if c is not t]
-        for t, _ in back:
-            if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+        g = _TensorList(grads, "grads")
+        if not g.copied:
+            return g, g, []
+        for t in g.copied:
+            if any(stride == 0 and size > 1 for stride, size in zip(t.stride(), t.shape)):
                 raise ValueError(f"{name}: a gradient's elements overlap in memory (an expanded tensor)")
-        return dense, dense, back
-    out = _tensor_list(out, "out")
-    if len(out) != len(grads) or any(o.shape != t.shape for o, t in zip(out, grads)):
-        raise ValueError(f"{name}: out must have a tensor of the same shape for each gradient")
-    if grads and out[0].device != grads[0].device:
-        raise ValueError(f"out is on {out[0].device}, grads on {grads[0].device}")
-    if not all(o.is_contiguous() for o in out):
+        return g, g, [(t, c) for t, c in zip(grads, g.tensors) if t is not c]
+    g, o = _TensorList(grads, "grads", contiguous=True), _TensorList(out, "out")
+    if o.copied or not all(map(torch.Tensor.is_contiguous, o.tensors)):
         raise ValueError(f"{name}: out must be contiguous tensors")
-    return [_contig(t) for t in grads], out, []
-
-
-def _check_overlap(g: _HostLists, o: _HostLists, name: str) -> None:
-    start, end = o.ranges()
-    if np.any(start[1:] < np.maximum.accumulate(end)[:-1]):
-        raise ValueError(f"{name}: a tensor is written twice (the same gradient, or overlapping ones, in the list)")
-    if g is not o and start.size:
-        g_start, g_end = g.ranges()
-        below = np.searchsorted(g_start, end)  # sources that start before each target ends
-        reach = np.concatenate([[0], np.maximum.accumulate(g_end)])
-        if np.any(reach[below] > start):
-            raise ValueError(f"{name}: out overlaps the gradients (leave it out to clip in place)")
+    if g.numels != o.numels:
+        raise ValueError(f"{name}: out must have a tensor of as many elements for each gradient")
+    if g.count and g.device_index != o.device_index:
+        raise ValueError(f"{name}: out and grads are on different devices")
+    return g, o, []
 
 
 def clip_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
@@ -1029,21 +1014,19 @@ def clip_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, no
 
     The rule of torch.nn.utils.clip_grad_norm_: each gradient times
     min(1, max_norm / (norm + 1e-6)), in place, or written to out (contiguous
-    tensors of the gradients' shapes and any of the types: 16-bit gradients
+    tensors of the gradients' sizes and any of the types: 16-bit gradients
     into an optimizer's float32 ones).  The factor is held in f32 and each
     product rounded once.  Gradients whose norm is within the bound are not
-    written in place.  A NaN norm makes every gradient NaN.  The norm is a
+    written in place.  A list that would write an element twice (a gradient
+    listed twice, overlapping views, an out that overlaps the gradients) is
+    refused.  A NaN norm makes every gradient NaN.  The norm is a
     float32 scalar on the device, and nothing waits for the host.
     """
     kind = _norm_kind(norm_type)
-    src, dst, back = _clip_targets(grads, out, "clip_grads")
-    if not src:
+    g, o, back = _clip_targets(grads, out, "clip_grads")
+    if not g.count:
         return torch.tensor(0.0)
-    g = _HostLists(src)
-    o = g if dst is src else _HostLists(dst)
-    _check_overlap(g, o, "clip_grads")
-    _cuda(src[0], "grads")
-    device = src[0].device
+    device = _cuda(g.tensors[0], "grads").device
     norm = torch.empty((), dtype=torch.float32, device=device)
     ws = torch.empty(int(_lib.load().opus_grad_norm_workspace_bytes(g.count)), dtype=torch.uint8, device=device)
     _call("opus_clip_grads", device, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels), g.count, kind,
@@ -1059,16 +1042,13 @@ def scale_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, n
 
     norm: a float32 scalar on the gradients' device.
     """
-    src, dst, back = _clip_targets(grads, out, "scale_grads")
+    g, o, back = _clip_targets(grads, out, "scale_grads")
     if norm.numel() != 1 or norm.dtype != torch.float32:
         raise ValueError(f"norm must be a float32 scalar, got {norm.dtype} {tuple(norm.shape)}")
-    if not src:
+    if not g.count:
         return
-    g = _HostLists(src)
-    o = g if dst is src else _HostLists(dst)
-    _check_overlap(g, o, "scale_grads")
-    _same_device(src[0], grads=src[0], norm=norm)
-    _call("opus_scale_grads", src[0].device, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels), g.count,
-          float(max_norm), _ptr(norm))
+    _same_device(g.tensors[0], grads=g.tensors[0], norm=norm)
+    _call("opus_scale_grads", g.tensors[0].device, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels),
+          g.count, float(max_norm), _ptr(norm))
     for t, c in back:
         t.copy_(c)

@@ -630,6 +630,26 @@ def test_scale_grads_with_a_joined_norm():
     assert whole > 1 and after <= 1.0 * (1 + 2 * half_step(torch.bfloat16))
 
 
+def test_clip_grads_refuses_what_it_would_write_twice():
+    a, b = torch.ones(600, device=DEV), torch.ones(40, device=DEV)
+    p = torch.nn.Parameter(torch.zeros(3, device=DEV))
+    p.grad = torch.ones(3, device=DEV)
+    for grads, out in (([a, b, a], None), ([a[:4], a[3:]], None), ([a[1:2], a], None), ([a, b], [torch.empty_like(a), b[:]]),
+                       ([a[:300]], [a[299:599]])):
+        if out is not None and out[-1].data_ptr() == b.data_ptr():
+            ops.clip_grads(grads, 1e9, out=out)  # one member in place and another not: allowed
+            continue
+        with pytest.raises(ValueError, match="twice"):
+            ops.clip_grads(grads, 1.0, out=out)
+        with pytest.raises(ValueError, match="twice"):
+            ops.scale_grads(grads, 1.0, torch.ones((), device=DEV), out=out)
+    with pytest.raises(ValueError, match="twice"):
+        clip_grad_norm_([p, p], 1.0)
+    assert bool((a == 1).all()) and bool((b == 1).all()) and bool((p.grad == 1).all())
+    assert float(ops.grad_norm([b, b])) == float(np.float32(80 ** 0.5))  # reading twice is fine
+    assert float(ops.clip_grads([a[:300], a[300:]], 1.0)) > 1  # neighbours share no element
+
+
 def test_clip_grads_beyond_32_bit_offsets():
     n = (1 << 31) + 12345
     t = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
