@@ -21,23 +21,91 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 
-// V elements of T in one access of at most 16 bytes (V * sizeof(T) a power of two).
+// Two 16-bit elements in a word, low half first.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// V elements of T in one access of at most 16 bytes (V * sizeof(T) a power of two), kept as words: taking 16-bit
+// elements apart one by one costs several instructions each.
 template <typename T, int V>
 struct alignas(V * sizeof(T)) Vec {
-  T v[V];
+  uint32_t w[V / 2];
+  __device__ __forceinline__ void get(float (&r)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 f = unpack2<T>(w[i]);
+      r[2 * i] = f.x, r[2 * i + 1] = f.y;
+    }
+  }
+  __device__ __forceinline__ void set(const float (&r)[V]) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = pack2<T>(r[2 * i], r[2 * i + 1]);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = 0u;
+  }
+};
+template <int V>
+struct alignas(V * 4) Vec<float, V> {
+  float w[V];
+  __device__ __forceinline__ void get(float (&r)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = w[i];
+  }
+  __device__ __forceinline__ void set(const float (&r)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = r[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = 0.f;
+  }
+};
+template <typename T>
+struct Vec<T, 1> {
+  T w;
+  __device__ __forceinline__ void get(float (&r)[1]) const { r[0] = to_f32(w); }
+  __device__ __forceinline__ void set(const float (&r)[1]) { w = from_f32<T>(r[0]); }
+  __device__ __forceinline__ void zero() { w = from_f32<T>(0.f); }
+};
+template <>
+struct Vec<float, 1> {
+  float w;
+  __device__ __forceinline__ void get(float (&r)[1]) const { r[0] = w; }
+  __device__ __forceinline__ void set(const float (&r)[1]) { w = r[0]; }
+  __device__ __forceinline__ void zero() { w = 0.f; }
 };
 
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float (&r)[V]) {
   const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) r[i] = to_f32(x.v[i]);
+  x.get(r);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&r)[V]) {
   Vec<T, V> x;
-#pragma unroll
-  for (int i = 0; i < V; ++i) x.v[i] = from_f32<T>(r[i]);
+  x.set(r);
   *reinterpret_cast<Vec<T, V>*>(p) = x;
 }
 

@@ -40,136 +40,198 @@ int check_norm(const char* what, const opus_residual_norm_args* a) {
   return OPUS_OK;
 }
 
-// The launch's shape for vectors of V elements: as few vectors a thread as keep a row within 512 threads
-// (more warps of one row hide its loads better than more loads of one warp), up to 1024 for the widest rows.
-int norm_shape(const char* what, const opus_residual_norm_args* a, bool vec, int V, NormShape* s, int* nv) {
-  if (!vec) V = 1;
+// Vector loads of the parameters need their arrays on 16-byte boundaries.
+bool norm_params_aligned(const opus_residual_norm_args* a) {
+  const void* p[5] = {a->weight, a->bias, a->post_weight, a->post_bias, a->gate};
+  for (const void* q : p)
+    if (reinterpret_cast<uintptr_t>(q) % 16 != 0) return false;
+  return true;
+}
+
+// The launch's shape for vectors of V elements, at most `most` of them (a power of two) a thread: as few threads
+// a row as that allows, and as few vectors a thread as those threads need.
+int norm_shape(const char* what, const opus_residual_norm_args* a, int V, int most, NormShape* s, int* nv) {
   const int full = (a->d + V - 1) / V;
-  const int steps[3] = {V == 1 ? 4 : 1, V == 1 ? 16 : 2, V == 1 ? 16 : 4};
-  int k = 0;
-  while (k < 2 && (full + steps[k] - 1) / steps[k] > 512) ++k;
-  if (V == 8 && k == 2) k = 1;
-  *nv = steps[k];
-  int need = (full + *nv - 1) / *nv;
   int group = 1;
-  if (need <= 32) {
-    while (group < need) group <<= 1;
-  } else {
-    group = (need + 31) / 32 * 32;
-  }
+  while (group < 32 && group * most < full) group <<= 1;
+  if (group * most < full) group = ((full + most - 1) / most + 31) / 32 * 32;
+  // rows of less than a warp: a vector for each lane, so that its loads are neighbours
+  while (group < 32 && group < full) group <<= 1;
   if (group > kNormMaxThreads) return set_error(OPUS_ERR_UNSUPPORTED, "%s: d = %d is too wide", what, a->d);
+  int k = 1;
+  while (k * group < full) k <<= 1;
+  *nv = k;
   s->rows = a->rows;
-  s->seq = a->gate != nullptr && a->gate_rows > 0 ? a->rows / a->gate_rows : a->rows;
+  s->seq = a->gate != nullptr && a->gate_rows > 1 ? a->rows / a->gate_rows : a->rows;
   if (s->seq < 1) s->seq = 1;
   s->d = a->d;
   s->group = group;
   s->groups = group >= 256 ? 1 : 256 / group;
   s->layer = a->kind;
   s->eps = a->eps;
+  s->blocks = 0;
   return OPUS_OK;
 }
 
 namespace {
 
-template <typename TX, typename TY, int V, int NV>
-__global__ void __launch_bounds__(norm_threads(V, NV))
-    residual_norm_kernel(const __grid_constant__ NormShape s,
-                                     const __grid_constant__ opus_residual_norm_args a) {
-  extern __shared__ float shared[];
-  GroupSum sum(shared, s.group);
+enum Form : int { kAlone, kJoin, kFull };  // no y; y; y with a norm or a gate
+
+template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
+__global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : 3)
+    residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
+  extern __shared__ __align__(16) float shared[];
   const int t = threadIdx.x % s.group;
-  const int64_t in_block = threadIdx.x / s.group;
-  const TX* x = static_cast<const TX*>(a.x);
-  const TY* y = static_cast<const TY*>(a.y);
-  TX* hp = static_cast<TX*>(a.h);
-  TY* np = static_cast<TY*>(a.n);
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * s.groups; base < s.rows;
-       base += static_cast<int64_t>(gridDim.x) * s.groups) {
-    const int64_t row = base + in_block;
-    const bool live = row < s.rows;
-    float h[NV][V], z[NV][V];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (k * s.group + t) * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] = z[k][i] = 0.f;
-      if (live && col < s.d) {
-        load_vec<TX, V>(x + row * a.x_stride + col, h[k]);
-        if (y != nullptr) load_vec<TY, V>(y + row * a.y_stride + col, z[k]);
-      }
+  const int g = threadIdx.x / s.group;
+  const RowRun run(s.rows, static_cast<int64_t>(blockIdx.x) * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
+  const TX* x = static_cast<const TX*>(a.x) + run.first * a.x_stride;
+  const TY* y = static_cast<const TY*>(a.y) + (F != kAlone ? run.first * a.y_stride : 0);
+  TX* h = static_cast<TX*>(a.h) + run.first * s.d;
+  TY* n = static_cast<TY*>(a.n) + run.first * s.d;
+  RawRow<TX, V, NV> xr;
+  RawRow<TY, V, NV> yr;
+  xr.load(run.first < run.last ? x : nullptr, s, t);
+  if constexpr (F != kAlone) yr.load(run.first < run.last ? y : nullptr, s, t);
+  GroupSum sum(shared, s.group, s.groups);
+  float* place = shared + GroupSum::size(s.group, s.groups);
+  Param<NV, V, Near> w(a.weight, a.weight_dtype, 1.f), b(a.bias, a.bias_dtype, 0.f);
+  Param<NV, V, Near> pw(a.post_weight, a.post_weight_dtype, 1.f), pb(a.post_bias, a.post_bias_dtype, 0.f);
+  Param<NV, V, Near> q(a.gate, a.gate_dtype, 1.f);
+  w.fill(&place, s);
+  b.fill(&place, s);
+  const bool one_gate = s.seq == s.rows;
+  if constexpr (F == kFull) {
+    pw.fill(&place, s);
+    pb.fill(&place, s);
+    if (one_gate) q.fill(&place, s);
+  }
+  __syncthreads();
+  int64_t until = run.first / s.seq * s.seq, gate_at = 0;  // first row of the next sample
+  for (int i = 0; i < run.rounds; ++i) {
+    const int64_t row = run.first + i;
+    const bool live = row < run.last;
+    RawRow<TX, V, NV> hr = xr;
+    RawRow<TY, V, NV> zr;
+    x += a.x_stride;
+    xr.load(row + 1 < run.last ? x : nullptr, s, t);
+    if constexpr (F != kAlone) {
+      zr = yr;
+      y += a.y_stride;
+      yr.load(row + 1 < run.last ? y : nullptr, s, t);
     }
-    float2 ys = make_float2(0.f, 0.f);
-    if (a.post) {
-      ys = row_stats<NV, V>(z, s, t, sum);
+    float2 ys = make_float2(0.f, 1.f);
+    float u[NV][V];
+    if constexpr (F == kFull) {
+      if (a.post) ys = zr.stats(s, t, sum);
+      if (one_gate) {
+        q.row(s, t, u);
+      } else {
+        if (row >= until && live) {
+          gate_at = row / s.seq * s.d;
+          until = (row / s.seq + 1) * s.seq;
+        }
+        load_param_row(a.gate, a.gate_dtype, gate_at, 1.f, s, t, u);
+      }
+      float p[NV][V], o[NV][V];
+      pw.row(s, t, p);
+      pb.row(s, t, o);
+      // z = u ((y - mean) / sd p + o)
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int col = (k * s.group + t) * V;
-        if (col >= s.d) continue;
-        float w[V], b[V];
-        load_param<V>(a.post_weight, a.post_weight_dtype, col, 1.f, w);
-        load_param<V>(a.post_bias, a.post_bias_dtype, col, 0.f, b);
+        float z[V];
+        zr.v[k].get(z);
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[k][i] = (z[k][i] - ys.x) * ys.y * w[i] + b[i];
+        for (int j = 0; j < V; ++j) u[k][j] *= fmaf((z[j] - ys.x) * ys.y, p[k][j], o[k][j]);
       }
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int col = (k * s.group + t) * V;
-      if (col >= s.d || !live) continue;
-      if (y != nullptr) {
-        float g[V];
-        load_param<V>(a.gate, a.gate_dtype, row / s.seq * s.d + col, 1.f, g);
+      float r[V];
+      hr.v[k].get(r);
+      if constexpr (F == kJoin) zr.v[k].get(u[k]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[k][i] = a.residual_scale * h[k][i] + g[i] * z[k][i];
+      for (int j = 0; j < V; ++j) r[j] = F == kAlone ? a.residual_scale * r[j] : fmaf(a.residual_scale, r[j], u[k][j]);
+      hr.v[k].set(r);
+      const int col = (k * s.group + t) * V;
+      if (live && col < s.d && (F != kAlone || a.h != nullptr)) *reinterpret_cast<Vec<TX, V>*>(h + col) = hr.v[k];
+    }
+    h += s.d;
+    const float2 hs = hr.stats(s, t, sum);
+    float p[NV][V], o[NV][V];
+    w.row(s, t, p);
+    b.row(s, t, o);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float r[V];
+      hr.v[k].get(r);
+      if (s.layer) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = fmaf((r[j] - hs.x) * hs.y, p[k][j], o[k][j]);
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[k][i] = a.residual_scale * h[k][i];
+        for (int j = 0; j < V; ++j) r[j] = fmaf(r[j] * hs.y, p[k][j], o[k][j]);
       }
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] = to_f32(from_f32<TX>(h[k][i]));
-      if (hp != nullptr) store_vec<TX, V>(hp + row * s.d + col, h[k]);
-    }
-    const float2 hs = row_stats<NV, V>(h, s, t, sum);
-    if (!live) continue;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
       const int col = (k * s.group + t) * V;
-      if (col >= s.d) continue;
-      float w[V], b[V];
-      load_param<V>(a.weight, a.weight_dtype, col, 1.f, w);
-      load_param<V>(a.bias, a.bias_dtype, col, 0.f, b);
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] = (h[k][i] - hs.x) * hs.y * w[i] + b[i];
-      store_vec<TY, V>(np + row * s.d + col, h[k]);
+      if (live && col < s.d) store_vec<TY, V>(n + col, r);
     }
-    if (t == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
+    n += s.d;
+    if (live && t == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
   }
 }
 
-template <typename TX, typename TY, int V, int NV>
-int launch(const NormShape& s, const opus_residual_norm_args& a, cudaStream_t st) {
-  const int threads = (s.group * s.groups + 31) / 32 * 32;
-  int64_t blocks = (s.rows + s.groups - 1) / s.groups;
-  const int64_t most = static_cast<int64_t>(sm_count()) * (2048 / threads);
-  if (blocks > most) blocks = most;
-  residual_norm_kernel<TX, TY, V, NV><<<static_cast<unsigned>(blocks), threads, 4 * (threads / 32) * sizeof(float), st>>>(s, a);
+template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
+int launch(NormShape s, const opus_residual_norm_args& a, cudaStream_t st) {
+  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Near, Wide>;
+  const int threads = s.group * s.groups;
+  const int arrays = F != kFull ? 2 : s.seq == s.rows ? 5 : 4;
+  const int shared = (GroupSum::size(s.group, s.groups) + arrays * Param<NV, V, Near>::size(s.group)) * static_cast<int>(sizeof(float));
+  const int rc = allow_shared<kernel>(shared);
+  if (rc) return rc;
+  const int64_t need = (s.rows + s.groups - 1) / s.groups;
+  const int64_t most = static_cast<int64_t>(sm_count()) * resident_blocks<kernel>(threads, shared);
+  s.blocks = static_cast<int>(need < most ? need : most);
+  kernel<<<s.blocks, threads, shared, st>>>(s, a);
   note_launch();
   OPUS_CUDA_TRY(cudaGetLastError());
   return OPUS_OK;
 }
 
-template <typename TX, typename TY>
-int launch_by_width(const opus_residual_norm_args& a, bool vec, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(TX);
+template <typename TX, typename TY, int V, int F>
+int launch_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
+  constexpr int kMost = 16 / V;
+  constexpr int kWide = wide_vectors(V);
   NormShape s;
   int nv;
-  const int rc = norm_shape("residual_norm", &a, vec, V, &s, &nv);
+  if (a.d > kNormNarrow) {
+    const int rc = norm_shape("residual_norm", &a, V, kWide, &s, &nv);
+    if (rc) return rc;
+    if constexpr (F == kFull) {
+      if (5 * Param<kWide, V, true>::size(s.group) * static_cast<int>(sizeof(float)) > kNormSharedParams)
+        return launch<TX, TY, V, kWide, F, false, true>(s, a, st);
+    }
+    return launch<TX, TY, V, kWide, F, true, true>(s, a, st);
+  }
+  const int rc = norm_shape("residual_norm", &a, V, kMost, &s, &nv);
   if (rc) return rc;
-  if (!vec) return nv == 4 ? launch<TX, TY, 1, 4>(s, a, st) : launch<TX, TY, 1, 16>(s, a, st);
-  if (nv == 1) return launch<TX, TY, V, 1>(s, a, st);
-  if (nv == 2) return launch<TX, TY, V, 2>(s, a, st);
-  if constexpr (V == 4) return launch<TX, TY, V, 4>(s, a, st);
-  return set_error(OPUS_ERR_UNSUPPORTED, "residual_norm: d = %d", a.d);
+  if constexpr (V > 1) {
+    if (nv == 1) return launch<TX, TY, V, 1, F, true, false>(s, a, st);
+  }
+  if constexpr (V < 8) {
+    if (nv <= 4 / (V == 4 ? 2 : 1)) return launch<TX, TY, V, 4 / (V == 4 ? 2 : 1), F, true, false>(s, a, st);
+  }
+  return launch<TX, TY, V, kMost, F, true, false>(s, a, st);
+}
+
+template <typename TX, typename TY, int V>
+int launch_by_form(const opus_residual_norm_args& a, cudaStream_t st) {
+  if (a.post || a.gate != nullptr) return launch_by_width<TX, TY, V, kFull>(a, st);
+  if (a.y != nullptr) return launch_by_width<TX, TY, V, kJoin>(a, st);
+  return launch_by_width<TX, TY, V, kAlone>(a, st);
+}
+
+template <typename TX, typename TY>
+int launch_by_alignment(const opus_residual_norm_args& a, bool vec, cudaStream_t st) {
+  return vec ? launch_by_form<TX, TY, 16 / sizeof(TX)>(a, st) : launch_by_form<TX, TY, 1>(a, st);
 }
 
 bool on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -192,14 +254,14 @@ extern "C" int opus_residual_norm(const opus_residual_norm_args* args, void* str
   if (!on(a.x, xb) || !on(a.h, xb) || !on(a.y, yb) || !on(a.n, yb) || !on(a.stats, 16))
     return set_error(OPUS_ERR_INVALID, "residual_norm: a pointer is not aligned to its elements");
   const int V = 16 / xb;
-  const bool vec = a.d % V == 0 && a.x_stride % V == 0 && on(a.x, 16) && on(a.h, 16) && on(a.n, V * yb) &&
+  const bool vec = norm_params_aligned(&a) && a.d % V == 0 && a.x_stride % V == 0 && on(a.x, 16) && on(a.h, 16) && on(a.n, V * yb) &&
                    (!a.y || (a.y_stride % V == 0 && on(a.y, V * yb)));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a.x_dtype == OPUS_DTYPE_F32) {
-    if (a.y_dtype == OPUS_DTYPE_F32) return launch_by_width<float, float>(a, vec, st);
-    if (a.y_dtype == OPUS_DTYPE_F16) return launch_by_width<float, __half>(a, vec, st);
-    return launch_by_width<float, __nv_bfloat16>(a, vec, st);
+    if (a.y_dtype == OPUS_DTYPE_F32) return launch_by_alignment<float, float>(a, vec, st);
+    if (a.y_dtype == OPUS_DTYPE_F16) return launch_by_alignment<float, __half>(a, vec, st);
+    return launch_by_alignment<float, __nv_bfloat16>(a, vec, st);
   }
-  if (a.x_dtype == OPUS_DTYPE_F16) return launch_by_width<__half, __half>(a, vec, st);
-  return launch_by_width<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
+  if (a.x_dtype == OPUS_DTYPE_F16) return launch_by_alignment<__half, __half>(a, vec, st);
+  return launch_by_alignment<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
 }

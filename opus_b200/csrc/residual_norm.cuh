@@ -3,7 +3,15 @@
 //
 // A row of d elements is held by a group of `group` threads (a power of two up
 // to 32, or whole warps), thread t holding the vectors t, t + group, ... of V
-// elements each, NV of them at most.  A block holds `groups` rows at a time.
+// elements each, NV of them, as they are in memory.  Every group owns a run of
+// neighbouring rows and loads one while it works on the one before.
+//
+// What bounds these kernels besides HBM is how many instructions a row takes:
+// at 6.5 TB/s an SM has about 2800 issue slots for a forward row of 2048 bf16
+// elements.  So 16 elements a thread (each thread's addresses, shuffles and
+// barriers serve more of them), parameters as f32 in shared memory with ones
+// and zeros where there are none (no branches between loads, which otherwise
+// wait for each other), and 16-bit elements taken apart by words.
 #pragma once
 
 #include "elements.cuh"
@@ -13,8 +21,11 @@ namespace opus {
 constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxWidth = 16384;
 
-// Threads of a block at most, by the elements that a thread holds (norm_shape keeps to it).
-constexpr int norm_threads(int V, int NV) { return V * NV >= 16 ? 1024 : 512; }
+// Rows of up to kNormNarrow elements take up to 16 elements a thread and 256 threads; wider ones 32 elements and
+// 512 threads, or 16 and 1024 where vectors have one element.
+constexpr int kNormNarrow = 4096;
+constexpr int wide_vectors(int V) { return V == 1 ? 16 : 32 / V; }
+constexpr int norm_threads(int V, bool wide) { return !wide ? 256 : V == 1 ? 1024 : 512; }
 
 struct NormShape {
   int64_t rows;
@@ -23,82 +34,230 @@ struct NormShape {
   int group, groups;  // threads of a row, rows of a block
   int layer;          // LayerNorm (1) or RMS norm (0)
   float eps;
+  int blocks;  // of the launch
 };
 
-// Sums over the group of up to two values each, one after the other in a fixed
-// order; the result is in every thread of the group.  `turn` alternates between
-// calls, so that one barrier a call is enough.
+// The rows [first, last) of worker w among n, and how many rounds the longest run takes.
+struct RowRun {
+  int64_t first, last;
+  int rounds;
+  __device__ RowRun(int64_t rows, int64_t w, int64_t n) {
+    const int64_t each = rows / n, more = rows % n;
+    first = w * each + (w < more ? w : more);
+    last = first + each + (w < more ? 1 : 0);
+    rounds = static_cast<int>(each + (more > 0 ? 1 : 0));
+  }
+};
+
+// Sums over the group of up to two values each, in a fixed order; the result is in every thread of the group.
+// A call takes one barrier of the group's own: `turn` alternates between two buffers.
 struct GroupSum {
-  float* buf;  // 2 * 2 * warps floats of shared memory
-  int group, warps, warp, lane, first;
+  float* buf;
+  int width, slots, span, barrier, threads;
   int turn;
 
-  __device__ GroupSum(float* shared, int group_) : buf(shared), group(group_), turn(0) {
-    lane = threadIdx.x & 31;
-    warp = threadIdx.x >> 5;
-    warps = blockDim.x >> 5;
-    first = (threadIdx.x / group) * (group >> 5);  // of the group's warps, when it has whole ones
+  // floats of shared memory
+  static __host__ __device__ int size(int group, int groups) {
+    return group <= 32 ? 0 : 2 * 2 * groups * (((group >> 5) + 3) / 4 * 4);
+  }
+  // every thread of the block calls it once
+  __device__ GroupSum(float* shared, int group, int groups) : turn(0) {
+    width = group < 32 ? group : 32;
+    slots = group <= 32 ? 0 : ((group >> 5) + 3) / 4 * 4;  // of the group's warps, zeros behind them
+    span = groups * slots;
+    const int g = static_cast<int>(threadIdx.x) / group;
+    buf = shared + g * slots;
+    barrier = 1 + g;  // named barriers 1 to 15: a block has at most 4 groups of more than a warp
+    threads = group;
+    if (slots) {
+      for (int i = threadIdx.x; i < 4 * span; i += blockDim.x) shared[i] = 0.f;
+      __syncthreads();
+    }
   }
   template <int N>
-  __device__ __forceinline__ void operator()(float (&v)[N]) {
-    const int width = group < 32 ? group : 32;
+  __device__ __forceinline__ void operator()(float (&v)[N], int t) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      for (int o = width >> 1; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if (group <= 32) return;
-    float* b = buf + turn * 2 * warps;
-    turn ^= 1;
-    if (lane == 0) {
+    for (int o = 16; o > 0; o >>= 1) {
+      if (o >= width) continue;
 #pragma unroll
-      for (int i = 0; i < N; ++i) b[i * warps + warp] = v[i];
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     }
-    __syncthreads();
-    const int n = group >> 5;
+    if (slots == 0) return;
+    float* b = buf + turn * 2 * span;
+    turn ^= 1;
+    if ((t & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[i * span + (t >> 5)] = v[i];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float s = 0.f;
-      for (int w = 0; w < n; ++w) s += b[i * warps + first + w];
+      for (int w = 0; w < slots; w += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(b + i * span + w);
+        s += (q.x + q.y) + (q.z + q.w);
+      }
       v[i] = s;
     }
   }
 };
 
-// mean (0 for an RMS norm) and 1 / sqrt(mean square about it + eps) of the row held in r.
-template <int NV, int V>
-__device__ __forceinline__ float2 row_stats(const float (&r)[NV][V], const NormShape& s, int t, GroupSum& sum) {
-  float mean = 0.f;
-  const float inv_d = 1.0f / static_cast<float>(s.d);
-  if (s.layer) {
-    float a[1] = {0.f};
+// A thread's part of a row, as it is in memory; zeros beyond the row.
+template <typename T, int V, int NV>
+struct RawRow {
+  Vec<T, V> v[NV];
+  __device__ __forceinline__ void load(const T* row, const NormShape& s, int t) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) a[0] += r[k][i];  // zeros beyond the row
-    sum(a);
-    mean = a[0] * inv_d;
-  }
-  float q[1] = {0.f};
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    if ((k * s.group + t) * V >= s.d) continue;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float c = r[k][i] - mean;
-      q[0] = fmaf(c, c, q[0]);
+    for (int k = 0; k < NV; ++k) {
+      const int col = (k * s.group + t) * V;
+      if (row != nullptr && col < s.d) v[k] = *reinterpret_cast<const Vec<T, V>*>(row + col);
+      else v[k].zero();
     }
   }
-  sum(q);
-  return make_float2(mean, rsqrtf(q[0] * inv_d + s.eps));
-}
-
-// V neighbours of a parameter vector, or `other` where there is none.
-template <int V>
-__device__ __forceinline__ void load_param(const void* p, int dtype, int64_t at, float other, float (&r)[V]) {
+  // mean (0 for an RMS norm) and 1 / sqrt(mean square about it + eps) of the row
+  __device__ __forceinline__ float2 stats(const NormShape& s, int t, GroupSum& sum) const {
+    const float inv_d = 1.0f / static_cast<float>(s.d);
+    float mean = 0.f;
+    if (s.layer) {
+      float a[1] = {0.f};
 #pragma unroll
-  for (int i = 0; i < V; ++i) r[i] = p != nullptr ? load_any(p, dtype, at + i) : other;
+      for (int k = 0; k < NV; ++k) {
+        float r[V];
+        v[k].get(r);
+#pragma unroll
+        for (int i = 0; i < V; ++i) a[0] += r[i];
+      }
+      sum(a, t);
+      mean = a[0] * inv_d;
+    }
+    float q[2] = {0.f, 0.f};  // two chains
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const float m = (k * s.group + t) * V < s.d ? mean : 0.f;
+      float r[V];
+      v[k].get(r);
+#pragma unroll
+      for (int i = 0; i < V; ++i) q[i & 1] = fmaf(r[i] - m, r[i] - m, q[i & 1]);
+    }
+    float whole[1] = {q[0] + q[1]};
+    sum(whole, t);
+    return make_float2(mean, rsqrtf(whole[0] * inv_d + s.eps));
+  }
+};
+
+// V neighbours of an array whose type is known at run time, in accesses of up to 16 bytes (V > 1: aligned arrays).
+template <typename T, int V>
+__device__ __forceinline__ void load_param_as(const void* p, int64_t at, float (&r)[V]) {
+  constexpr int W = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
+#pragma unroll
+  for (int j = 0; j < V / W; ++j) {
+    float part[W];
+    load_vec<T, W>(static_cast<const T*>(p) + at + j * W, part);
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[j * W + i] = part[i];
+  }
+}
+template <int V>
+__device__ __forceinline__ void load_param_vec(const void* p, int dtype, int64_t at, float (&r)[V]) {
+  if (dtype == OPUS_DTYPE_F32) load_param_as<float, V>(p, at, r);
+  else if (dtype == OPUS_DTYPE_F16) load_param_as<__half, V>(p, at, r);
+  else load_param_as<__nv_bfloat16, V>(p, at, r);
 }
 
-int norm_shape(const char* what, const opus_residual_norm_args* a, bool vec, int V, NormShape* s, int* nv);
+// A thread's part of one of the parameters' rows, from where it is (`other` where there is none, 0 beyond the row).
+// The branches on the type enclose all of a thread's loads.
+template <typename T, int NV, int V>
+__device__ __forceinline__ void load_param_row_as(const void* p, int64_t at, const NormShape& s, int t, float (&r)[NV][V]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int col = (k * s.group + t) * V;
+    if (col < s.d) load_param_as<T, V>(p, at + col, r[k]);
+  }
+}
+template <int NV, int V>
+__device__ __forceinline__ void load_param_row(const void* p, int dtype, int64_t at, float other, const NormShape& s, int t,
+                                               float (&r)[NV][V]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[k][i] = (k * s.group + t) * V < s.d ? other : 0.f;
+  if (p == nullptr) return;
+  if (dtype == OPUS_DTYPE_F32) load_param_row_as<float>(p, at, s, t, r);
+  else if (dtype == OPUS_DTYPE_F16) load_param_row_as<__half>(p, at, s, t, r);
+  else load_param_row_as<__nv_bfloat16>(p, at, s, t, r);
+}
+
+// A parameter of d elements that rows share.  Near: as f32 in shared memory, `other` where there is none and 0
+// beyond the row; vectors of 8 lie in two planes of 4, so that neighbouring lanes read neighbouring 16 bytes.
+// Otherwise read from where it is.
+template <int NV, int V, bool Near>
+struct Param {
+  const void* p;
+  int dtype;
+  float other;
+  float* near;
+  __device__ __forceinline__ Param(const void* p_, int dtype_, float other_) : p(p_), dtype(dtype_), other(other_), near(nullptr) {}
+  static __host__ __device__ int size(int group) { return Near ? group * NV * V : 0; }
+  // by every thread; a barrier has to follow
+  __device__ __forceinline__ void fill(float** shared, const NormShape& s) {
+    if constexpr (Near) {
+      near = *shared;
+      const int whole = size(s.group);
+      *shared += whole;
+      for (int col = threadIdx.x * V; col < whole; col += blockDim.x * V) {
+        float r[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = col < s.d ? other : 0.f;
+        if (p != nullptr && col < s.d) load_param_vec<V>(p, dtype, col, r);
+        if constexpr (V == 8) {
+          *reinterpret_cast<float4*>(near + col / 2) = make_float4(r[0], r[1], r[2], r[3]);
+          *reinterpret_cast<float4*>(near + (whole + col) / 2) = make_float4(r[4], r[5], r[6], r[7]);
+        } else {
+          store_vec<float, V>(near + col, r);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void row(const NormShape& s, int t, float (&r)[NV][V]) const {
+    if constexpr (!Near) {
+      load_param_row(p, dtype, 0, other, s, t, r);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int col = (k * s.group + t) * V;
+        if constexpr (V == 8) {
+          const float4 a = *reinterpret_cast<const float4*>(near + col / 2);
+          const float4 b = *reinterpret_cast<const float4*>(near + (size(s.group) + col) / 2);
+          r[k][0] = a.x, r[k][1] = a.y, r[k][2] = a.z, r[k][3] = a.w;
+          r[k][4] = b.x, r[k][5] = b.y, r[k][6] = b.z, r[k][7] = b.w;
+        } else {
+          load_vec<float, V>(near + col, r[k]);
+        }
+      }
+    }
+  }
+};
+
+// Blocks of a kernel that one multiprocessor holds.
+template <auto Kernel>
+int resident_blocks(int threads, int shared_bytes) {
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, shared_bytes) != cudaSuccess || n < 1) n = 1;
+  return n;
+}
+
+// Shared memory that the parameters may take; above it they are read from where they are.
+constexpr int kNormSharedParams = 160 * 1024;
+
+int norm_shape(const char* what, const opus_residual_norm_args* a, int V, int most, NormShape* s, int* nv);
 int check_norm(const char* what, const opus_residual_norm_args* a);
+bool norm_params_aligned(const opus_residual_norm_args* a);
+
+// Sets a kernel's dynamic shared memory limit where it needs more than the default.
+template <auto Kernel>
+int allow_shared(int bytes) {
+  if (bytes > 48 * 1024) OPUS_CUDA_TRY(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return OPUS_OK;
+}
 
 }  // namespace opus

@@ -8,116 +8,341 @@
 //   dy = dz, or through the norm of y: c = dz o w_post,
 //   dy = (c - <c> - yh <c yh>) / sd_y;  dw_post = sum dz o yh;  db_post = sum dz
 //
-// Rows (dx, dy) come from one kernel, sums over rows from another that reads
-// the rows again: each thread keeps a column's sums over a run of rows in f32,
-// runs meet in a third kernel, always in the same order.
+// d up to 4096: one kernel reads each row once, writes dx and dy, and keeps a
+// column's sums over its run of rows in registers (16 columns a thread, five
+// sums each); a second kernel joins the runs.  Wider rows would need more
+// than 256 threads and leave them too few registers for that: one kernel for
+// dx and dy, another that reads the rows again for the sums, and the same
+// join.  Every sum has a fixed order.
+//
+// Bound: HBM bandwidth (h, dn, dh_in and y read once, dx and dy written once).
 #include "residual_norm.cuh"
 
 namespace opus {
 namespace {
 
-template <typename TX, typename TY, int V, int NV>
-__global__ void __launch_bounds__(norm_threads(V, NV))
-    rows_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a,
-                            float2* __restrict__ means) {
-  extern __shared__ float shared[];
-  GroupSum sum(shared, s.group);
+enum Column : int { kWeight = 0, kBias, kPostWeight, kPostBias, kGate, kColumns };
+
+// The worker (group of threads) whose run of rows holds `row`: RowRun's split, inverted.
+__device__ __forceinline__ int64_t worker_of(int64_t row, int64_t rows, int64_t n) {
+  const int64_t each = rows / n, more = rows % n, cut = more * (each + 1);
+  return row < cut ? row / (each + 1) : more + (row - cut) / each;
+}
+
+// parts[block][array][d]: sums over the block's rows.  gates[worker + sample][d]: sums over the worker's rows of
+// one sample, where each sample has a gate (a step to the next worker or sample is a step to the next slot).
+// Full: with a norm of y or a gate.  Bias: sums for bias and post_bias too.
+template <typename TX, typename TY, int V, int NV, bool Full, bool Bias>
+__global__ void __launch_bounds__(norm_threads(V, false))
+    grad_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a, int wanted,
+                float* __restrict__ parts, float* __restrict__ gates) {
+  extern __shared__ __align__(16) float shared[];
   const int t = threadIdx.x % s.group;
-  const int64_t in_block = threadIdx.x / s.group;
-  const TX* hp = static_cast<const TX*>(a.h);
-  const TY* y = static_cast<const TY*>(a.y);
-  const TY* dnp = static_cast<const TY*>(a.grad_n);
-  const TX* dhp = static_cast<const TX*>(a.grad_h);
-  TX* dx = static_cast<TX*>(a.grad_x);
-  TY* dy = static_cast<TY*>(a.grad_y);
+  const int g = threadIdx.x / s.group;
+  const int64_t worker = static_cast<int64_t>(blockIdx.x) * s.groups + g;
+  const RowRun run(s.rows, worker, static_cast<int64_t>(s.blocks) * s.groups);
+  const TX* hp = static_cast<const TX*>(a.h) + run.first * a.h_stride;
+  const TX* dhp = static_cast<const TX*>(a.grad_h) + run.first * a.grad_h_stride;
+  const TY* dnp = static_cast<const TY*>(a.grad_n) + run.first * a.grad_n_stride;
+  const TY* yp = static_cast<const TY*>(a.y) + run.first * a.y_stride;
+  TX* dx = static_cast<TX*>(a.grad_x) + run.first * s.d;
+  TY* dy = static_cast<TY*>(a.grad_y) + run.first * s.d;
+  const float4* stats = reinterpret_cast<const float4*>(a.stats) + run.first;
+  RawRow<TX, V, NV> hr, dhr;
+  RawRow<TY, V, NV> dnr, yr;
+  float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);
+  const auto fetch = [&](int64_t row) {
+    const bool live = row < run.last;
+    hr.load(live ? hp : nullptr, s, t);
+    dnr.load(live && a.grad_n != nullptr ? dnp : nullptr, s, t);
+    dhr.load(live && a.grad_h != nullptr ? dhp : nullptr, s, t);
+    if constexpr (Full) yr.load(live ? yp : nullptr, s, t);
+    if (live) ahead = *stats;
+    hp += a.h_stride, dhp += a.grad_h_stride, dnp += a.grad_n_stride, yp += a.y_stride, ++stats;
+  };
+  fetch(run.first);
+  GroupSum sum(shared, s.group, s.groups);
+  float* meet = shared + GroupSum::size(s.group, s.groups);
+  float* place = meet + (s.groups > 1 ? blockDim.x * V * NV : 0);
+  const bool one_gate = s.seq == s.rows;
+  Param<NV, V, true> w(a.weight, a.weight_dtype, 1.f), q(a.gate, a.gate_dtype, 1.f);
+  Param<NV, V, true> pw(a.post_weight, a.post_weight_dtype, 1.f), pb(a.post_bias, a.post_bias_dtype, 0.f);
+  w.fill(&place, s);
+  if constexpr (Full) {
+    pw.fill(&place, s);
+    if constexpr (Bias) pb.fill(&place, s);
+    if (one_gate) q.fill(&place, s);
+  }
+  __syncthreads();
   const float inv_d = 1.0f / static_cast<float>(s.d);
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * s.groups; base < s.rows;
-       base += static_cast<int64_t>(gridDim.x) * s.groups) {
-    const int64_t row = base + in_block;
-    const bool live = row < s.rows;
-    const float4 st = live ? reinterpret_cast<const float4*>(a.stats)[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-    float hat[NV][V], g[NV][V];
+  float acc_w[NV][V], acc_b[Bias ? NV : 1][V], acc_pw[Full ? NV : 1][V], acc_pb[Full && Bias ? NV : 1][V], acc_g[Full ? NV : 1][V];
+  const auto clear = [](auto& acc) {
+    for (auto& k : acc)
+      for (float& v : k) v = 0.f;
+  };
+  clear(acc_w), clear(acc_b), clear(acc_pw), clear(acc_pb), clear(acc_g);
+  int64_t sample = -1, until = -1;  // of the gate whose sums are held; the first row of the next sample
+  const auto flush_gate = [&]() {
+    if constexpr (Full) {
+      if (sample < 0 || (wanted & (1 << kGate)) == 0) return;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int col = (k * s.group + t) * V;
+        if (col < s.d) store_vec<float, V>(gates + (worker + sample) * s.d + col, acc_g[k]);
+      }
+      clear(acc_g);
+    }
+  };
+  for (int i = 0; i < run.rounds; ++i) {
+    const int64_t row = run.first + i;
+    const bool live = row < run.last;
+    const RawRow<TX, V, NV> h = hr, in = dhr;
+    const RawRow<TY, V, NV> dn = dnr, y = yr;
+    const float4 st = ahead;
+    fetch(row + 1);
+    float u[NV][V];
     float m[2] = {0.f, 0.f};
+    w.row(s, t, u);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float hat[V], v[V];
+      h.v[k].get(hat);
+      dn.v[k].get(v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        hat[j] = (hat[j] - st.x) * st.y;
+        acc_w[k][j] = fmaf(v[j], hat[j], acc_w[k][j]);
+        if constexpr (Bias) acc_b[k][j] += v[j];
+        u[k][j] *= v[j];
+        m[0] += u[k][j];
+        m[1] = fmaf(u[k][j], hat[j], m[1]);
+      }
+    }
+    sum(m, t);
+    m[0] = s.layer ? m[0] * inv_d : 0.f;
+    m[1] *= inv_d * st.y;  // times 1 / sd: hat is taken apart below
+    // dh in u
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float hat[V], r[V];
+      h.v[k].get(hat);
+      in.v[k].get(r);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        u[k][j] = fmaf(st.y, u[k][j] - m[0] - (hat[j] - st.x) * m[1], r[j]);
+        r[j] = a.residual_scale * u[k][j];
+      }
+      const int col = (k * s.group + t) * V;
+      if (live && col < s.d) store_vec<TX, V>(dx + col, r);
+    }
+    dx += s.d;
+    if constexpr (Full) {
+      float e[NV][V];
+      if (one_gate) {
+        q.row(s, t, e);
+      } else {
+        if (live && row >= until) {
+          flush_gate();
+          sample = row / s.seq;
+          until = (sample + 1) * s.seq;
+        }
+        load_param_row(a.gate, a.gate_dtype, (sample < 0 ? 0 : sample) * s.d, 1.f, s, t, e);
+      }
+      if (!a.post) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          float z[V];
+          y.v[k].get(z);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            acc_g[k][j] = fmaf(u[k][j], z[j], acc_g[k][j]);
+            u[k][j] *= e[k][j];
+          }
+        }
+      } else {
+        float f[NV][V], o[NV][V];
+        pw.row(s, t, f);
+        if constexpr (Bias) pb.row(s, t, o);
+        float p[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          float z[V];
+          y.v[k].get(z);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            z[j] = (z[j] - st.z) * st.w;  // normed y
+            acc_g[k][j] = fmaf(u[k][j], Bias ? fmaf(z[j], f[k][j], o[k][j]) : z[j] * f[k][j], acc_g[k][j]);
+            const float dz = u[k][j] * e[k][j];
+            acc_pw[k][j] = fmaf(dz, z[j], acc_pw[k][j]);
+            if constexpr (Bias) acc_pb[k][j] += dz;
+            u[k][j] = dz * f[k][j];
+            p[0] += u[k][j];
+            p[1] = fmaf(u[k][j], z[j], p[1]);
+          }
+        }
+        sum(p, t);
+        p[0] = s.layer ? p[0] * inv_d : 0.f;
+        p[1] *= inv_d * st.w;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          float z[V];
+          y.v[k].get(z);
+#pragma unroll
+          for (int j = 0; j < V; ++j) u[k][j] = st.w * (u[k][j] - p[0] - (z[j] - st.z) * p[1]);
+        }
+      }
+    }
+    if (live && a.grad_y != nullptr) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int col = (k * s.group + t) * V;
+        if (col < s.d) store_vec<TY, V>(dy + col, u[k]);
+      }
+    }
+    dy += s.d;
+  }
+  if (!one_gate) flush_gate();
+  // the block's groups together, in order
+  const auto finish = [&](auto& acc, int which) {
+    if ((wanted & (1 << which)) == 0) return;
+    if (s.groups > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) meet[(k * V + j) * blockDim.x + threadIdx.x] = acc[k][j];
+      __syncthreads();
+      if (g == 0) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            for (int o = 1; o < s.groups; ++o) acc[k][j] += meet[(k * V + j) * blockDim.x + o * s.group + t];
+      }
+    }
+    if (g != 0) return;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int col = (k * s.group + t) * V;
+      if (col < s.d) store_vec<float, V>(parts + (static_cast<int64_t>(blockIdx.x) * kColumns + which) * s.d + col, acc[k]);
+    }
+  };
+  finish(acc_w, kWeight);
+  if constexpr (Bias) finish(acc_b, kBias);
+  if constexpr (Full) {
+    finish(acc_pw, kPostWeight);
+    if constexpr (Bias) finish(acc_pb, kPostBias);
+    if (one_gate) finish(acc_g, kGate);
+  }
+}
+
+// ---- wider rows
+template <typename TX, typename TY, int V, int NV>
+__global__ void __launch_bounds__(norm_threads(V, true))
+    rows_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a,
+                float2* __restrict__ means) {
+  extern __shared__ __align__(16) float shared[];
+  const int t = threadIdx.x % s.group;
+  const int g = threadIdx.x / s.group;
+  const RowRun run(s.rows, static_cast<int64_t>(blockIdx.x) * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
+  const TX* dhp = static_cast<const TX*>(a.grad_h);
+  const TY* dnp = static_cast<const TY*>(a.grad_n);
+  const float inv_d = 1.0f / static_cast<float>(s.d);
+  GroupSum sum(shared, s.group, s.groups);
+  for (int i = 0; i < run.rounds; ++i) {
+    const int64_t row = run.first + i;
+    const bool live = row < run.last;
+    const float4 st = live ? reinterpret_cast<const float4*>(a.stats)[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    RawRow<TX, V, NV> hr;
+    RawRow<TY, V, NV> r2;  // dn, then y
+    hr.load(live ? static_cast<const TX*>(a.h) + row * a.h_stride : nullptr, s, t);
+    r2.load(live && dnp != nullptr ? dnp + row * a.grad_n_stride : nullptr, s, t);
+    float v[NV][V];
+    float m[2] = {0.f, 0.f};
+    load_param_row(a.weight, a.weight_dtype, 0, 1.f, s, t, v);
 #pragma unroll
-      for (int i = 0; i < V; ++i) hat[k][i] = g[k][i] = 0.f;
-      if (!live || col >= s.d) continue;
-      load_vec<TX, V>(hp + row * a.h_stride + col, hat[k]);
-      if (dnp != nullptr) load_vec<TY, V>(dnp + row * a.grad_n_stride + col, g[k]);
-      float w[V];
-      load_param<V>(a.weight, a.weight_dtype, col, 1.f, w);
+    for (int k = 0; k < NV; ++k) {
+      float hat[V], dn[V];
+      hr.v[k].get(hat);
+      r2.v[k].get(dn);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        hat[k][i] = (hat[k][i] - st.x) * st.y;
-        g[k][i] *= w[i];
-        m[0] += g[k][i];
-        m[1] = fmaf(g[k][i], hat[k][i], m[1]);
+      for (int j = 0; j < V; ++j) {
+        v[k][j] *= dn[j];
+        m[0] += v[k][j];
+        m[1] = fmaf(v[k][j], (hat[j] - st.x) * st.y, m[1]);
       }
     }
-    sum(m);
+    sum(m, t);
     m[0] = s.layer ? m[0] * inv_d : 0.f;
     m[1] *= inv_d;
-    if (live && t == 0 && means != nullptr) means[row] = make_float2(m[0], m[1]);
+    if (live && t == 0) means[row] = make_float2(m[0], m[1]);
+    r2.load(live && a.post ? static_cast<const TY*>(a.y) + row * a.y_stride : nullptr, s, t);
+    RawRow<TX, V, NV> in;
+    in.load(live && dhp != nullptr ? dhp + row * a.grad_h_stride : nullptr, s, t);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      float hat[V], r[V];
+      hr.v[k].get(hat);
+      in.v[k].get(r);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[k][j] = r[j] + st.y * (v[k][j] - m[0] - (hat[j] - st.x) * st.y * m[1]);
+        r[j] = a.residual_scale * v[k][j];
+      }
       const int col = (k * s.group + t) * V;
-      if (!live || col >= s.d) continue;
-      float in[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) in[i] = 0.f;
-      if (dhp != nullptr) load_vec<TX, V>(dhp + row * a.grad_h_stride + col, in);
-      float out[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        g[k][i] = in[i] + st.y * (g[k][i] - m[0] - hat[k][i] * m[1]);
-        out[i] = a.residual_scale * g[k][i];
-      }
-      store_vec<TX, V>(dx + row * s.d + col, out);
-      if (y != nullptr && a.gate != nullptr) {
-        float q[V];
-        load_param<V>(a.gate, a.gate_dtype, row / s.seq * s.d + col, 1.f, q);
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[k][i] *= q[i];
-      }
-      if (y != nullptr && !a.post) store_vec<TY, V>(dy + row * s.d + col, g[k]);
+      if (live && col < s.d) store_vec<TX, V>(static_cast<TX*>(a.grad_x) + row * s.d + col, r);
     }
-    if (!a.post) continue;
-    float p[2] = {0.f, 0.f};
+    if (a.gate != nullptr) {
+      float q[NV][V];
+      load_param_row(a.gate, a.gate_dtype, live && s.seq != s.rows ? row / s.seq * s.d : 0, 1.f, s, t, q);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (k * s.group + t) * V;
-      if (!live || col >= s.d) continue;
-      float w[V];
-      load_vec<TY, V>(y + row * a.y_stride + col, hat[k]);
-      load_param<V>(a.post_weight, a.post_weight_dtype, col, 1.f, w);
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        hat[k][i] = (hat[k][i] - st.z) * st.w;
-        g[k][i] *= w[i];
-        p[0] += g[k][i];
-        p[1] = fmaf(g[k][i], hat[k][i], p[1]);
+        for (int j = 0; j < V; ++j) v[k][j] *= q[k][j];
+    }
+    if (a.post) {
+      float p[2] = {0.f, 0.f}, u[NV][V];
+      load_param_row(a.post_weight, a.post_weight_dtype, 0, 1.f, s, t, u);  // zeros beyond the row
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float y[V];
+        r2.v[k].get(y);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          v[k][j] *= u[k][j];
+          p[0] += v[k][j];
+          p[1] = fmaf(v[k][j], (y[j] - st.z) * st.w, p[1]);
+        }
+      }
+      sum(p, t);
+      p[0] = s.layer ? p[0] * inv_d : 0.f;
+      p[1] *= inv_d;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float y[V];
+        r2.v[k].get(y);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[k][j] = st.w * (v[k][j] - p[0] - (y[j] - st.z) * st.w * p[1]);
       }
     }
-    sum(p);
-    p[0] = s.layer ? p[0] * inv_d : 0.f;
-    p[1] *= inv_d;
+    if (!live || a.grad_y == nullptr) continue;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int col = (k * s.group + t) * V;
-      if (!live || col >= s.d) continue;
-#pragma unroll
-      for (int i = 0; i < V; ++i) g[k][i] = st.w * (g[k][i] - p[0] - hat[k][i] * p[1]);
-      store_vec<TY, V>(dy + row * s.d + col, g[k]);
+      if (col < s.d) store_vec<TY, V>(static_cast<TY*>(a.grad_y) + row * s.d + col, v[k]);
     }
   }
 }
 
-enum Column : int { kWeight = 0, kBias, kPostWeight, kPostBias, kGate, kColumns };
-
 constexpr int kColWarps = 8;
 constexpr int kRun = 64;  // rows of a run at least
+
+template <int V>
+__device__ __forceinline__ void column_param(const void* p, int dtype, int64_t at, float other, float (&r)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) r[i] = other;
+  if (p != nullptr) load_param_vec<V>(p, dtype, at, r);
+}
 
 // One block: 32 * V columns, one run of rows.  parts[run][array][d].
 template <typename TX, typename TY, int V>
@@ -140,9 +365,9 @@ __global__ void __launch_bounds__(kColWarps * 32)
   const bool deep = (wanted & (1 << kPostWeight | 1 << kPostBias | 1 << kGate)) != 0;
   if (own) {
     float w[V], pw[V], pb[V];
-    load_param<V>(a.weight, a.weight_dtype, col, 1.f, w);
-    load_param<V>(a.post_weight, a.post_weight_dtype, col, 1.f, pw);
-    load_param<V>(a.post_bias, a.post_bias_dtype, col, 0.f, pb);
+    column_param<V>(a.weight, a.weight_dtype, col, 1.f, w);
+    column_param<V>(a.post_weight, a.post_weight_dtype, col, 1.f, pw);
+    column_param<V>(a.post_bias, a.post_bias_dtype, col, 0.f, pb);
     for (int64_t row = first + warp; row < last; row += kColWarps) {
       const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
       float hat[V], dn[V];
@@ -163,7 +388,7 @@ __global__ void __launch_bounds__(kColWarps * 32)
       for (int i = 0; i < V; ++i) dh[i] = 0.f;
       if (a.grad_h != nullptr) load_vec<TX, V>(static_cast<const TX*>(a.grad_h) + row * a.grad_h_stride + col, dh);
       load_vec<TY, V>(static_cast<const TY*>(a.y) + row * a.y_stride + col, z);
-      load_param<V>(a.gate, a.gate_dtype, row / s.seq * s.d + col, 1.f, g);
+      column_param<V>(a.gate, a.gate_dtype, (s.seq == s.rows ? 0 : row / s.seq) * s.d + col, 1.f, g);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         dh[i] += st.y * (dn[i] * w[i] - m.x - hat[i] * m.y);
@@ -200,23 +425,57 @@ struct ColumnOutputs {
   int dtype[kColumns];
 };
 
-// Sums the runs of 32 columns of one array (blockIdx.y) and one sample (blockIdx.z).
-__global__ void __launch_bounds__(256) columns_join_kernel(const float* __restrict__ parts, int64_t runs, int d,
-                                                           const __grid_constant__ ColumnOutputs out) {
-  __shared__ float meet[8][32];
+constexpr int kSlices = 32;
+
+// Sums v[first + r * stride + col] over r in [0, count) for 32 columns by the block's 32 slices; warp 0 has the result.
+__device__ __forceinline__ float join_parts(const float* v, int64_t count, int64_t stride, bool own) {
+  __shared__ float meet[kSlices][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + lane, c = blockIdx.y;
-  if (out.p[c] == nullptr) return;
-  const int64_t first = blockIdx.z * runs;
-  float v = 0.f;
-  if (col < d)
-    for (int64_t r = runs * slice / 8; r < runs * (slice + 1) / 8; ++r) v += parts[((first + r) * kColumns + c) * d + col];
-  meet[slice][lane] = v;
+  float sum = 0.f;
+  if (own) {
+#pragma unroll 4
+    for (int64_t r = slice; r < count; r += kSlices) sum += v[r * stride];
+  }
+  meet[slice][lane] = sum;
   __syncthreads();
-  if (slice != 0 || col >= d) return;
+  // warp w turns slice sums of column w + ... into one: 32 slices of a column lie in one warp after the transpose
+  float x = meet[lane][slice];
 #pragma unroll
-  for (int u = 1; u < 8; ++u) v += meet[u][lane];
-  store_any(out.p[c], out.dtype[c], blockIdx.z * static_cast<int64_t>(d) + col, v);
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;  // of column `slice`, in every lane
+}
+
+// blockIdx.y: an array of parts[run][array][d] (its sums over all runs).
+__global__ void __launch_bounds__(kSlices * 32) columns_join_kernel(const float* __restrict__ parts, int64_t runs, int d,
+                                                                    const __grid_constant__ ColumnOutputs out) {
+  const int c = blockIdx.y;
+  if (out.p[c] == nullptr) return;
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+  const float v = join_parts(parts + static_cast<int64_t>(c) * d + col, runs, static_cast<int64_t>(kColumns) * d, col < d);
+  const int at = blockIdx.x * 32 + (threadIdx.x >> 5);
+  if ((threadIdx.x & 31) == 0 && at < d) store_any(out.p[c], out.dtype[c], at, v);
+}
+
+// The gates of samples first + blockIdx.y: from gates[worker + sample][d] of `workers` groups of threads.
+__global__ void __launch_bounds__(kSlices * 32) gates_join_kernel(const float* __restrict__ gates, int64_t rows, int64_t seq,
+                                                                  int64_t workers, int64_t first, int d, void* out, int dtype) {
+  const int64_t sample = first + blockIdx.y;
+  const int64_t a = worker_of(sample * seq, rows, workers), b = worker_of((sample + 1) * seq - 1, rows, workers);
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+  const float v = join_parts(gates + (a + sample) * d + col, b - a + 1, d, col < d);
+  const int at = blockIdx.x * 32 + (threadIdx.x >> 5);
+  if ((threadIdx.x & 31) == 0 && at < d) store_any(out, dtype, sample * d + at, v);
+}
+
+// The gates of wide rows: runs per_seq of each sample, array kGate of parts[run][array][d].
+__global__ void __launch_bounds__(kSlices * 32) gate_runs_join_kernel(const float* __restrict__ parts, int64_t per_seq,
+                                                                      int64_t first, int d, void* out, int dtype) {
+  const int64_t sample = first + blockIdx.y;
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+  const float v = join_parts(parts + (sample * per_seq * kColumns + kGate) * d + col, per_seq,
+                             static_cast<int64_t>(kColumns) * d, col < d);
+  const int at = blockIdx.x * 32 + (threadIdx.x >> 5);
+  if ((threadIdx.x & 31) == 0 && at < d) store_any(out, dtype, sample * d + at, v);
 }
 
 struct Runs {
@@ -237,64 +496,131 @@ Runs runs_of(int64_t rows, int64_t seq) {
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
+constexpr int kGradBlocksPerSm = 4;  // of the one-pass kernel at most: bounds the workspace
+constexpr int64_t kMaxGridY = 65535;
+
+int launch_columns_join(const float* parts, int64_t runs, int d, int wanted, ColumnOutputs out, cudaStream_t st) {
+  for (int c = 0; c < kColumns; ++c)
+    if ((wanted & (1 << c)) == 0) out.p[c] = nullptr;
+  if (wanted == 0) return OPUS_OK;
+  columns_join_kernel<<<dim3((d + 31) / 32, kColumns), kSlices * 32, 0, st>>>(parts, runs, d, out);
+  note_launch();
+  OPUS_CUDA_TRY(cudaGetLastError());
+  return OPUS_OK;
+}
+
+template <typename TX, typename TY, int V, int NV, bool Full, bool Bias>
+int launch_one_pass(NormShape s, const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws,
+                    cudaStream_t st) {
+  constexpr auto kernel = grad_kernel<TX, TY, V, NV, Full, Bias>;
+  const int threads = s.group * s.groups;
+  const int arrays = !Full ? 1 : (Bias ? 3 : 2) + (s.seq == s.rows ? 1 : 0);
+  const int shared = (GroupSum::size(s.group, s.groups) + (s.groups > 1 ? threads * V * NV : 0) +
+                      arrays * Param<NV, V, true>::size(s.group)) * static_cast<int>(sizeof(float));
+  const int ready = allow_shared<kernel>(shared);
+  if (ready) return ready;
+  int per_sm = resident_blocks<kernel>(threads, shared);
+  per_sm = per_sm < kGradBlocksPerSm ? per_sm : kGradBlocksPerSm;
+  const int64_t need = (s.rows + s.groups - 1) / s.groups, most = static_cast<int64_t>(sm_count()) * per_sm;
+  s.blocks = static_cast<int>(need < most ? need : most);
+  float* parts = reinterpret_cast<float*>(ws);
+  float* gates = parts + static_cast<int64_t>(s.blocks) * kColumns * s.d;
+  kernel<<<s.blocks, threads, shared, st>>>(s, a, wanted, parts, gates);
+  note_launch();
+  OPUS_CUDA_TRY(cudaGetLastError());
+  const bool per_sample = s.seq != s.rows && (wanted & (1 << kGate)) != 0;
+  const int rc = launch_columns_join(parts, s.blocks, s.d, per_sample ? wanted & ~(1 << kGate) : wanted, out, st);
+  if (rc || !per_sample) return rc;
+  for (int64_t at = 0; at < a.gate_rows; at += kMaxGridY) {
+    const int64_t n = a.gate_rows - at < kMaxGridY ? a.gate_rows - at : kMaxGridY;
+    gates_join_kernel<<<dim3((s.d + 31) / 32, static_cast<unsigned>(n)), kSlices * 32, 0, st>>>(
+        gates, s.rows, s.seq, static_cast<int64_t>(s.blocks) * s.groups, at, s.d, a.grad_gate, a.gate_dtype);
+    note_launch();
+    OPUS_CUDA_TRY(cudaGetLastError());
+  }
+  return OPUS_OK;
+}
+
 template <typename TX, typename TY, int V>
 int launch_columns(const NormShape& s, const opus_residual_norm_args& a, const float2* means, int wanted,
-                   const Runs& r, float* parts, const ColumnOutputs& out, cudaStream_t st) {
+                   const Runs& r, float* parts, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(r.samples * r.per_seq), (s.d / V + 31) / 32);
   columns_kernel<TX, TY, V><<<grid, kColWarps * 32, 0, st>>>(s, a, means, wanted, r.seq, r.run, r.per_seq, parts);
   note_launch();
   OPUS_CUDA_TRY(cudaGetLastError());
-  ColumnOutputs o = out;
-  for (int c = 0; c < kColumns; ++c)
-    if ((wanted & (1 << c)) == 0) o.p[c] = nullptr;
-  // gates of many samples go in slices of the grid's z limit
-  for (int64_t at = 0; at < r.samples; at += 65535) {
-    const int64_t n = r.samples - at < 65535 ? r.samples - at : 65535;
-    columns_join_kernel<<<dim3((s.d + 31) / 32, kColumns, static_cast<unsigned>(n)), 256, 0, st>>>(
-        parts + at * r.per_seq * kColumns * s.d, r.per_seq, s.d, o);
-    note_launch();
-    OPUS_CUDA_TRY(cudaGetLastError());
-    if (o.p[kGate]) o.p[kGate] = static_cast<uint8_t*>(o.p[kGate]) + n * s.d * dtype_bytes(o.dtype[kGate]);
-  }
   return OPUS_OK;
 }
 
 template <typename TX, typename TY, int V, int NV>
-int launch(const NormShape& s, const opus_residual_norm_args& a, int wanted, uint8_t* ws, cudaStream_t st) {
+int launch_wide(NormShape s, const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws,
+                cudaStream_t st) {
   float2* means = reinterpret_cast<float2*>(ws);
   float* parts = reinterpret_cast<float*>(ws + align256(s.rows * 8));
-  const int threads = (s.group * s.groups + 31) / 32 * 32;
-  int64_t blocks = (s.rows + s.groups - 1) / s.groups;
-  const int64_t most = static_cast<int64_t>(sm_count()) * (2048 / threads);
-  if (blocks > most) blocks = most;
-  rows_kernel<TX, TY, V, NV><<<static_cast<unsigned>(blocks), threads, 4 * (threads / 32) * sizeof(float), st>>>(s, a, means);
+  constexpr auto kernel = rows_kernel<TX, TY, V, NV>;
+  const int threads = s.group * s.groups;
+  const int shared = GroupSum::size(s.group, s.groups) * static_cast<int>(sizeof(float));
+  const int64_t need = (s.rows + s.groups - 1) / s.groups;
+  const int64_t most = static_cast<int64_t>(sm_count()) * resident_blocks<kernel>(threads, shared);
+  s.blocks = static_cast<int>(need < most ? need : most);
+  kernel<<<s.blocks, threads, shared, st>>>(s, a, means);
   note_launch();
   OPUS_CUDA_TRY(cudaGetLastError());
-  const ColumnOutputs out{{a.grad_weight, a.grad_bias, a.grad_post_weight, a.grad_post_bias, a.grad_gate},
-                          {a.weight_dtype, a.bias_dtype, a.post_weight_dtype, a.post_bias_dtype, a.gate_dtype}};
   // sums over all rows, then the gates of several samples in runs of their own
-  const bool gates = a.gate_rows > 1 && (wanted & (1 << kGate)) != 0;
-  const int whole = gates ? wanted & ~(1 << kGate) : wanted;
+  const bool per_sample = s.seq != s.rows && (wanted & (1 << kGate)) != 0;
+  const int whole = per_sample ? wanted & ~(1 << kGate) : wanted;
+  int rc = OPUS_OK;
   if (whole != 0) {
-    const int rc = launch_columns<TX, TY, V>(s, a, means, whole, runs_of(s.rows, s.rows), parts, out, st);
-    if (rc) return rc;
+    const Runs r = runs_of(s.rows, s.rows);
+    rc = launch_columns<TX, TY, V>(s, a, means, whole, r, parts, st);
+    if (rc == OPUS_OK) rc = launch_columns_join(parts, r.per_seq, s.d, whole, out, st);
   }
-  if (gates) return launch_columns<TX, TY, V>(s, a, means, 1 << kGate, runs_of(s.rows, s.seq), parts, out, st);
-  return OPUS_OK;
+  if (rc || !per_sample) return rc;
+  const Runs r = runs_of(s.rows, s.seq);
+  rc = launch_columns<TX, TY, V>(s, a, means, 1 << kGate, r, parts, st);
+  for (int64_t at = 0; rc == OPUS_OK && at < r.samples; at += kMaxGridY) {
+    const int64_t n = r.samples - at < kMaxGridY ? r.samples - at : kMaxGridY;
+    gate_runs_join_kernel<<<dim3((s.d + 31) / 32, static_cast<unsigned>(n)), kSlices * 32, 0, st>>>(
+        parts, r.per_seq, at, s.d, a.grad_gate, a.gate_dtype);
+    note_launch();
+    OPUS_CUDA_TRY(cudaGetLastError());
+  }
+  return rc;
+}
+
+template <typename TX, typename TY, int V, int NV>
+int launch_pass(const NormShape& s, const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws,
+                cudaStream_t st) {
+  const bool bias = a.post_bias != nullptr || (wanted & (1 << kBias)) != 0;
+  if (a.post || a.gate != nullptr)
+    return bias ? launch_one_pass<TX, TY, V, NV, true, true>(s, a, wanted, out, ws, st)
+                : launch_one_pass<TX, TY, V, NV, true, false>(s, a, wanted, out, ws, st);
+  return bias ? launch_one_pass<TX, TY, V, NV, false, true>(s, a, wanted, out, ws, st)
+              : launch_one_pass<TX, TY, V, NV, false, false>(s, a, wanted, out, ws, st);
+}
+
+template <typename TX, typename TY, int V>
+int launch_by_width(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
+  constexpr int kMost = 16 / V;
+  NormShape s;
+  int nv;
+  const bool wide = a.d > kNormNarrow;
+  const int rc = norm_shape("residual_norm_grad", &a, V, wide ? wide_vectors(V) : kMost, &s, &nv);
+  if (rc) return rc;
+  if (wide) return launch_wide<TX, TY, V, wide_vectors(V)>(s, a, wanted, out, ws, st);
+  if constexpr (V > 1) {
+    if (nv == 1) return launch_pass<TX, TY, V, 1>(s, a, wanted, out, ws, st);
+  }
+  if constexpr (V < 8) {
+    if (nv <= 4 / (V == 4 ? 2 : 1)) return launch_pass<TX, TY, V, 4 / (V == 4 ? 2 : 1)>(s, a, wanted, out, ws, st);
+  }
+  return launch_pass<TX, TY, V, kMost>(s, a, wanted, out, ws, st);
 }
 
 template <typename TX, typename TY>
-int launch_by_width(const opus_residual_norm_args& a, bool vec, int wanted, uint8_t* ws, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(TX);
-  NormShape s;
-  int nv;
-  const int rc = norm_shape("residual_norm_grad", &a, vec, V, &s, &nv);
-  if (rc) return rc;
-  if (!vec) return nv == 4 ? launch<TX, TY, 1, 4>(s, a, wanted, ws, st) : launch<TX, TY, 1, 16>(s, a, wanted, ws, st);
-  if (nv == 1) return launch<TX, TY, V, 1>(s, a, wanted, ws, st);
-  if (nv == 2) return launch<TX, TY, V, 2>(s, a, wanted, ws, st);
-  if constexpr (V == 4) return launch<TX, TY, V, 4>(s, a, wanted, ws, st);
-  return set_error(OPUS_ERR_UNSUPPORTED, "residual_norm_grad: d = %d", a.d);
+int launch_by_alignment(const opus_residual_norm_args& a, bool vec, int wanted, const ColumnOutputs& out, uint8_t* ws,
+                        cudaStream_t st) {
+  return vec ? launch_by_width<TX, TY, 16 / sizeof(TX)>(a, wanted, out, ws, st)
+             : launch_by_width<TX, TY, 1>(a, wanted, out, ws, st);
 }
 
 bool on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -306,13 +632,24 @@ using namespace opus;
 
 extern "C" int64_t opus_residual_norm_grad_workspace_bytes(const opus_residual_norm_args* a) {
   if (a == nullptr || a->rows <= 0 || a->d < 1) return 256;
+  const int64_t samples = a->gate != nullptr && a->gate_rows > 1 && a->rows % a->gate_rows == 0 ? a->gate_rows : 0;
   const Runs whole = runs_of(a->rows, a->rows);
   int64_t runs = whole.samples * whole.per_seq;
-  if (a->gate != nullptr && a->gate_rows > 1 && a->rows % a->gate_rows == 0) {
-    const Runs r = runs_of(a->rows, a->rows / a->gate_rows);
+  if (samples > 0) {
+    const Runs r = runs_of(a->rows, a->rows / samples);
     if (r.samples * r.per_seq > runs) runs = r.samples * r.per_seq;
   }
-  return align256(a->rows * 8) + align256(runs * kColumns * a->d * 4);
+  const int64_t wide = align256(a->rows * 8) + align256(runs * kColumns * a->d * 4);
+  // the one-pass kernel: a block holds at most 256 rows, and no more blocks run than there are rows
+  int64_t blocks = static_cast<int64_t>(sm_count()) * kGradBlocksPerSm;
+  blocks = blocks < a->rows ? blocks : a->rows;
+  int64_t workers = 0;
+  if (samples > 0) {
+    workers = blocks * (a->d > 2048 ? 1 : a->d > 256 ? 8 : 256);
+    workers = (workers < a->rows + 256 ? workers : a->rows + 256) + samples;
+  }
+  const int64_t one_pass = align256((blocks * kColumns + workers) * a->d * 4);
+  return wide > one_pass ? wide : one_pass;
 }
 
 extern "C" int opus_residual_norm_grad(const opus_residual_norm_args* args, void* workspace, int64_t workspace_bytes,
@@ -350,16 +687,17 @@ extern "C" int opus_residual_norm_grad(const opus_residual_norm_args* args, void
       !on(a.grad_y, yb) || !on(a.stats, 16))
     return set_error(OPUS_ERR_INVALID, "residual_norm_grad: a pointer is not aligned to its elements");
   const int V = 16 / xb;
-  const bool vec = a.d % V == 0 && a.h_stride % V == 0 && on(a.h, 16) && on(a.grad_x, 16) && on(a.grad_y, V * yb) &&
+  const bool vec = norm_params_aligned(&a) && a.d % V == 0 && a.h_stride % V == 0 && on(a.h, 16) && on(a.grad_x, 16) && on(a.grad_y, V * yb) &&
                    (!a.y || (a.y_stride % V == 0 && on(a.y, V * yb))) &&
                    (!a.grad_n || (a.grad_n_stride % V == 0 && on(a.grad_n, V * yb))) &&
                    (!a.grad_h || (a.grad_h_stride % V == 0 && on(a.grad_h, 16)));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const ColumnOutputs out{{outs[0], outs[1], outs[2], outs[3], outs[4]}, {types[0], types[1], types[2], types[3], types[4]}};
   if (a.x_dtype == OPUS_DTYPE_F32) {
-    if (a.y_dtype == OPUS_DTYPE_F32) return launch_by_width<float, float>(a, vec, wanted, ws, st);
-    if (a.y_dtype == OPUS_DTYPE_F16) return launch_by_width<float, __half>(a, vec, wanted, ws, st);
-    return launch_by_width<float, __nv_bfloat16>(a, vec, wanted, ws, st);
+    if (a.y_dtype == OPUS_DTYPE_F32) return launch_by_alignment<float, float>(a, vec, wanted, out, ws, st);
+    if (a.y_dtype == OPUS_DTYPE_F16) return launch_by_alignment<float, __half>(a, vec, wanted, out, ws, st);
+    return launch_by_alignment<float, __nv_bfloat16>(a, vec, wanted, out, ws, st);
   }
-  if (a.x_dtype == OPUS_DTYPE_F16) return launch_by_width<__half, __half>(a, vec, wanted, ws, st);
-  return launch_by_width<__nv_bfloat16, __nv_bfloat16>(a, vec, wanted, ws, st);
+  if (a.x_dtype == OPUS_DTYPE_F16) return launch_by_alignment<__half, __half>(a, vec, wanted, out, ws, st);
+  return launch_by_alignment<__nv_bfloat16, __nv_bfloat16>(a, vec, wanted, out, ws, st);
 }
