@@ -84,16 +84,21 @@ __global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : 3)
   const int t = threadIdx.x % s.group;
   const int g = threadIdx.x / s.group;
   const RowRun run(s.rows, static_cast<int64_t>(blockIdx.x) * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
+  const Columns<V, NV> c(s, t);
   const TX* x = static_cast<const TX*>(a.x) + run.first * a.x_stride;
   const TY* y = static_cast<const TY*>(a.y) + (F != kAlone ? run.first * a.y_stride : 0);
-  TX* h = static_cast<TX*>(a.h) + run.first * s.d;
-  TY* n = static_cast<TY*>(a.n) + run.first * s.d;
+  TX* hp = static_cast<TX*>(a.h) + run.first * s.d;
+  TY* np = static_cast<TY*>(a.n) + run.first * s.d;
   RawRow<TX, V, NV> xr;
   RawRow<TY, V, NV> yr;
-  xr.load(run.first < run.last ? x : nullptr, s, t);
-  if constexpr (F != kAlone) yr.load(run.first < run.last ? y : nullptr, s, t);
-  GroupSum sum(shared, s.group, s.groups);
-  float* place = shared + GroupSum::size(s.group, s.groups);
+  xr.zero();
+  yr.zero();
+  if (run.first < run.last) {
+    xr.load(x, c);
+    if constexpr (F != kAlone) yr.load(y, c);
+  }
+  GroupSum<norm_sub_warp(V, NV)> sum(shared, s.group, s.groups);
+  float* place = shared + group_floats(s.group, s.groups);
   Param<NV, V, Near> w(a.weight, a.weight_dtype, 1.f), b(a.bias, a.bias_dtype, 0.f);
   Param<NV, V, Near> pw(a.post_weight, a.post_weight_dtype, 1.f), pb(a.post_bias, a.post_bias_dtype, 0.f);
   Param<NV, V, Near> q(a.gate, a.gate_dtype, 1.f);
@@ -106,76 +111,65 @@ __global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : 3)
     if (one_gate) q.fill(&place, s);
   }
   __syncthreads();
-  int64_t until = run.first / s.seq * s.seq, gate_at = 0;  // first row of the next sample
-  for (int i = 0; i < run.rounds; ++i) {
-    const int64_t row = run.first + i;
-    const bool live = row < run.last;
-    RawRow<TX, V, NV> hr = xr;
-    RawRow<TY, V, NV> zr;
+  int64_t until = 0, gate_at = 0;  // the first row of the next sample, this sample's gate
+  for (int64_t row = run.first; row < run.last; ++row) {
+    float h[NV][V], u[NV][V];
+    xr.get(h);
+    if constexpr (F != kAlone) yr.get(u);
     x += a.x_stride;
-    xr.load(row + 1 < run.last ? x : nullptr, s, t);
-    if constexpr (F != kAlone) {
-      zr = yr;
-      y += a.y_stride;
-      yr.load(row + 1 < run.last ? y : nullptr, s, t);
+    if constexpr (F != kAlone) y += a.y_stride;
+    if (row + 1 < run.last) {
+      xr.load(x, c);
+      if constexpr (F != kAlone) yr.load(y, c);
     }
     float2 ys = make_float2(0.f, 1.f);
-    float u[NV][V];
     if constexpr (F == kFull) {
-      if (a.post) ys = zr.stats(s, t, sum);
+      float p[NV][V];
+      if (a.post) {
+        ys = row_stats(u, s, c, t, sum);
+        float o[NV][V];
+        pw.row(c, p);
+        pb.row(c, o);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) u[k][j] = fmaf((u[k][j] - ys.x) * ys.y, p[k][j], o[k][j]);
+      }
       if (one_gate) {
-        q.row(s, t, u);
+        q.row(c, p);
       } else {
-        if (row >= until && live) {
+        if (row >= until) {
           gate_at = row / s.seq * s.d;
           until = (row / s.seq + 1) * s.seq;
         }
-        load_param_row(a.gate, a.gate_dtype, gate_at, 1.f, s, t, u);
+        load_param_row(a.gate, a.gate_dtype, gate_at, 1.f, c, p);
       }
-      float p[NV][V], o[NV][V];
-      pw.row(s, t, p);
-      pb.row(s, t, o);
-      // z = u ((y - mean) / sd p + o)
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float z[V];
-        zr.v[k].get(z);
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) u[k][j] *= fmaf((z[j] - ys.x) * ys.y, p[k][j], o[k][j]);
-      }
+        for (int j = 0; j < V; ++j) u[k][j] *= p[k][j];
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      float r[V];
-      hr.v[k].get(r);
-      if constexpr (F == kJoin) zr.v[k].get(u[k]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) r[j] = F == kAlone ? a.residual_scale * r[j] : fmaf(a.residual_scale, r[j], u[k][j]);
-      hr.v[k].set(r);
-      const int col = (k * s.group + t) * V;
-      if (live && col < s.d && (F != kAlone || a.h != nullptr)) *reinterpret_cast<Vec<TX, V>*>(h + col) = hr.v[k];
+      for (int j = 0; j < V; ++j) h[k][j] = F == kAlone ? a.residual_scale * h[k][j] : fmaf(a.residual_scale, h[k][j], u[k][j]);
+      Vec<TX, V> stored;
+      stored.set(h[k]);
+      stored.get(h[k]);  // what is normed is what is stored
+      if (c.own[k] && (F != kAlone || a.h != nullptr)) *reinterpret_cast<Vec<TX, V>*>(hp + c.at[k]) = stored;
     }
-    h += s.d;
-    const float2 hs = hr.stats(s, t, sum);
-    float p[NV][V], o[NV][V];
-    w.row(s, t, p);
-    b.row(s, t, o);
+    hp += s.d;
+    const float2 hs = row_stats(h, s, c, t, sum);
+    float o[NV][V];
+    w.row(c, u);
+    b.row(c, o);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float r[V];
-      hr.v[k].get(r);
-      if (s.layer) {
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) r[j] = fmaf((r[j] - hs.x) * hs.y, p[k][j], o[k][j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) r[j] = fmaf(r[j] * hs.y, p[k][j], o[k][j]);
-      }
-      const int col = (k * s.group + t) * V;
-      if (live && col < s.d) store_vec<TY, V>(n + col, r);
-    }
-    n += s.d;
-    if (live && t == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
+      for (int j = 0; j < V; ++j) h[k][j] = fmaf((h[k][j] - hs.x) * hs.y, u[k][j], o[k][j]);
+    store_row(np, c, h);
+    np += s.d;
+    if (t == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
   }
 }
 
@@ -184,7 +178,7 @@ int launch(NormShape s, const opus_residual_norm_args& a, cudaStream_t st) {
   constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Near, Wide>;
   const int threads = s.group * s.groups;
   const int arrays = F != kFull ? 2 : s.seq == s.rows ? 5 : 4;
-  const int shared = (GroupSum::size(s.group, s.groups) + arrays * Param<NV, V, Near>::size(s.group)) * static_cast<int>(sizeof(float));
+  const int shared = (group_floats(s.group, s.groups) + arrays * Param<NV, V, Near>::size(s.group)) * static_cast<int>(sizeof(float));
   const int rc = allow_shared<kernel>(shared);
   if (rc) return rc;
   const int64_t need = (s.rows + s.groups - 1) / s.groups;

@@ -37,54 +37,54 @@ struct NormShape {
   int blocks;  // of the launch
 };
 
-// The rows [first, last) of worker w among n, and how many rounds the longest run takes.
+// The rows [first, last) of worker w among n.
 struct RowRun {
   int64_t first, last;
-  int rounds;
   __device__ RowRun(int64_t rows, int64_t w, int64_t n) {
     const int64_t each = rows / n, more = rows % n;
     first = w * each + (w < more ? w : more);
     last = first + each + (w < more ? 1 : 0);
-    rounds = static_cast<int>(each + (more > 0 ? 1 : 0));
   }
 };
 
+// Shared memory of a group's sums: slots of its warps (a multiple of 4), twice for two values, twice for two turns.
+__host__ __device__ constexpr int group_slots(int group) { return group <= 32 ? 0 : ((group >> 5) + 3) / 4 * 4; }
+__host__ __device__ constexpr int group_floats(int group, int groups) { return 4 * groups * group_slots(group); }
+
+// Whether a thread's group may be less than a warp (norm_shape's smallest vector counts).
+constexpr bool norm_sub_warp(int V, int NV) { return NV == 1 || (V == 1 && NV == 4); }
+
 // Sums over the group of up to two values each, in a fixed order; the result is in every thread of the group.
 // A call takes one barrier of the group's own: `turn` alternates between two buffers.
+template <bool SubWarp>
 struct GroupSum {
   float* buf;
-  int width, slots, span, barrier, threads;
+  int slots, span, barrier, threads;
+  unsigned lanes;
   int turn;
 
-  // floats of shared memory
-  static __host__ __device__ int size(int group, int groups) {
-    return group <= 32 ? 0 : 2 * 2 * groups * (((group >> 5) + 3) / 4 * 4);
-  }
   // every thread of the block calls it once
-  __device__ GroupSum(float* shared, int group, int groups) : turn(0) {
-    width = group < 32 ? group : 32;
-    slots = group <= 32 ? 0 : ((group >> 5) + 3) / 4 * 4;  // of the group's warps, zeros behind them
+  __device__ GroupSum(float* shared, int group, int groups) : threads(group), lanes(0xffffffffu), turn(0) {
+    slots = group_slots(group);  // of the group's warps, zeros behind them
     span = groups * slots;
     const int g = static_cast<int>(threadIdx.x) / group;
     buf = shared + g * slots;
     barrier = 1 + g;  // named barriers 1 to 15: a block has at most 4 groups of more than a warp
-    threads = group;
-    if (slots) {
-      for (int i = threadIdx.x; i < 4 * span; i += blockDim.x) shared[i] = 0.f;
-      __syncthreads();
-    }
+    if (SubWarp && group < 32) lanes = ((1u << group) - 1) << ((threadIdx.x & 31) / group * group);
+    for (int i = threadIdx.x; i < 4 * span; i += blockDim.x) shared[i] = 0.f;
+    __syncthreads();
   }
   template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N], int t) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      if (o >= width) continue;
+      if (SubWarp && o >= threads) continue;
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(lanes, v[i], o);
     }
     if (slots == 0) return;
-    float* b = buf + turn * 2 * span;
-    turn ^= 1;
+    float* b = buf + turn;
+    turn = 2 * span - turn;
     if ((t & 31) == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) b[i * span + (t >> 5)] = v[i];
@@ -92,12 +92,27 @@ struct GroupSum {
     asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float s = 0.f;
-      for (int w = 0; w < slots; w += 4) {
-        const float4 q = *reinterpret_cast<const float4*>(b + i * span + w);
-        s += (q.x + q.y) + (q.z + q.w);
+      const float4 q = *reinterpret_cast<const float4*>(b + i * span);
+      float s = (q.x + q.y) + (q.z + q.w);
+      for (int w = 4; w < slots; w += 4) {
+        const float4 r = *reinterpret_cast<const float4*>(b + i * span + w);
+        s += (r.x + r.y) + (r.z + r.w);
       }
       v[i] = s;
+    }
+  }
+};
+
+// Which columns a thread holds.
+template <int V, int NV>
+struct Columns {
+  int at[NV];
+  bool own[NV];
+  __device__ Columns(const NormShape& s, int t) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      at[k] = (k * s.group + t) * V;
+      own[k] = at[k] < s.d;
     }
   }
 };
@@ -106,44 +121,53 @@ struct GroupSum {
 template <typename T, int V, int NV>
 struct RawRow {
   Vec<T, V> v[NV];
-  __device__ __forceinline__ void load(const T* row, const NormShape& s, int t) {
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (k * s.group + t) * V;
-      if (row != nullptr && col < s.d) v[k] = *reinterpret_cast<const Vec<T, V>*>(row + col);
-      else v[k].zero();
-    }
+    for (int k = 0; k < NV; ++k) v[k].zero();
   }
-  // mean (0 for an RMS norm) and 1 / sqrt(mean square about it + eps) of the row
-  __device__ __forceinline__ float2 stats(const NormShape& s, int t, GroupSum& sum) const {
-    const float inv_d = 1.0f / static_cast<float>(s.d);
-    float mean = 0.f;
-    if (s.layer) {
-      float a[1] = {0.f};
+  __device__ __forceinline__ void load(const T* row, const Columns<V, NV>& c) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float r[V];
-        v[k].get(r);
+    for (int k = 0; k < NV; ++k)
+      if (c.own[k]) v[k] = *reinterpret_cast<const Vec<T, V>*>(row + c.at[k]);
+  }
+  __device__ __forceinline__ void get(float (&r)[NV][V]) const {
 #pragma unroll
-        for (int i = 0; i < V; ++i) a[0] += r[i];
-      }
-      sum(a, t);
-      mean = a[0] * inv_d;
-    }
-    float q[2] = {0.f, 0.f};  // two chains
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const float m = (k * s.group + t) * V < s.d ? mean : 0.f;
-      float r[V];
-      v[k].get(r);
-#pragma unroll
-      for (int i = 0; i < V; ++i) q[i & 1] = fmaf(r[i] - m, r[i] - m, q[i & 1]);
-    }
-    float whole[1] = {q[0] + q[1]};
-    sum(whole, t);
-    return make_float2(mean, rsqrtf(whole[0] * inv_d + s.eps));
+    for (int k = 0; k < NV; ++k) v[k].get(r[k]);
   }
 };
+
+template <typename T, int V, int NV>
+__device__ __forceinline__ void store_row(T* row, const Columns<V, NV>& c, const float (&r)[NV][V]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (c.own[k]) store_vec<T, V>(row + c.at[k], r[k]);
+}
+
+// mean (0 for an RMS norm) and 1 / sqrt(mean square about it + eps) of a row (zeros beyond it)
+template <int V, int NV, typename Sum>
+__device__ __forceinline__ float2 row_stats(const float (&r)[NV][V], const NormShape& s, const Columns<V, NV>& c, int t, Sum& sum) {
+  const float inv_d = 1.0f / static_cast<float>(s.d);
+  float mean = 0.f;
+  if (s.layer) {
+    float a[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[0] += r[k][i];
+    sum(a, t);
+    mean = a[0] * inv_d;
+  }
+  float q[2] = {0.f, 0.f};  // two chains
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const float m = c.own[k] ? mean : 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i & 1] = fmaf(r[k][i] - m, r[k][i] - m, q[i & 1]);
+  }
+  float whole[1] = {q[0] + q[1]};
+  sum(whole, t);
+  return make_float2(mean, rsqrtf(whole[0] * inv_d + s.eps));
+}
 
 // V neighbours of an array whose type is known at run time, in accesses of up to 16 bytes (V > 1: aligned arrays).
 template <typename T, int V>
@@ -167,24 +191,22 @@ __device__ __forceinline__ void load_param_vec(const void* p, int dtype, int64_t
 // A thread's part of one of the parameters' rows, from where it is (`other` where there is none, 0 beyond the row).
 // The branches on the type enclose all of a thread's loads.
 template <typename T, int NV, int V>
-__device__ __forceinline__ void load_param_row_as(const void* p, int64_t at, const NormShape& s, int t, float (&r)[NV][V]) {
+__device__ __forceinline__ void load_param_row_as(const void* p, int64_t at, const Columns<V, NV>& c, float (&r)[NV][V]) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int col = (k * s.group + t) * V;
-    if (col < s.d) load_param_as<T, V>(p, at + col, r[k]);
-  }
+  for (int k = 0; k < NV; ++k)
+    if (c.own[k]) load_param_as<T, V>(p, at + c.at[k], r[k]);
 }
 template <int NV, int V>
-__device__ __forceinline__ void load_param_row(const void* p, int dtype, int64_t at, float other, const NormShape& s, int t,
+__device__ __forceinline__ void load_param_row(const void* p, int dtype, int64_t at, float other, const Columns<V, NV>& c,
                                                float (&r)[NV][V]) {
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) r[k][i] = (k * s.group + t) * V < s.d ? other : 0.f;
+    for (int i = 0; i < V; ++i) r[k][i] = c.own[k] ? other : 0.f;
   if (p == nullptr) return;
-  if (dtype == OPUS_DTYPE_F32) load_param_row_as<float>(p, at, s, t, r);
-  else if (dtype == OPUS_DTYPE_F16) load_param_row_as<__half>(p, at, s, t, r);
-  else load_param_row_as<__nv_bfloat16>(p, at, s, t, r);
+  if (dtype == OPUS_DTYPE_F32) load_param_row_as<float>(p, at, c, r);
+  else if (dtype == OPUS_DTYPE_F16) load_param_row_as<__half>(p, at, c, r);
+  else load_param_row_as<__nv_bfloat16>(p, at, c, r);
 }
 
 // A parameter of d elements that rows share.  Near: as f32 in shared memory, `other` where there is none and 0
@@ -195,14 +217,16 @@ struct Param {
   const void* p;
   int dtype;
   float other;
-  float* near;
-  __device__ __forceinline__ Param(const void* p_, int dtype_, float other_) : p(p_), dtype(dtype_), other(other_), near(nullptr) {}
+  float *near, *far;  // the two planes
+  __device__ __forceinline__ Param(const void* p_, int dtype_, float other_)
+      : p(p_), dtype(dtype_), other(other_), near(nullptr), far(nullptr) {}
   static __host__ __device__ int size(int group) { return Near ? group * NV * V : 0; }
   // by every thread; a barrier has to follow
   __device__ __forceinline__ void fill(float** shared, const NormShape& s) {
     if constexpr (Near) {
       near = *shared;
       const int whole = size(s.group);
+      far = near + whole / 2;
       *shared += whole;
       for (int col = threadIdx.x * V; col < whole; col += blockDim.x * V) {
         float r[V];
@@ -211,27 +235,26 @@ struct Param {
         if (p != nullptr && col < s.d) load_param_vec<V>(p, dtype, col, r);
         if constexpr (V == 8) {
           *reinterpret_cast<float4*>(near + col / 2) = make_float4(r[0], r[1], r[2], r[3]);
-          *reinterpret_cast<float4*>(near + (whole + col) / 2) = make_float4(r[4], r[5], r[6], r[7]);
+          *reinterpret_cast<float4*>(far + col / 2) = make_float4(r[4], r[5], r[6], r[7]);
         } else {
           store_vec<float, V>(near + col, r);
         }
       }
     }
   }
-  __device__ __forceinline__ void row(const NormShape& s, int t, float (&r)[NV][V]) const {
+  __device__ __forceinline__ void row(const Columns<V, NV>& c, float (&r)[NV][V]) const {
     if constexpr (!Near) {
-      load_param_row(p, dtype, 0, other, s, t, r);
+      load_param_row(p, dtype, 0, other, c, r);
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int col = (k * s.group + t) * V;
         if constexpr (V == 8) {
-          const float4 a = *reinterpret_cast<const float4*>(near + col / 2);
-          const float4 b = *reinterpret_cast<const float4*>(near + (size(s.group) + col) / 2);
+          const float4 a = *reinterpret_cast<const float4*>(near + c.at[k] / 2);
+          const float4 b = *reinterpret_cast<const float4*>(far + c.at[k] / 2);
           r[k][0] = a.x, r[k][1] = a.y, r[k][2] = a.z, r[k][3] = a.w;
           r[k][4] = b.x, r[k][5] = b.y, r[k][6] = b.z, r[k][7] = b.w;
         } else {
-          load_vec<float, V>(near + col, r[k]);
+          load_vec<float, V>(near + c.at[k], r[k]);
         }
       }
     }

@@ -41,6 +41,7 @@ __global__ void __launch_bounds__(norm_threads(V, false))
   const int g = threadIdx.x / s.group;
   const int64_t worker = static_cast<int64_t>(blockIdx.x) * s.groups + g;
   const RowRun run(s.rows, worker, static_cast<int64_t>(s.blocks) * s.groups);
+  const Columns<V, NV> c(s, t);
   const TX* hp = static_cast<const TX*>(a.h) + run.first * a.h_stride;
   const TX* dhp = static_cast<const TX*>(a.grad_h) + run.first * a.grad_h_stride;
   const TY* dnp = static_cast<const TY*>(a.grad_n) + run.first * a.grad_n_stride;
@@ -51,18 +52,18 @@ __global__ void __launch_bounds__(norm_threads(V, false))
   RawRow<TX, V, NV> hr, dhr;
   RawRow<TY, V, NV> dnr, yr;
   float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);
-  const auto fetch = [&](int64_t row) {
-    const bool live = row < run.last;
-    hr.load(live ? hp : nullptr, s, t);
-    dnr.load(live && a.grad_n != nullptr ? dnp : nullptr, s, t);
-    dhr.load(live && a.grad_h != nullptr ? dhp : nullptr, s, t);
-    if constexpr (Full) yr.load(live ? yp : nullptr, s, t);
-    if (live) ahead = *stats;
+  hr.zero(), dhr.zero(), dnr.zero(), yr.zero();
+  const auto fetch = [&]() {
+    hr.load(hp, c);
+    if (a.grad_n != nullptr) dnr.load(dnp, c);
+    if (a.grad_h != nullptr) dhr.load(dhp, c);
+    if constexpr (Full) yr.load(yp, c);
+    ahead = *stats;
     hp += a.h_stride, dhp += a.grad_h_stride, dnp += a.grad_n_stride, yp += a.y_stride, ++stats;
   };
-  fetch(run.first);
-  GroupSum sum(shared, s.group, s.groups);
-  float* meet = shared + GroupSum::size(s.group, s.groups);
+  if (run.first < run.last) fetch();
+  GroupSum<norm_sub_warp(V, NV)> sum(shared, s.group, s.groups);
+  float* meet = shared + group_floats(s.group, s.groups);
   float* place = meet + (s.groups > 1 ? blockDim.x * V * NV : 0);
   const bool one_gate = s.seq == s.rows;
   Param<NV, V, true> w(a.weight, a.weight_dtype, 1.f), q(a.gate, a.gate_dtype, 1.f);
@@ -87,118 +88,91 @@ __global__ void __launch_bounds__(norm_threads(V, false))
       if (sample < 0 || (wanted & (1 << kGate)) == 0) return;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int col = (k * s.group + t) * V;
-        if (col < s.d) store_vec<float, V>(gates + (worker + sample) * s.d + col, acc_g[k]);
+        if (c.own[k]) store_vec<float, V>(gates + (worker + sample) * s.d + c.at[k], acc_g[k]);
       }
       clear(acc_g);
     }
   };
-  for (int i = 0; i < run.rounds; ++i) {
-    const int64_t row = run.first + i;
-    const bool live = row < run.last;
-    const RawRow<TX, V, NV> h = hr, in = dhr;
-    const RawRow<TY, V, NV> dn = dnr, y = yr;
+  for (int64_t row = run.first; row < run.last; ++row) {
+    float hat[NV][V], u[NV][V], r[NV][V], y[NV][V], f[NV][V];
+    hr.get(hat);
+    dnr.get(u);
+    dhr.get(r);
+    if constexpr (Full) yr.get(y);
     const float4 st = ahead;
-    fetch(row + 1);
-    float u[NV][V];
+    if (row + 1 < run.last) fetch();
     float m[2] = {0.f, 0.f};
-    w.row(s, t, u);
+    w.row(c, f);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float hat[V], v[V];
-      h.v[k].get(hat);
-      dn.v[k].get(v);
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        hat[j] = (hat[j] - st.x) * st.y;
-        acc_w[k][j] = fmaf(v[j], hat[j], acc_w[k][j]);
-        if constexpr (Bias) acc_b[k][j] += v[j];
-        u[k][j] *= v[j];
+        hat[k][j] = (hat[k][j] - st.x) * st.y;
+        acc_w[k][j] = fmaf(u[k][j], hat[k][j], acc_w[k][j]);
+        if constexpr (Bias) acc_b[k][j] += u[k][j];
+        u[k][j] *= f[k][j];
         m[0] += u[k][j];
-        m[1] = fmaf(u[k][j], hat[j], m[1]);
+        m[1] = fmaf(u[k][j], hat[k][j], m[1]);
       }
-    }
     sum(m, t);
     m[0] = s.layer ? m[0] * inv_d : 0.f;
-    m[1] *= inv_d * st.y;  // times 1 / sd: hat is taken apart below
+    m[1] *= inv_d;
     // dh in u
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float hat[V], r[V];
-      h.v[k].get(hat);
-      in.v[k].get(r);
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        u[k][j] = fmaf(st.y, u[k][j] - m[0] - (hat[j] - st.x) * m[1], r[j]);
-        r[j] = a.residual_scale * u[k][j];
+        u[k][j] = fmaf(st.y, u[k][j] - m[0] - hat[k][j] * m[1], r[k][j]);
+        r[k][j] = a.residual_scale * u[k][j];
       }
-      const int col = (k * s.group + t) * V;
-      if (live && col < s.d) store_vec<TX, V>(dx + col, r);
-    }
+    store_row(dx, c, r);
     dx += s.d;
     if constexpr (Full) {
-      float e[NV][V];
       if (one_gate) {
-        q.row(s, t, e);
+        q.row(c, r);
       } else {
-        if (live && row >= until) {
+        if (row >= until) {
           flush_gate();
           sample = row / s.seq;
           until = (sample + 1) * s.seq;
         }
-        load_param_row(a.gate, a.gate_dtype, (sample < 0 ? 0 : sample) * s.d, 1.f, s, t, e);
+        load_param_row(a.gate, a.gate_dtype, sample * s.d, 1.f, c, r);
       }
       if (!a.post) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          float z[V];
-          y.v[k].get(z);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            acc_g[k][j] = fmaf(u[k][j], z[j], acc_g[k][j]);
-            u[k][j] *= e[k][j];
+            acc_g[k][j] = fmaf(u[k][j], y[k][j], acc_g[k][j]);
+            u[k][j] *= r[k][j];
           }
-        }
       } else {
-        float f[NV][V], o[NV][V];
-        pw.row(s, t, f);
-        if constexpr (Bias) pb.row(s, t, o);
+        pw.row(c, f);
+        if constexpr (Bias) pb.row(c, hat);
         float p[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          float z[V];
-          y.v[k].get(z);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            z[j] = (z[j] - st.z) * st.w;  // normed y
-            acc_g[k][j] = fmaf(u[k][j], Bias ? fmaf(z[j], f[k][j], o[k][j]) : z[j] * f[k][j], acc_g[k][j]);
-            const float dz = u[k][j] * e[k][j];
-            acc_pw[k][j] = fmaf(dz, z[j], acc_pw[k][j]);
+            y[k][j] = (y[k][j] - st.z) * st.w;  // normed y
+            acc_g[k][j] = fmaf(u[k][j], Bias ? fmaf(y[k][j], f[k][j], hat[k][j]) : y[k][j] * f[k][j], acc_g[k][j]);
+            const float dz = u[k][j] * r[k][j];
+            acc_pw[k][j] = fmaf(dz, y[k][j], acc_pw[k][j]);
             if constexpr (Bias) acc_pb[k][j] += dz;
             u[k][j] = dz * f[k][j];
             p[0] += u[k][j];
-            p[1] = fmaf(u[k][j], z[j], p[1]);
+            p[1] = fmaf(u[k][j], y[k][j], p[1]);
           }
-        }
         sum(p, t);
         p[0] = s.layer ? p[0] * inv_d : 0.f;
-        p[1] *= inv_d * st.w;
+        p[1] *= inv_d;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          float z[V];
-          y.v[k].get(z);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) u[k][j] = st.w * (u[k][j] - p[0] - (z[j] - st.z) * p[1]);
-        }
+          for (int j = 0; j < V; ++j) u[k][j] = st.w * (u[k][j] - p[0] - y[k][j] * p[1]);
       }
     }
-    if (live && a.grad_y != nullptr) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int col = (k * s.group + t) * V;
-        if (col < s.d) store_vec<TY, V>(dy + col, u[k]);
-      }
-    }
+    if (a.grad_y != nullptr) store_row(dy, c, u);
     dy += s.d;
   }
   if (!one_gate) flush_gate();
@@ -223,8 +197,7 @@ __global__ void __launch_bounds__(norm_threads(V, false))
     if (g != 0) return;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int col = (k * s.group + t) * V;
-      if (col < s.d) store_vec<float, V>(parts + (static_cast<int64_t>(blockIdx.x) * kColumns + which) * s.d + col, acc[k]);
+      if (c.own[k]) store_vec<float, V>(parts + (static_cast<int64_t>(blockIdx.x) * kColumns + which) * s.d + c.at[k], acc[k]);
     }
   };
   finish(acc_w, kWeight);
@@ -245,21 +218,20 @@ __global__ void __launch_bounds__(norm_threads(V, true))
   const int t = threadIdx.x % s.group;
   const int g = threadIdx.x / s.group;
   const RowRun run(s.rows, static_cast<int64_t>(blockIdx.x) * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
-  const TX* dhp = static_cast<const TX*>(a.grad_h);
-  const TY* dnp = static_cast<const TY*>(a.grad_n);
+  const Columns<V, NV> c(s, t);
   const float inv_d = 1.0f / static_cast<float>(s.d);
-  GroupSum sum(shared, s.group, s.groups);
-  for (int i = 0; i < run.rounds; ++i) {
-    const int64_t row = run.first + i;
-    const bool live = row < run.last;
-    const float4 st = live ? reinterpret_cast<const float4*>(a.stats)[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-    RawRow<TX, V, NV> hr;
+  GroupSum<false> sum(shared, s.group, s.groups);
+  for (int64_t row = run.first; row < run.last; ++row) {
+    const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
+    RawRow<TX, V, NV> hr, in;
     RawRow<TY, V, NV> r2;  // dn, then y
-    hr.load(live ? static_cast<const TX*>(a.h) + row * a.h_stride : nullptr, s, t);
-    r2.load(live && dnp != nullptr ? dnp + row * a.grad_n_stride : nullptr, s, t);
+    hr.zero(), in.zero(), r2.zero();
+    hr.load(static_cast<const TX*>(a.h) + row * a.h_stride, c);
+    if (a.grad_n != nullptr) r2.load(static_cast<const TY*>(a.grad_n) + row * a.grad_n_stride, c);
+    if (a.grad_h != nullptr) in.load(static_cast<const TX*>(a.grad_h) + row * a.grad_h_stride, c);
     float v[NV][V];
     float m[2] = {0.f, 0.f};
-    load_param_row(a.weight, a.weight_dtype, 0, 1.f, s, t, v);
+    load_param_row(a.weight, a.weight_dtype, 0, 1.f, c, v);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float hat[V], dn[V];
@@ -275,10 +247,8 @@ __global__ void __launch_bounds__(norm_threads(V, true))
     sum(m, t);
     m[0] = s.layer ? m[0] * inv_d : 0.f;
     m[1] *= inv_d;
-    if (live && t == 0) means[row] = make_float2(m[0], m[1]);
-    r2.load(live && a.post ? static_cast<const TY*>(a.y) + row * a.y_stride : nullptr, s, t);
-    RawRow<TX, V, NV> in;
-    in.load(live && dhp != nullptr ? dhp + row * a.grad_h_stride : nullptr, s, t);
+    if (t == 0) means[row] = make_float2(m[0], m[1]);
+    if (a.post) r2.load(static_cast<const TY*>(a.y) + row * a.y_stride, c);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float hat[V], r[V];
@@ -289,12 +259,11 @@ __global__ void __launch_bounds__(norm_threads(V, true))
         v[k][j] = r[j] + st.y * (v[k][j] - m[0] - (hat[j] - st.x) * st.y * m[1]);
         r[j] = a.residual_scale * v[k][j];
       }
-      const int col = (k * s.group + t) * V;
-      if (live && col < s.d) store_vec<TX, V>(static_cast<TX*>(a.grad_x) + row * s.d + col, r);
+      if (c.own[k]) store_vec<TX, V>(static_cast<TX*>(a.grad_x) + row * s.d + c.at[k], r);
     }
     if (a.gate != nullptr) {
       float q[NV][V];
-      load_param_row(a.gate, a.gate_dtype, live && s.seq != s.rows ? row / s.seq * s.d : 0, 1.f, s, t, q);
+      load_param_row(a.gate, a.gate_dtype, s.seq != s.rows ? row / s.seq * s.d : 0, 1.f, c, q);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -302,7 +271,7 @@ __global__ void __launch_bounds__(norm_threads(V, true))
     }
     if (a.post) {
       float p[2] = {0.f, 0.f}, u[NV][V];
-      load_param_row(a.post_weight, a.post_weight_dtype, 0, 1.f, s, t, u);  // zeros beyond the row
+      load_param_row(a.post_weight, a.post_weight_dtype, 0, 1.f, c, u);  // zeros beyond the row
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         float y[V];
@@ -325,12 +294,7 @@ __global__ void __launch_bounds__(norm_threads(V, true))
         for (int j = 0; j < V; ++j) v[k][j] = st.w * (v[k][j] - p[0] - (y[j] - st.z) * st.w * p[1]);
       }
     }
-    if (!live || a.grad_y == nullptr) continue;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (k * s.group + t) * V;
-      if (col < s.d) store_vec<TY, V>(static_cast<TY*>(a.grad_y) + row * s.d + col, v[k]);
-    }
+    if (a.grad_y != nullptr) store_row(static_cast<TY*>(a.grad_y) + row * s.d, c, v);
   }
 }
 
@@ -515,7 +479,7 @@ int launch_one_pass(NormShape s, const opus_residual_norm_args& a, int wanted, c
   constexpr auto kernel = grad_kernel<TX, TY, V, NV, Full, Bias>;
   const int threads = s.group * s.groups;
   const int arrays = !Full ? 1 : (Bias ? 3 : 2) + (s.seq == s.rows ? 1 : 0);
-  const int shared = (GroupSum::size(s.group, s.groups) + (s.groups > 1 ? threads * V * NV : 0) +
+  const int shared = (group_floats(s.group, s.groups) + (s.groups > 1 ? threads * V * NV : 0) +
                       arrays * Param<NV, V, true>::size(s.group)) * static_cast<int>(sizeof(float));
   const int ready = allow_shared<kernel>(shared);
   if (ready) return ready;
@@ -558,7 +522,7 @@ int launch_wide(NormShape s, const opus_residual_norm_args& a, int wanted, const
   float* parts = reinterpret_cast<float*>(ws + align256(s.rows * 8));
   constexpr auto kernel = rows_kernel<TX, TY, V, NV>;
   const int threads = s.group * s.groups;
-  const int shared = GroupSum::size(s.group, s.groups) * static_cast<int>(sizeof(float));
+  const int shared = group_floats(s.group, s.groups) * static_cast<int>(sizeof(float));
   const int64_t need = (s.rows + s.groups - 1) / s.groups;
   const int64_t most = static_cast<int64_t>(sm_count()) * resident_blocks<kernel>(threads, shared);
   s.blocks = static_cast<int>(need < most ? need : most);
