@@ -78,7 +78,7 @@ namespace {
 enum Form : int { kAlone, kJoin, kFull };  // no y; y; y with a norm or a gate
 
 template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
-__global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : 3)
+__global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull || V < 8 ? 2 : 3)
     residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
   extern __shared__ __align__(16) float shared[];
   const int t = threadIdx.x % s.group;
