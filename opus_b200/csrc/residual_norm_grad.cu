@@ -551,40 +551,53 @@ int launch_wide(NormShape s, const opus_residual_norm_args& a, int wanted, const
   return rc;
 }
 
-template <typename TX, typename TY, int V, int NV>
-int launch_pass(const NormShape& s, const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws,
-                cudaStream_t st) {
-  const bool bias = a.post_bias != nullptr || (wanted & (1 << kBias)) != 0;
-  if (a.post || a.gate != nullptr)
-    return bias ? launch_one_pass<TX, TY, V, NV, true, true>(s, a, wanted, out, ws, st)
-                : launch_one_pass<TX, TY, V, NV, true, false>(s, a, wanted, out, ws, st);
-  return bias ? launch_one_pass<TX, TY, V, NV, false, true>(s, a, wanted, out, ws, st)
-              : launch_one_pass<TX, TY, V, NV, false, false>(s, a, wanted, out, ws, st);
+template <typename TX, typename TY, int V, bool Full, bool Bias>
+int launch_by_width(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
+  // 16 elements a thread, 8 where the sums of 16 columns would not leave registers enough and 8 reach the row's end
+  constexpr bool kLean = V < 8 && Full && (Bias || V == 1);
+  constexpr int kMost = 16 / V, kLess = 8 / V;
+  NormShape s;
+  int nv;
+  const bool lean = kLean && a.d <= kNormNarrow / 2;
+  const int rc = norm_shape("residual_norm_grad", &a, V, lean ? kLess : kMost, &s, &nv);
+  if (rc) return rc;
+  if constexpr (V > 1) {
+    if (nv == 1) return launch_one_pass<TX, TY, V, 1, Full, Bias>(s, a, wanted, out, ws, st);
+  }
+  if constexpr (V == 4) {
+    if (nv == 2) return launch_one_pass<TX, TY, V, 2, Full, Bias>(s, a, wanted, out, ws, st);
+  }
+  if constexpr (V == 1) {
+    if (nv <= 4) return launch_one_pass<TX, TY, V, 4, Full, Bias>(s, a, wanted, out, ws, st);
+    if constexpr (kLean) {
+      if (nv == 8) return launch_one_pass<TX, TY, V, 8, Full, Bias>(s, a, wanted, out, ws, st);
+    }
+  }
+  return launch_one_pass<TX, TY, V, kMost, Full, Bias>(s, a, wanted, out, ws, st);
 }
 
 template <typename TX, typename TY, int V>
-int launch_by_width(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
-  constexpr int kMost = 16 / V;
-  NormShape s;
-  int nv;
-  const bool wide = a.d > kNormNarrow;
-  const int rc = norm_shape("residual_norm_grad", &a, V, wide ? wide_vectors(V) : kMost, &s, &nv);
-  if (rc) return rc;
-  if (wide) return launch_wide<TX, TY, V, wide_vectors(V)>(s, a, wanted, out, ws, st);
-  if constexpr (V > 1) {
-    if (nv == 1) return launch_pass<TX, TY, V, 1>(s, a, wanted, out, ws, st);
+int launch_by_form(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
+  if (a.d > kNormNarrow) {
+    NormShape s;
+    int nv;
+    const int rc = norm_shape("residual_norm_grad", &a, V, wide_vectors(V), &s, &nv);
+    if (rc) return rc;
+    return launch_wide<TX, TY, V, wide_vectors(V)>(s, a, wanted, out, ws, st);
   }
-  if constexpr (V < 8) {
-    if (nv <= 4 / (V == 4 ? 2 : 1)) return launch_pass<TX, TY, V, 4 / (V == 4 ? 2 : 1)>(s, a, wanted, out, ws, st);
-  }
-  return launch_pass<TX, TY, V, kMost>(s, a, wanted, out, ws, st);
+  const bool bias = a.post_bias != nullptr || (wanted & (1 << kBias)) != 0;
+  if (a.post || a.gate != nullptr)
+    return bias ? launch_by_width<TX, TY, V, true, true>(a, wanted, out, ws, st)
+                : launch_by_width<TX, TY, V, true, false>(a, wanted, out, ws, st);
+  return bias ? launch_by_width<TX, TY, V, false, true>(a, wanted, out, ws, st)
+              : launch_by_width<TX, TY, V, false, false>(a, wanted, out, ws, st);
 }
 
 template <typename TX, typename TY>
 int launch_by_alignment(const opus_residual_norm_args& a, bool vec, int wanted, const ColumnOutputs& out, uint8_t* ws,
                         cudaStream_t st) {
-  return vec ? launch_by_width<TX, TY, 16 / sizeof(TX)>(a, wanted, out, ws, st)
-             : launch_by_width<TX, TY, 1>(a, wanted, out, ws, st);
+  return vec ? launch_by_form<TX, TY, 16 / sizeof(TX)>(a, wanted, out, ws, st)
+             : launch_by_form<TX, TY, 1>(a, wanted, out, ws, st);
 }
 
 bool on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
