@@ -138,6 +138,21 @@ def test_embedding_grad(n, V, d, dtype):
     ops.check_device_error()
 
 
+@pytest.mark.parametrize("n,V,d", [(2048, 50304, 8), (4096, 5, 16), (4097, 70, 8), (16384, 151936, 16), (32768, 262143, 8),
+                                   (32769, 262144, 8), (81920, 50257, 64), (188416, 50304, 16), (188417, 50304, 16),
+                                   (300_000, 3, 8), (250_000, 300_000, 24)])
+def test_embedding_grad_sort_sizes(n, V, d):
+    """One to sixteen blocks of the sorting cluster, one to three digits, and lists that are sorted through global memory."""
+    g = gen(n)
+    t = (V ** torch.rand(n, device=DEV, generator=g, dtype=torch.float64)).long().clamp_(max=V - 1)  # log-uniform: long runs
+    dy = randn(g, n, d)
+    got = check_embedding_grad(dy, t, V, padding_idx=V - 1)
+    assert torch.equal(got, ops.embedding_grad(dy, t, V, padding_idx=V - 1))
+    check_embedding_grad(dy, t, V, out=randn(g, V, d))
+    check_embedding_grad(dy, torch.arange(n, device=DEV) * 7919 % V, V)
+    ops.check_device_error()
+
+
 @pytest.mark.parametrize("pattern", ["one", "each", "pairs", "descending", "padding", "blocks"])
 def test_embedding_grad_patterns(pattern):
     n, V, d = 6000, 7000, 72
