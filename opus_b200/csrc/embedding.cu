@@ -10,11 +10,11 @@
 // inside the unit straight into dW.  A run that crosses units leaves its parts
 // in a workspace, and a second kernel joins them in order.  No sum is made by
 // atomics: each has one order, and the result is the same for every call.
-// Rows of dW that no token names are zeroed by the same launch as the sums.
 //
 // Up to 188416 positions are sorted by one cluster of up to 16 blocks that
-// hold them in shared memory and exchange them through it (one launch);
-// longer lists go through global memory with three launches a pass.
+// hold them in shared memory and exchange them through it (one launch), while
+// the other multiprocessors zero dW; longer lists go through global memory
+// with three launches a pass.
 //
 // Tokens outside [0, V) give a row of zeros, add to no gradient, and are
 // recorded in the device error word.  Tokens equal to padding_idx add to no
@@ -28,6 +28,7 @@ namespace opus {
 namespace {
 
 constexpr int kFwdThreads = 256;
+constexpr int kFwdBlocksPerSm = 6;
 
 __device__ __forceinline__ int64_t load_token(const void* tokens, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(tokens)[i] : static_cast<const int32_t*>(tokens)[i];
@@ -35,35 +36,48 @@ __device__ __forceinline__ int64_t load_token(const void* tokens, int wide, int6
 
 constexpr int kFwdRows = 4;  // a thread's, at a time: as many loads in flight
 
-// A thread keeps its column; `across` threads hold a row (of blockIdx.y's part), kFwdThreads / across rows a block.
-template <typename T, int V>
-__global__ void __launch_bounds__(kFwdThreads) lookup_kernel(const void* __restrict__ tokens, int wide, int64_t n,
+// A thread keeps its column; `across` threads hold a row (of blockIdx.y's part), blockDim.x / across rows a block.
+// Scaled: with a scale other than 1, which leaves rows as they are.
+template <typename T, int V, typename Token, bool Scaled>
+__global__ void __launch_bounds__(kFwdThreads) lookup_kernel(const Token* __restrict__ tokens, int64_t n,
                                                              const T* __restrict__ w, int64_t vocab, int64_t stride,
                                                              int d, int across, float scale, T* __restrict__ y, int* err) {
   const int col = (blockIdx.y * across + threadIdx.x % across) * V;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / across);
   if (col >= d) return;
-  for (int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.x / across) + threadIdx.x / across; first < n;
-       first += step * kFwdRows) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / across);
+  int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.x / across) + threadIdx.x / across;
+  const T* from = w + col;
+  T* to = y + first * d + col;
+  const int64_t to_step = step * d;
+  for (; first < n; first += step * kFwdRows) {
     int64_t t[kFwdRows];
     Vec<T, V> x[kFwdRows];
 #pragma unroll
-    for (int k = 0; k < kFwdRows; ++k) t[k] = first + k * step < n ? load_token(tokens, wide, first + k * step) : -1;
-#pragma unroll
     for (int k = 0; k < kFwdRows; ++k) {
-      if (t[k] >= 0 && t[k] < vocab) x[k] = *reinterpret_cast<const Vec<T, V>*>(w + t[k] * stride + col);
-      else x[k].zero();
+      t[k] = first + k * step < n ? static_cast<int64_t>(tokens[first + k * step]) : -1;
     }
 #pragma unroll
     for (int k = 0; k < kFwdRows; ++k) {
-      const int64_t row = first + k * step;
-      if (row >= n) break;
-      if ((t[k] < 0 || t[k] >= vocab) && col == 0) record_device_error(err, kDevBadToken);
-      float r[V];
-      x[k].get(r);
+      if (static_cast<uint64_t>(t[k]) < static_cast<uint64_t>(vocab)) {
+        x[k] = *reinterpret_cast<const Vec<T, V>*>(from + t[k] * stride);
+      } else {
+        x[k].zero();
+        if (col == 0 && first + k * step < n) record_device_error(err, kDevBadToken);
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < V; ++i) r[i] *= scale;
-      store_vec<T, V>(y + row * d + col, r);
+    for (int k = 0; k < kFwdRows; ++k) {
+      if (first + k * step < n) {
+        if constexpr (Scaled) {
+          float r[V];
+          x[k].get(r);
+#pragma unroll
+          for (int i = 0; i < V; ++i) r[i] *= scale;
+          x[k].set(r);
+        }
+        *reinterpret_cast<Vec<T, V>*>(to) = x[k];
+      }
+      to += to_step;
     }
   }
 }
@@ -78,22 +92,36 @@ constexpr int kMaxBins = 1 << kMaxBits;
 
 // The sort key of position i: its token, or V (behind every token) for one that adds to no row.
 struct KeySource {
-  const void* tokens;  // first pass; later passes read keys
-  const uint32_t* keys;
-  const uint32_t* pos;
+  const void* tokens;  // first pass; later passes read items (key, position)
+  const uint2* items;
   int wide;
   int64_t vocab;
   int64_t padding;
 };
 
-__device__ __forceinline__ uint32_t load_key(const KeySource& s, int64_t i, int* err) {
-  if (s.keys != nullptr) return s.keys[i];
+__device__ __forceinline__ uint2 load_item(const KeySource& s, int64_t i, int* err) {
+  if (s.items != nullptr) return s.items[i];
+  uint2 item = make_uint2(static_cast<uint32_t>(s.vocab), static_cast<uint32_t>(i));
   const int64_t t = load_token(s.tokens, s.wide, i);
   if (t < 0 || t >= s.vocab) {
     record_device_error(err, kDevBadToken);
-    return static_cast<uint32_t>(s.vocab);
+  } else if (t != s.padding) {
+    item.x = static_cast<uint32_t>(t);
   }
-  return static_cast<uint32_t>(t == s.padding ? s.vocab : t);
+  return item;
+}
+
+// The lanes whose digit is this lane's, among those in `live` (match_any takes many more cycles where a warp's
+// digits differ).
+__device__ __forceinline__ unsigned same_digit(uint32_t digit, int bits, unsigned live) {
+  unsigned same = live;
+#pragma unroll
+  for (int b = 0; b < kMaxBits; ++b) {
+    if (b >= bits) break;
+    const unsigned set = __ballot_sync(0xffffffffu, (digit >> b) & 1u);
+    same &= (digit >> b) & 1u ? set : ~set;
+  }
+  return same;
 }
 
 // counts[bin * tiles + tile]: keys of the tile whose digit is bin.
@@ -106,7 +134,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(KeySource src,
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
   for (int r = 0; r < kSortRounds; ++r) {
     const int64_t i = base + r * kSortThreads + threadIdx.x;
-    if (i < n) atomicAdd(&hist[(load_key(src, i, err) >> shift) & (bins - 1)], 1u);
+    if (i < n) atomicAdd(&hist[(load_item(src, i, err).x >> shift) & (bins - 1)], 1u);
   }
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kSortThreads) counts[static_cast<int64_t>(b) * tiles + blockIdx.x] = hist[b];
@@ -156,9 +184,7 @@ __global__ void __launch_bounds__(kScanThreads) sort_scan_kernel(uint32_t* __res
 // Writes every key of the tile, with its position, to its place by this digit.
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
                                                                   int tiles, const uint32_t* __restrict__ offsets,
-                                                                  uint32_t* __restrict__ keys_out,
-                                                                  uint32_t* __restrict__ pos_out,
-                                                                  uint8_t* __restrict__ present) {
+                                                                  uint2* __restrict__ out) {
   __shared__ uint32_t count[kSortWarps][kMaxBins];
   const int bins = 1 << bits;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -166,14 +192,15 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(KeySource src,
   __syncthreads();
   // a warp's keys are kSortRounds runs of 32 neighbours: rounds in order keep equal keys in order
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + warp * (32 * kSortRounds) + lane;
-  uint32_t key[kSortRounds], place[kSortRounds];
+  uint2 item[kSortRounds];
+  uint32_t place[kSortRounds];
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
     const int64_t i = base + r * 32;
     const bool live = i < n;
-    key[r] = live ? load_key(src, i, nullptr) : 0u;
-    const uint32_t digit = live ? (key[r] >> shift) & (bins - 1) : kMaxBins;
-    const uint32_t same = __match_any_sync(0xffffffffu, digit);
+    item[r] = live ? load_item(src, i, nullptr) : make_uint2(0u, 0u);
+    const uint32_t digit = (item[r].x >> shift) & (bins - 1);
+    const unsigned same = same_digit(digit, bits, __ballot_sync(0xffffffffu, live)) | (live ? 0u : 1u << lane);
     const int leader = __ffs(same) - 1;
     uint32_t before = 0;
     if (live && lane == leader) {
@@ -199,10 +226,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(KeySource src,
   for (int r = 0; r < kSortRounds; ++r) {
     const int64_t i = base + r * 32;
     if (i >= n) continue;
-    const uint32_t at = count[warp][(key[r] >> shift) & (bins - 1)] + place[r];
-    keys_out[at] = key[r];
-    pos_out[at] = src.pos != nullptr ? src.pos[i] : static_cast<uint32_t>(i);
-    if (present != nullptr && key[r] < src.vocab) present[key[r]] = 1;
+    out[count[warp][(item[r].x >> shift) & (bins - 1)] + place[r]] = item[r];
   }
 }
 
@@ -223,9 +247,11 @@ struct ClusterSort {
   int n, items;  // items: M
   int64_t vocab, padding;
   int passes, digit, bits;
-  uint32_t *keys, *pos;  // sorted
-  uint8_t* present;      // vocab bytes (NULL: not wanted): 1 where a key is
-  uint32_t* counters;    // two, zeroed
+  uint2* sorted;       // (key, position)
+  uint32_t* counters;  // two, zeroed
+  int blocks;          // of the cluster: cluster 0 sorts, the others zero
+  uint8_t* zero;       // zero_bytes from an address that is a multiple of 16, less than 16 more behind them
+  int64_t zero_bytes;
   int* err;
 };
 
@@ -234,8 +260,8 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint2 v) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
 }
 
 __host__ __device__ constexpr int cluster_sort_bytes(int items) {
@@ -244,9 +270,17 @@ __host__ __device__ constexpr int cluster_sort_bytes(int items) {
 
 __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(const __grid_constant__ ClusterSort p) {
   extern __shared__ __align__(16) uint32_t smem[];
-  const int blocks = static_cast<int>(gridDim.x), rank = static_cast<int>(cluster_ctarank());
+  const int blocks = p.blocks;
+  if (blockIdx.x >= blocks) {  // none of these blocks' clusters sorts
+    const int64_t whole = p.zero_bytes / 16, step = static_cast<int64_t>(gridDim.x - blocks) * kClusterThreads;
+    int64_t i = (blockIdx.x - blocks) * static_cast<int64_t>(kClusterThreads) + threadIdx.x;
+    if (i < p.zero_bytes - whole * 16) p.zero[whole * 16 + i] = 0;
+    for (; i < whole; i += step) reinterpret_cast<uint4*>(p.zero)[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int rank = static_cast<int>(cluster_ctarank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t* buffers = smem;  // keys and positions, twice
+  uint2* buffers = reinterpret_cast<uint2*>(smem);   // items, twice
   uint32_t* totals = smem + 4 * p.items;             // [bins] of this block, read by the others
   uint32_t* base = totals + kMaxBins;                // [bins]
   uint32_t* warp_sums = base + kMaxBins;             // [32] and a spare
@@ -255,38 +289,28 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(const 
   const int mine = p.n - first < p.items ? (p.n - first > 0 ? p.n - first : 0) : p.items;
   const int warp_items = ((mine + kClusterWarps - 1) / kClusterWarps + 31) / 32 * 32;
   if (rank == 0 && threadIdx.x < 2) p.counters[threadIdx.x] = 0;
-  if (p.present != nullptr) {  // whole words first: the array is padded to 16 bytes
-    const int64_t words = (p.vocab + 15) / 16;
-    for (int64_t i = rank * kClusterThreads + threadIdx.x; i < words; i += blocks * kClusterThreads)
-      reinterpret_cast<uint4*>(p.present)[i] = make_uint4(0, 0, 0, 0);
-  }
-  for (int i = threadIdx.x; i < mine; i += kClusterThreads) {
-    const int64_t t = load_token(p.tokens, p.wide, first + i);
-    uint32_t key = static_cast<uint32_t>(p.vocab);
-    if (t < 0 || t >= p.vocab) record_device_error(p.err, kDevBadToken);
-    else if (t != p.padding) key = static_cast<uint32_t>(t);
-    buffers[i] = key;
-    buffers[p.items + i] = static_cast<uint32_t>(first + i);
-  }
+  const KeySource src{p.tokens, nullptr, p.wide, p.vocab, p.padding};
+#pragma unroll 4
+  for (int i = threadIdx.x; i < mine; i += kClusterThreads) buffers[i] = load_item(src, first + i, p.err);
   __syncthreads();
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.digit;
-    const int bins = 1 << (p.bits - shift < p.digit ? p.bits - shift : p.digit);
-    const uint32_t* keys = buffers + (pass & 1) * 2 * p.items;
-    const uint32_t* pos = keys + p.items;
-    const int to = ((pass + 1) & 1) * 2 * p.items;
+    const int bits = p.bits - shift < p.digit ? p.bits - shift : p.digit, bins = 1 << bits;
+    const uint2* items = buffers + (pass & 1) * p.items;
+    uint2* to = buffers + ((pass + 1) & 1) * p.items;
     for (int i = threadIdx.x; i < kClusterWarps * kMaxBins / 2; i += kClusterThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0;
     __syncthreads();
-    uint32_t key[kItemRounds], place[kItemRounds];
+    uint2 item[kItemRounds];
+    uint32_t place[kItemRounds];
     uint16_t* count = counts + warp * kMaxBins;
 #pragma unroll
     for (int r = 0; r < kItemRounds; ++r) {
       const int i = warp * warp_items + r * 32 + lane;
       if (r * 32 >= warp_items) continue;  // the same for the whole warp
       const bool live = i < mine;
-      key[r] = live ? keys[i] : 0u;
-      const uint32_t digit = live ? (key[r] >> shift) & (bins - 1) : kMaxBins;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      item[r] = live ? items[i] : make_uint2(0u, 0u);
+      const uint32_t digit = (item[r].x >> shift) & (bins - 1);
+      const unsigned same = same_digit(digit, bits, __ballot_sync(0xffffffffu, live)) | (live ? 0u : 1u << lane);
       const int leader = __ffs(same) - 1;
       uint32_t before = 0;
       if (live && lane == leader) {
@@ -301,11 +325,13 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(const 
     const int bin = threadIdx.x;
     uint32_t total = 0;
     if (bin < bins) {
-#pragma unroll 8
+      uint32_t c[kClusterWarps];  // all loads first: they wait together
+#pragma unroll
+      for (int w = 0; w < kClusterWarps; ++w) c[w] = counts[w * kMaxBins + bin];
+#pragma unroll
       for (int w = 0; w < kClusterWarps; ++w) {
-        const uint32_t c = counts[w * kMaxBins + bin];
         counts[w * kMaxBins + bin] = static_cast<uint16_t>(total);
-        total += c;
+        total += c[w];
       }
       totals[bin] = total;
     }
@@ -314,10 +340,13 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(const 
     uint32_t lower = 0, all = 0;
     if (bin < bins) {
       const uint32_t at = smem_u32(totals + bin);
-      for (int r = 0; r < blocks; ++r) {
-        const uint32_t c = ld_cluster(mapa_shared(at, r));
-        all += c;
-        lower += r < rank ? c : 0u;
+      uint32_t c[kMostBlocks];
+#pragma unroll
+      for (int r = 0; r < kMostBlocks; ++r) c[r] = r < blocks ? ld_cluster(mapa_shared(at, r)) : 0u;
+#pragma unroll
+      for (int r = 0; r < kMostBlocks; ++r) {
+        all += c[r];
+        lower += r < rank ? c[r] : 0u;
       }
     }
     // digits before this one: bins <= 512, so the first 16 warps hold them
@@ -329,28 +358,23 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(const 
     }
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    if (bin < bins) {
-      uint32_t before = incl - all + lower;
-      for (int w = 0; w < warp; ++w) before += warp_sums[w];
-      base[bin] = before;
-    }
+    uint32_t before = lane < warp ? warp_sums[lane] : 0u;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (bin < bins) base[bin] = before + incl - all + lower;
     __syncthreads();
     const bool done = pass + 1 == p.passes;
 #pragma unroll
     for (int r = 0; r < kItemRounds; ++r) {
       const int i = warp * warp_items + r * 32 + lane;
       if (r * 32 >= warp_items || i >= mine) continue;
-      const uint32_t digit = (key[r] >> shift) & (bins - 1);
+      const uint32_t digit = (item[r].x >> shift) & (bins - 1);
       const uint32_t at = base[digit] + count[digit] + place[r];
       if (done) {
-        p.keys[at] = key[r];
-        p.pos[at] = pos[i];
-        if (p.present != nullptr && key[r] < p.vocab) p.present[key[r]] = 1;
+        p.sorted[at] = item[r];
       } else {
         const uint32_t block = at / static_cast<uint32_t>(p.items), slot = at - block * p.items;
-        const uint32_t there = mapa_shared(smem_u32(buffers + to + slot), block);
-        st_cluster(there, key[r]);
-        st_cluster(there + 4u * p.items, pos[i]);
+        st_cluster(mapa_shared(smem_u32(to + slot), block), item[r]);
       }
     }
     // items are where the next pass reads them; and no block leaves while another reads its totals
@@ -362,21 +386,20 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(const 
 // ------------------------------------------------------------------ sums
 constexpr int kUnit = 32;         // sorted positions of a unit
 constexpr int kSumWarps = 8;      // of a block
-constexpr int kBatch = 8;         // rows a warp has in flight
-constexpr int kLongUnits = 16;    // a run that goes on for more units is joined by a block, others by a warp
+constexpr int kLongUnits = 31;    // a run that goes on for more units is joined by a block, others by a warp
 
 // What the sums leave for the join: runs that cross units, by their first unit.
 struct Crossing {
   uint32_t* counters;  // short runs, long runs
-  uint32_t* lists;     // [units] short, [units] long
+  uint2* lists;        // [units] short, [units] long: unit, key
 };
 
-template <typename TO, int V>
-__device__ __forceinline__ void write_row(TO* out, const float (&acc)[V], float scale, int accumulate) {
+template <typename TO, int V, bool Add>
+__device__ __forceinline__ void write_row(TO* out, const float (&acc)[V], float scale) {
   float r[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) r[k] = acc[k] * scale;
-  if (accumulate) {
+  if constexpr (Add) {
     float o[V];
     load_vec<TO, V>(out, o);
 #pragma unroll
@@ -386,33 +409,44 @@ __device__ __forceinline__ void write_row(TO* out, const float (&acc)[V], float 
 }
 
 // One warp: one unit, 32 * V columns.  parts[unit]: [0] the part of a run that came from the unit before (or
-// fills the unit), [1] the part of a run that starts here and goes on.
-template <typename T, typename TO, int V>
-__device__ void sum_unit(int64_t unit, int slab, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-                         int64_t n, int64_t units, uint32_t vocab, const T* __restrict__ dy, int64_t stride, int d,
-                         float scale, int accumulate, TO* __restrict__ dw, float* __restrict__ parts,
-                         const Crossing& crossing) {
+// fills the unit), [1] the part of a run that starts here and goes on.  Add: into what is there (a batch's rows of
+// dW are loaded with its rows of dY: loaded where a run ends, each would be waited for on its own).
+template <typename T, typename TO, int V, bool Add>
+__device__ void sum_unit(int64_t unit, int slab, const uint2* __restrict__ sorted, int64_t n, int64_t units,
+                         uint32_t vocab, const T* __restrict__ dy, int64_t stride, int d, float scale,
+                         TO* __restrict__ dw, float* __restrict__ parts, const Crossing& crossing) {
+  constexpr int kBatch = Add ? 4 : 8;  // rows in flight (with rows of dW, 8 took registers for two blocks of five)
   const int lane = threadIdx.x & 31;
   const int64_t first = unit * kUnit;
   const int col = (slab * 32 + lane) * V;
   const bool live = col < d;
   const int64_t mine = first + lane;
-  const uint32_t my_key = mine < n ? keys[mine] : vocab;
-  const uint32_t my_pos = mine < n ? pos[mine] : 0u;
-  const uint32_t before = first > 0 ? keys[first - 1] : vocab;
-  const uint32_t after = first + kUnit < n ? keys[first + kUnit] : vocab;
+  const uint2 item = mine < n ? sorted[mine] : make_uint2(vocab, 0u);
+  const uint32_t my_key = item.x, my_pos = item.y;
+  const uint32_t before = first > 0 ? sorted[first - 1].x : vocab;
+  const uint32_t after = first + kUnit < n ? sorted[first + kUnit].x : vocab;
   const int len = __popc(__ballot_sync(0xffffffffu, my_key < vocab));  // keys equal to vocab sort last
+  const uint32_t my_next = __shfl_down_sync(0xffffffffu, my_key, 1);
+  const unsigned ends = __ballot_sync(0xffffffffu, lane == 31 || my_next != my_key);  // runs end, or the unit does
   float acc[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = 0.f;
   bool crossed = __shfl_sync(0xffffffffu, my_key, 0) == before;
   for (int b = 0; b < len; b += kBatch) {
     Vec<T, V> x[kBatch];
+    Vec<TO, V> o[Add ? kBatch : 1];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const uint32_t p = __shfl_sync(0xffffffffu, my_pos, b + i);  // b + kBatch <= 32
       if (live && b + i < len) x[i] = *reinterpret_cast<const Vec<T, V>*>(dy + static_cast<int64_t>(p) * stride + col);
       else x[i].zero();
+    }
+    if constexpr (Add) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t key = __shfl_sync(0xffffffffu, my_key, b + i);
+        if (live && b + i < len && (ends >> (b + i) & 1u)) o[i] = *reinterpret_cast<const Vec<TO, V>*>(dw + static_cast<int64_t>(key) * d + col);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -422,20 +456,31 @@ __device__ void sum_unit(int64_t unit, int slab, const uint32_t* __restrict__ ke
       x[i].get(r);
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[k] += r[k];
+      if ((ends >> j & 1u) == 0) continue;
       const uint32_t key = __shfl_sync(0xffffffffu, my_key, j);
-      const uint32_t following = __shfl_sync(0xffffffffu, my_key, (j + 1) & 31);
-      const uint32_t next = j + 1 < kUnit ? following : after;
-      if (next == key && j + 1 < kUnit) continue;
-      const bool goes_on = next == key;  // behind the unit's end
+      const bool goes_on = j + 1 == kUnit && after == key;
       if (live) {
-        if (crossed) store_vec<float, V>(parts + (unit * 2) * d + col, acc);
-        else if (goes_on) store_vec<float, V>(parts + (unit * 2 + 1) * d + col, acc);
-        else write_row<TO, V>(dw + static_cast<int64_t>(key) * d + col, acc, scale, accumulate);
+        if (crossed) {
+          store_vec<float, V>(parts + (unit * 2) * d + col, acc);
+        } else if (goes_on) {
+          store_vec<float, V>(parts + (unit * 2 + 1) * d + col, acc);
+        } else {
+          if constexpr (Add) {
+            float old[V];
+            o[i].get(old);
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] = acc[k] * scale + old[k];
+          } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] *= scale;
+          }
+          store_vec<TO, V>(dw + static_cast<int64_t>(key) * d + col, acc);
+        }
       }
       if (goes_on && !crossed && slab == 0 && lane == 0) {
         const int64_t far = (unit + 1 + kLongUnits) * kUnit;
-        const int is_long = far < n && keys[far] == key;
-        crossing.lists[is_long * units + atomicAdd(crossing.counters + is_long, 1u)] = static_cast<uint32_t>(unit);
+        const int is_long = far < n && sorted[far].x == key;
+        crossing.lists[is_long * units + atomicAdd(crossing.counters + is_long, 1u)] = make_uint2(static_cast<uint32_t>(unit), key);
       }
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[k] = 0.f;
@@ -444,36 +489,18 @@ __device__ void sum_unit(int64_t unit, int slab, const uint32_t* __restrict__ ke
   }
 }
 
-// Blocks below sum_blocks sum units; the others zero the rows that no token names, a warp 32 neighbouring rows.
-template <typename T, typename TO, int V>
-__global__ void __launch_bounds__(kSumWarps * 32) sum_kernel(const uint32_t* __restrict__ keys,
-                                                             const uint32_t* __restrict__ pos, int64_t n,
-                                                             uint32_t vocab, const T* __restrict__ dy, int64_t stride,
-                                                             int d, float scale, int accumulate,
+template <typename T, typename TO, int V, bool Add>
+__global__ void __launch_bounds__(kSumWarps * 32) sum_kernel(const uint2* __restrict__ sorted, int64_t n, uint32_t vocab,
+                                                             const T* __restrict__ dy, int64_t stride, int d, float scale,
                                                              TO* __restrict__ dw, float* __restrict__ parts,
-                                                             const __grid_constant__ Crossing crossing,
-                                                             const uint8_t* __restrict__ present, unsigned sum_blocks) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x < sum_blocks) {
-    const int slabs = (d / V + 31) / 32;
-    const int64_t units = (n + kUnit - 1) / kUnit;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * kSumWarps + warp;
-    if (item >= units * slabs) return;
-    sum_unit<T, TO, V>(item / slabs, static_cast<int>(item % slabs), keys, pos, n, units, vocab, dy, stride, d, scale,
-                       accumulate, dw, parts, crossing);
-    return;
-  }
-  const int64_t warps = static_cast<int64_t>(gridDim.x - sum_blocks) * kSumWarps;
-  for (int64_t r = (static_cast<int64_t>(blockIdx.x - sum_blocks) * kSumWarps + warp) * 32; r < vocab; r += warps * 32) {
-    unsigned absent = __ballot_sync(0xffffffffu, r + lane < vocab && present[r + lane] == 0);
-    while (absent != 0) {
-      const int64_t row = r + __ffs(absent) - 1;
-      absent &= absent - 1;
-      Vec<TO, V> zero;
-      zero.zero();
-      for (int col = lane * V; col < d; col += 32 * V) *reinterpret_cast<Vec<TO, V>*>(dw + row * d + col) = zero;
-    }
-  }
+                                                             const __grid_constant__ Crossing crossing) {
+  wait_for_predecessors();
+  const int slabs = (d / V + 31) / 32;
+  const int64_t units = (n + kUnit - 1) / kUnit;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
+  if (item < units * slabs)
+    sum_unit<T, TO, V, Add>(item / slabs, static_cast<int>(item % slabs), sorted, n, units, vocab, dy, stride, d, scale,
+                            dw, parts, crossing);
 }
 
 // Sums parts[u][0] over the units [a, b) behind a run's first.
@@ -488,28 +515,29 @@ __device__ __forceinline__ void sum_parts(const float* __restrict__ parts, int64
   }
 }
 
-// Joins the parts of runs that cross units: a long run and slab of columns by a block, in 32 slices of its units
-// that meet in order, a short one by a warp.
+// Joins the parts of runs that cross units: a long run and slab of columns by a block (from the grid's first), in
+// 32 slices of its units that meet in order, a short one by a warp (from the grid's last).
 constexpr int kJoinWarps = 32;
-template <typename TO, int V>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const uint32_t* __restrict__ keys, int64_t n, int d,
-                                                               float scale, int accumulate, TO* __restrict__ dw,
+template <typename TO, int V, bool Add>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const uint2* __restrict__ sorted, int64_t n, int d,
+                                                               float scale, TO* __restrict__ dw,
                                                                const float* __restrict__ parts,
                                                                const __grid_constant__ Crossing crossing) {
   __shared__ float slice[kJoinWarps][32 * V];
+  wait_for_predecessors();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slabs = (d / V + 31) / 32;
   const int64_t units = (n + kUnit - 1) / kUnit;
   const int64_t n_short = static_cast<int64_t>(crossing.counters[0]) * slabs;
   const int64_t n_long = static_cast<int64_t>(crossing.counters[1]) * slabs;
   for (int64_t item = blockIdx.x; item < n_long; item += gridDim.x) {
-    const int64_t unit = crossing.lists[units + item / slabs];
+    const uint2 run = crossing.lists[units + item / slabs];
+    const int64_t unit = run.x;
     const int col = (static_cast<int>(item % slabs) * 32 + lane) * V;
-    const uint32_t key = keys[(unit + 1) * kUnit];
     int64_t more = 0;  // units behind the first that hold parts of the run: a prefix of those that follow
     while (true) {
       const int64_t u = unit + 1 + more + threadIdx.x;
-      const int in = __syncthreads_count(u < units && keys[u * kUnit] == key);
+      const int in = __syncthreads_count(u < units && sorted[u * kUnit].x == run.y);
       more += in;
       if (in < kJoinWarps * 32) break;
     }
@@ -520,33 +548,36 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const uint32_t* _
       if (warp == 0) load_vec<float, V>(parts + (unit * 2 + 1) * d + col, acc);
       sum_parts<V>(parts, unit + 1 + more * warp / kJoinWarps, unit + 1 + more * (warp + 1) / kJoinWarps, d, col, acc);
     }
+    // slices w and w + half, until one is left
 #pragma unroll
-    for (int k = 0; k < V; ++k) slice[warp][k * 32 + lane] = acc[k];
-    __syncthreads();
-    if (warp == 0 && col < d) {
+    for (int half = kJoinWarps / 2; half > 0; half >>= 1) {
+      if (warp >= half && warp < 2 * half) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        for (int w = 1; w < kJoinWarps; ++w) acc[k] += slice[w][k * 32 + lane];
+        for (int k = 0; k < V; ++k) slice[warp][k * 32 + lane] = acc[k];
       }
-      write_row<TO, V>(dw + static_cast<int64_t>(key) * d + col, acc, scale, accumulate);
+      __syncthreads();
+      if (warp < half) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += slice[warp + half][k * 32 + lane];
+      }
     }
+    if (warp == 0 && col < d) write_row<TO, V, Add>(dw + static_cast<int64_t>(run.y) * d + col, acc, scale);
     __syncthreads();
   }
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp; item < n_short;
+  for (int64_t item = static_cast<int64_t>(gridDim.x - 1 - blockIdx.x) * kJoinWarps + warp; item < n_short;
        item += static_cast<int64_t>(gridDim.x) * kJoinWarps) {
-    const int64_t unit = crossing.lists[item / slabs];
+    const uint2 run = crossing.lists[item / slabs];
+    const int64_t unit = run.x, u = unit + 1 + lane;
     const int col = (static_cast<int>(item % slabs) * 32 + lane) * V;
-    const uint32_t key = keys[(unit + 1) * kUnit];
-    const int64_t u = unit + 1 + lane;
-    const int more = __popc(__ballot_sync(0xffffffffu, u < units && keys[u * kUnit] == key));  // kLongUnits + 1 at most
+    const int more = __popc(__ballot_sync(0xffffffffu, u < units && sorted[u * kUnit].x == run.y));  // kLongUnits at most
     if (col >= d) continue;
     float acc[V];
     load_vec<float, V>(parts + (unit * 2 + 1) * d + col, acc);
     sum_parts<V>(parts, unit + 1, unit + 1 + more, d, col, acc);
-    write_row<TO, V>(dw + static_cast<int64_t>(key) * d + col, acc, scale, accumulate);
+    write_row<TO, V, Add>(dw + static_cast<int64_t>(run.y) * d + col, acc, scale);
   }
 }
-static_assert(kLongUnits + 1 <= 32, "a warp looks at a short run's units at once");
+static_assert(kLongUnits < 32, "a warp looks at a short run's units at once");
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -554,9 +585,9 @@ struct Plan {
   int bits, passes, digit;
   bool cluster;  // sorted by one cluster
   int64_t tiles, units;
-  // offsets: sorted keys and positions; the counters and lists of crossing runs; the rows' flags; the parts; for
-  // the sort through global memory its second keys and positions and its counts
-  int64_t keys, crossing, present, parts, second, counts, bytes;
+  // offsets: the sorted items; the counters and lists of crossing runs; the parts; for the sort through global
+  // memory its second items and its counts
+  int64_t crossing, parts, second, counts, bytes;
 };
 
 Plan plan_of(int64_t n, int64_t vocab, int d) {
@@ -567,65 +598,81 @@ Plan plan_of(int64_t n, int64_t vocab, int d) {
   p.tiles = (n + kTile - 1) / kTile;
   p.units = (n + kUnit - 1) / kUnit;
   p.cluster = n <= static_cast<int64_t>(kMostBlocks) * kMostItems;
-  p.keys = align256(n * 4);
-  p.crossing = 2 * p.keys;
-  p.present = p.crossing + 256 + align256(p.units * 8);
-  p.parts = p.present + align256(vocab);
+  p.crossing = align256(n * 8);
+  p.parts = p.crossing + 256 + align256(p.units * 16);
   p.second = p.parts + align256(p.units * 2 * d * 4);
-  p.counts = p.second + (p.cluster ? 0 : 2 * p.keys);
+  p.counts = p.second + (p.cluster ? 0 : align256(n * 8));
   p.bytes = p.counts + (p.cluster ? 0 : align256((p.tiles << p.digit) * 4));
   return p;
 }
 
-template <typename T, typename TO, int V>
-int launch_sums(const uint32_t* keys, const uint32_t* pos, const Plan& p, int64_t n, int64_t vocab, const void* dy,
-                int64_t stride, int d, float scale, int accumulate, void* dw, uint8_t* ws, cudaStream_t st) {
+template <typename T, typename TO, int V, bool Add>
+int launch_sums(const Plan& p, int64_t n, int64_t vocab, const void* dy, int64_t stride, int d, float scale, void* dw,
+                uint8_t* ws, cudaStream_t st) {
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws + p.crossing);
-  const Crossing crossing{counters, counters + 64};
+  const Crossing crossing{counters, reinterpret_cast<uint2*>(ws + p.crossing + 256)};
   const int64_t slabs = (d / V + 31) / 32, items = p.units * slabs;
-  const int64_t sum_blocks = (items + kSumWarps - 1) / kSumWarps;
-  int64_t zero_blocks = accumulate ? 0 : (vocab + 32 * kSumWarps - 1) / (32 * kSumWarps);
-  const int64_t most = static_cast<int64_t>(sm_count()) * 8;
-  zero_blocks = zero_blocks < most ? zero_blocks : most;
-  if (sum_blocks + zero_blocks > 0x7fffffff) return set_error(OPUS_ERR_UNSUPPORTED, "embedding_grad: too many positions");
-  sum_kernel<T, TO, V><<<static_cast<unsigned>(sum_blocks + zero_blocks), kSumWarps * 32, 0, st>>>(
-      keys, pos, n, static_cast<uint32_t>(vocab), static_cast<const T*>(dy), stride, d, scale, accumulate,
-      static_cast<TO*>(dw), parts, crossing, ws + p.present, static_cast<unsigned>(sum_blocks));
+  const int64_t blocks = (items + kSumWarps - 1) / kSumWarps;
+  if (blocks > 0x7fffffff) return set_error(OPUS_ERR_UNSUPPORTED, "embedding_grad: too many positions");
+  const uint2* sorted = reinterpret_cast<const uint2*>(ws);
+  OPUS_CUDA_TRY(launch_early(sum_kernel<T, TO, V, Add>, dim3(static_cast<unsigned>(blocks)), kSumWarps * 32, 0, st, sorted,
+                             n, static_cast<uint32_t>(vocab), static_cast<const T*>(dy), stride, d, scale,
+                             static_cast<TO*>(dw), parts, crossing));
   note_launch();
-  OPUS_CUDA_TRY(cudaGetLastError());
   if (p.units < 2) return OPUS_OK;  // nothing crosses
-  const int64_t want = (items + kJoinWarps - 1) / kJoinWarps;
-  join_kernel<TO, V><<<static_cast<unsigned>(want < 2 * sm_count() ? want : 2 * sm_count()), kJoinWarps * 32, 0, st>>>(
-      keys, n, d, scale, accumulate, static_cast<TO*>(dw), parts, crossing);
+  const int64_t want = (items + kJoinWarps - 1) / kJoinWarps, most = 2 * sm_count();
+  OPUS_CUDA_TRY(launch_early(join_kernel<TO, V, Add>, dim3(static_cast<unsigned>(want < most ? want : most)),
+                             kJoinWarps * 32, 0, st, sorted, n, d, scale, static_cast<TO*>(dw), parts, crossing));
   note_launch();
-  OPUS_CUDA_TRY(cudaGetLastError());
   return OPUS_OK;
 }
 
 template <typename T, typename TO>
-int launch_sums_by_width(bool wide, const uint32_t* keys, const uint32_t* pos, const Plan& p, int64_t n, int64_t vocab,
+int launch_sums_by_width(bool wide, const Plan& p, int64_t n, int64_t vocab,
                          const void* dy, int64_t stride, int d, float scale, int accumulate, void* dw, uint8_t* ws,
                          cudaStream_t st) {
   constexpr int V = 16 / (sizeof(T) > sizeof(TO) ? sizeof(T) : sizeof(TO));
-  if (wide) return launch_sums<T, TO, V>(keys, pos, p, n, vocab, dy, stride, d, scale, accumulate, dw, ws, st);
-  return launch_sums<T, TO, 1>(keys, pos, p, n, vocab, dy, stride, d, scale, accumulate, dw, ws, st);
+  if (wide)
+    return accumulate ? launch_sums<T, TO, V, true>(p, n, vocab, dy, stride, d, scale, dw, ws, st)
+                      : launch_sums<T, TO, V, false>(p, n, vocab, dy, stride, d, scale, dw, ws, st);
+  return accumulate ? launch_sums<T, TO, 1, true>(p, n, vocab, dy, stride, d, scale, dw, ws, st)
+                    : launch_sums<T, TO, 1, false>(p, n, vocab, dy, stride, d, scale, dw, ws, st);
 }
 
-int launch_cluster_sort(const Plan& p, const KeySource& src, int64_t n, uint8_t* ws, bool flags, int* err, cudaStream_t st) {
-  int blocks = 1;
-  while (blocks < kMostBlocks && static_cast<int64_t>(blocks) * kBlockItems < n) blocks *= 2;
+// Clusters of 2^k sorting blocks that the device holds at once (a cluster lies in one group of its
+// multiprocessors): one that had to wait for others would begin to zero when they have ended.
+int resident_clusters(const cudaLaunchConfig_t& cfg, int k) {
+  static std::atomic<int> known[5];
+  int n = known[k].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, cluster_sort_kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+    known[k].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// zero_bytes of zero (0: none) are zeroed by the blocks that do not sort.
+int launch_cluster_sort(const Plan& p, const KeySource& src, int64_t n, uint8_t* ws, void* zero, int64_t zero_bytes,
+                        int* err, cudaStream_t st) {
+  int blocks = 1, k = 0;
+  for (; blocks < kMostBlocks && static_cast<int64_t>(blocks) * kBlockItems < n; ++k) blocks *= 2;
   ClusterSort a{};
   a.tokens = src.tokens, a.wide = src.wide, a.vocab = src.vocab, a.padding = src.padding;
   a.n = static_cast<int>(n);
   a.items = static_cast<int>(((n + blocks - 1) / blocks + 31) / 32 * 32);
   a.passes = p.passes, a.digit = p.digit, a.bits = p.bits;
-  a.keys = reinterpret_cast<uint32_t*>(ws);
-  a.pos = reinterpret_cast<uint32_t*>(ws + p.keys);
-  a.present = flags ? ws + p.present : nullptr;
+  a.sorted = reinterpret_cast<uint2*>(ws);
   a.counters = reinterpret_cast<uint32_t*>(ws + p.crossing);
+  a.blocks = blocks;
   a.err = err;
-  const int shared = cluster_sort_bytes(a.items);
+  // bytes before the first 16-byte boundary are left to a memset of their own
+  const int64_t head = zero_bytes > 0 ? (16 - reinterpret_cast<uintptr_t>(zero) % 16) % 16 : 0;
+  if (head > 0) OPUS_CUDA_TRY(cudaMemsetAsync(zero, 0, head < zero_bytes ? head : zero_bytes, st));
+  a.zero = static_cast<uint8_t*>(zero) + head;
+  a.zero_bytes = zero_bytes > head ? zero_bytes - head : 0;
+  // every launch takes the shared memory of the longest list: one block a multiprocessor, whatever n
+  const int shared = cluster_sort_bytes(kMostItems);
   OPUS_CUDA_TRY(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
   OPUS_CUDA_TRY(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchAttribute attr[1];
@@ -634,60 +681,76 @@ int launch_cluster_sort(const Plan& p, const KeySource& src, int64_t n, uint8_t*
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks), cfg.blockDim = dim3(kClusterThreads);
   cfg.dynamicSmemBytes = shared, cfg.stream = st, cfg.attrs = attr, cfg.numAttrs = 1;
+  int64_t zeroing = (a.zero_bytes + kClusterThreads * 16 * 8 - 1) / (kClusterThreads * 16 * 8);
+  zeroing = (zeroing + blocks - 1) / blocks;
+  if (zeroing > 0) {
+    const int held = resident_clusters(cfg, k) - 1;
+    zeroing = zeroing < held ? zeroing : held > 0 ? held : 1;
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * (1 + zeroing)));
   OPUS_CUDA_TRY(cudaLaunchKernelEx(&cfg, cluster_sort_kernel, a));
   note_launch();
   return OPUS_OK;
 }
 
-int launch_global_sort(const Plan& p, KeySource src, int64_t n, uint8_t* ws, bool flags, int* err, cudaStream_t st) {
+int launch_global_sort(const Plan& p, KeySource src, int64_t n, uint8_t* ws, void* zero, int64_t zero_bytes, int* err,
+                       cudaStream_t st) {
+  if (zero_bytes > 0) OPUS_CUDA_TRY(cudaMemsetAsync(zero, 0, zero_bytes, st));
   OPUS_CUDA_TRY(cudaMemsetAsync(ws + p.crossing, 0, 8, st));
-  if (flags) OPUS_CUDA_TRY(cudaMemsetAsync(ws + p.present, 0, src.vocab, st));
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
   const int tiles = static_cast<int>(p.tiles);
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.digit;
     const int bits = p.bits - shift < p.digit ? p.bits - shift : p.digit;
-    const bool last = pass + 1 == p.passes;
     sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(src, n, shift, bits, tiles, counts, pass == 0 ? err : nullptr);
     note_launch();
     OPUS_CUDA_TRY(cudaGetLastError());
     sort_scan_kernel<<<1, kScanThreads, 0, st>>>(counts, p.tiles << bits);
     note_launch();
     OPUS_CUDA_TRY(cudaGetLastError());
-    // the last pass ends in the first pair of arrays
-    uint8_t* to = ws + ((p.passes - pass) % 2 == 1 ? 0 : p.second);
-    uint32_t* keys = reinterpret_cast<uint32_t*>(to);
-    uint32_t* pos = reinterpret_cast<uint32_t*>(to + p.keys);
-    sort_place_kernel<<<tiles, kSortThreads, 0, st>>>(src, n, shift, bits, tiles, counts, keys, pos,
-                                                      last && flags ? ws + p.present : nullptr);
+    // the last pass ends in the first array
+    uint2* to = reinterpret_cast<uint2*>(ws + ((p.passes - pass) % 2 == 1 ? 0 : p.second));
+    sort_place_kernel<<<tiles, kSortThreads, 0, st>>>(src, n, shift, bits, tiles, counts, to);
     note_launch();
     OPUS_CUDA_TRY(cudaGetLastError());
-    src.keys = keys;
-    src.pos = pos;
+    src.items = to;
   }
   return OPUS_OK;
 }
 
-template <typename T>
-int launch_lookup(const void* tokens, int wide, int64_t n, const void* w, int64_t vocab, int64_t stride, int d,
-                  float scale, void* y, bool vec, int* err, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  const int per_row = vec ? d / V : d;
+template <typename T, int V, typename Token, bool Scaled>
+int launch_lookup(const void* tokens, int64_t n, const void* w, int64_t vocab, int64_t stride, int d, float scale,
+                  void* y, int* err, cudaStream_t st) {
+  constexpr auto kernel = lookup_kernel<T, V, Token, Scaled>;
+  const int per_row = d / V;
   const int parts = (per_row + kFwdThreads - 1) / kFwdThreads, across = (per_row + parts - 1) / parts;
   const int rows = kFwdThreads / across;  // of a block
-  int64_t blocks = (n + rows * kFwdRows - 1) / (rows * kFwdRows);
-  const int64_t most = static_cast<int64_t>(sm_count()) * 64;
-  if (blocks > most) blocks = most;
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
-  if (vec)
-    lookup_kernel<T, V><<<grid, rows * across, 0, st>>>(tokens, wide, n, static_cast<const T*>(w), vocab, stride, d,
-                                                        across, scale, static_cast<T*>(y), err);
-  else
-    lookup_kernel<T, 1><<<grid, rows * across, 0, st>>>(tokens, wide, n, static_cast<const T*>(w), vocab, stride, d,
-                                                        across, scale, static_cast<T*>(y), err);
+  // blocks that stay: what a thread sets up serves many rows
+  const int64_t need = (n + rows * kFwdRows - 1) / (rows * kFwdRows);
+  const int64_t most = (static_cast<int64_t>(sm_count()) * kFwdBlocksPerSm + parts - 1) / parts;
+  const dim3 grid(static_cast<unsigned>(need < most ? need : most), static_cast<unsigned>(parts));
+  kernel<<<grid, rows * across, 0, st>>>(static_cast<const Token*>(tokens), n, static_cast<const T*>(w), vocab, stride, d,
+                                         across, scale, static_cast<T*>(y), err);
   note_launch();
   OPUS_CUDA_TRY(cudaGetLastError());
   return OPUS_OK;
+}
+
+template <typename T, int V>
+int launch_lookup_by_token(const void* tokens, int wide, int64_t n, const void* w, int64_t vocab, int64_t stride, int d,
+                           float scale, void* y, int* err, cudaStream_t st) {
+  if (wide)
+    return scale == 1.0f ? launch_lookup<T, V, int64_t, false>(tokens, n, w, vocab, stride, d, scale, y, err, st)
+                         : launch_lookup<T, V, int64_t, true>(tokens, n, w, vocab, stride, d, scale, y, err, st);
+  return scale == 1.0f ? launch_lookup<T, V, int32_t, false>(tokens, n, w, vocab, stride, d, scale, y, err, st)
+                       : launch_lookup<T, V, int32_t, true>(tokens, n, w, vocab, stride, d, scale, y, err, st);
+}
+
+template <typename T>
+int launch_lookup_by_width(const void* tokens, int wide, int64_t n, const void* w, int64_t vocab, int64_t stride, int d,
+                           float scale, void* y, bool vec, int* err, cudaStream_t st) {
+  return vec ? launch_lookup_by_token<T, 16 / sizeof(T)>(tokens, wide, n, w, vocab, stride, d, scale, y, err, st)
+             : launch_lookup_by_token<T, 1>(tokens, wide, n, w, vocab, stride, d, scale, y, err, st);
 }
 
 constexpr int64_t kMaxTokens = 0x7fffffff;  // positions and keys are 32 bits
@@ -727,10 +790,10 @@ extern "C" int opus_embedding(const void* tokens, int token_bits, int64_t n, con
   const int wide = token_bits == 64;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == OPUS_DTYPE_F32)
-    return launch_lookup<float>(tokens, wide, n, weight, vocab, row_stride, d, scale, out, vec, err, st);
+    return launch_lookup_by_width<float>(tokens, wide, n, weight, vocab, row_stride, d, scale, out, vec, err, st);
   if (dtype == OPUS_DTYPE_F16)
-    return launch_lookup<__half>(tokens, wide, n, weight, vocab, row_stride, d, scale, out, vec, err, st);
-  return launch_lookup<__nv_bfloat16>(tokens, wide, n, weight, vocab, row_stride, d, scale, out, vec, err, st);
+    return launch_lookup_by_width<__half>(tokens, wide, n, weight, vocab, row_stride, d, scale, out, vec, err, st);
+  return launch_lookup_by_width<__nv_bfloat16>(tokens, wide, n, weight, vocab, row_stride, d, scale, out, vec, err, st);
 }
 
 extern "C" int64_t opus_embedding_grad_workspace_bytes(int64_t n, int64_t vocab, int d) {
@@ -766,29 +829,28 @@ extern "C" int opus_embedding_grad(const void* grad_out, int grad_dtype, int64_t
   int* err = device_error_word();
   if (err == nullptr) return set_error(OPUS_ERR_CUDA, "device error word unavailable");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const KeySource src{tokens, nullptr, nullptr, token_bits == 64, vocab, padding_idx};
-  rc = p.cluster ? launch_cluster_sort(p, src, n, ws, !accumulate, err, st)
-                 : launch_global_sort(p, src, n, ws, !accumulate, err, st);
+  const KeySource src{tokens, nullptr, token_bits == 64, vocab, padding_idx};
+  const int64_t zero_bytes = accumulate ? 0 : vocab * d * dtype_bytes(out_dtype);
+  rc = p.cluster ? launch_cluster_sort(p, src, n, ws, grad_weight, zero_bytes, err, st)
+                 : launch_global_sort(p, src, n, ws, grad_weight, zero_bytes, err, st);
   if (rc) return rc;
-  const uint32_t* keys = reinterpret_cast<const uint32_t*>(ws);
-  const uint32_t* pos = reinterpret_cast<const uint32_t*>(ws + p.keys);
   const bool f32_out = out_dtype == OPUS_DTYPE_F32;
   const int V = 16 / (f32_out ? 4 : dtype_bytes(grad_dtype));
   const bool vec = d % V == 0 && row_stride % V == 0 && aligned(grad_out, V * dtype_bytes(grad_dtype)) &&
                    aligned(grad_weight, V * dtype_bytes(out_dtype));
   if (grad_dtype == OPUS_DTYPE_F32)
-    return launch_sums_by_width<float, float>(vec, keys, pos, p, n, vocab, grad_out, row_stride, d, scale, accumulate,
+    return launch_sums_by_width<float, float>(vec, p, n, vocab, grad_out, row_stride, d, scale, accumulate,
                                               grad_weight, ws, st);
   if (grad_dtype == OPUS_DTYPE_F16) {
     if (f32_out)
-      return launch_sums_by_width<__half, float>(vec, keys, pos, p, n, vocab, grad_out, row_stride, d, scale,
+      return launch_sums_by_width<__half, float>(vec, p, n, vocab, grad_out, row_stride, d, scale,
                                                  accumulate, grad_weight, ws, st);
-    return launch_sums_by_width<__half, __half>(vec, keys, pos, p, n, vocab, grad_out, row_stride, d, scale,
+    return launch_sums_by_width<__half, __half>(vec, p, n, vocab, grad_out, row_stride, d, scale,
                                                 accumulate, grad_weight, ws, st);
   }
   if (f32_out)
-    return launch_sums_by_width<__nv_bfloat16, float>(vec, keys, pos, p, n, vocab, grad_out, row_stride, d, scale,
+    return launch_sums_by_width<__nv_bfloat16, float>(vec, p, n, vocab, grad_out, row_stride, d, scale,
                                                       accumulate, grad_weight, ws, st);
-  return launch_sums_by_width<__nv_bfloat16, __nv_bfloat16>(vec, keys, pos, p, n, vocab, grad_out, row_stride, d, scale,
+  return launch_sums_by_width<__nv_bfloat16, __nv_bfloat16>(vec, p, n, vocab, grad_out, row_stride, d, scale,
                                                             accumulate, grad_weight, ws, st);
 }

@@ -175,6 +175,7 @@ __device__ float whole_norm(const double* __restrict__ partial, int parts, int k
 
 __global__ void __launch_bounds__(kThreads) norm_join_kernel(const double* __restrict__ partial, int parts, int kind,
                                                              float* __restrict__ norm) {
+  wait_for_predecessors();
   const float n = whole_norm(partial, parts, kind);
   if (threadIdx.x == 0) *norm = n;
 }
@@ -216,6 +217,7 @@ template <typename TI, typename TO, int Most>
 __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ GradTable<Most> t, int kind,
                                                          const double* __restrict__ partial, int parts,
                                                          float max_norm, float* __restrict__ norm) {
+  wait_for_predecessors();
   float n;
   if (parts > 0) {
     n = whole_norm(partial, parts, kind);
@@ -351,9 +353,9 @@ int launch_scale_pair(const Lists& l, int types, int kind, const double* partial
   for (int at = 0; at < l.count;) {
     at = fill_table(l, at, types, &t);
     if (t.units == 0) continue;
-    scale_kernel<TI, TO, Most><<<grid_of(t.units), kThreads, 0, st>>>(t, kind, partial, parts, max_norm, norm);
+    OPUS_CUDA_TRY(launch_early(scale_kernel<TI, TO, Most>, dim3(grid_of(t.units)), kThreads, 0, st, t, kind, partial,
+                               parts, max_norm, norm));
     note_launch();
-    OPUS_CUDA_TRY(cudaGetLastError());
   }
   return OPUS_OK;
 }
@@ -395,9 +397,8 @@ int launch_scale(const Lists& l, int kind, const double* partial, int parts, flo
 }
 
 int launch_join(const double* partial, int parts, int kind, float* norm, cudaStream_t st) {
-  norm_join_kernel<<<1, kThreads, 0, st>>>(partial, parts, kind, norm);
+  OPUS_CUDA_TRY(launch_early(norm_join_kernel, dim3(1), kThreads, 0, st, partial, parts, kind, norm));
   note_launch();
-  OPUS_CUDA_TRY(cudaGetLastError());
   return OPUS_OK;
 }
 

@@ -39,6 +39,20 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const voi
     if (_e != cudaSuccess) return ::opus::cuda_fail(_e, #expr); \
   } while (0)
 
+// Launches a kernel that calls wait_for_predecessors() before it touches global memory: it is set up while the last
+// blocks of the kernel before it end (about 1.5 us of a chain of short kernels; set up earlier, its waiting blocks
+// took the registers of those still to run).
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t st, A&&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = shared, cfg.stream = st;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // Device-side error codes (written to the device error word).
 enum DeviceError : int {
   kDevOk = 0,
@@ -69,6 +83,11 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 __device__ __forceinline__ void record_device_error(int* err, int code) {
   if (err != nullptr) atomicCAS(err, 0, code);
 }
+
+// ---- kernels that follow each other (launch_early)
+// Every thread of a kernel launched early calls it before it reads or writes global memory: it returns when the
+// kernels before it have ended and what they wrote can be seen.
+__device__ __forceinline__ void wait_for_predecessors() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {

@@ -412,6 +412,7 @@ __device__ __forceinline__ float join_parts(const float* v, int64_t count, int64
 // blockIdx.y: an array of parts[run][array][d] (its sums over all runs).
 __global__ void __launch_bounds__(kSlices * 32) columns_join_kernel(const float* __restrict__ parts, int64_t runs, int d,
                                                                     const __grid_constant__ ColumnOutputs out) {
+  wait_for_predecessors();
   const int c = blockIdx.y;
   if (out.p[c] == nullptr) return;
   const int col = blockIdx.x * 32 + (threadIdx.x & 31);
@@ -423,6 +424,7 @@ __global__ void __launch_bounds__(kSlices * 32) columns_join_kernel(const float*
 // The gates of samples first + blockIdx.y: from gates[worker + sample][d] of `workers` groups of threads.
 __global__ void __launch_bounds__(kSlices * 32) gates_join_kernel(const float* __restrict__ gates, int64_t rows, int64_t seq,
                                                                   int64_t workers, int64_t first, int d, void* out, int dtype) {
+  wait_for_predecessors();
   const int64_t sample = first + blockIdx.y;
   const int64_t a = worker_of(sample * seq, rows, workers), b = worker_of((sample + 1) * seq - 1, rows, workers);
   const int col = blockIdx.x * 32 + (threadIdx.x & 31);
@@ -467,9 +469,8 @@ int launch_columns_join(const float* parts, int64_t runs, int d, int wanted, Col
   for (int c = 0; c < kColumns; ++c)
     if ((wanted & (1 << c)) == 0) out.p[c] = nullptr;
   if (wanted == 0) return OPUS_OK;
-  columns_join_kernel<<<dim3((d + 31) / 32, kColumns), kSlices * 32, 0, st>>>(parts, runs, d, out);
+  OPUS_CUDA_TRY(launch_early(columns_join_kernel, dim3((d + 31) / 32, kColumns), kSlices * 32, 0, st, parts, runs, d, out));
   note_launch();
-  OPUS_CUDA_TRY(cudaGetLastError());
   return OPUS_OK;
 }
 
@@ -497,10 +498,10 @@ int launch_one_pass(NormShape s, const opus_residual_norm_args& a, int wanted, c
   if (rc || !per_sample) return rc;
   for (int64_t at = 0; at < a.gate_rows; at += kMaxGridY) {
     const int64_t n = a.gate_rows - at < kMaxGridY ? a.gate_rows - at : kMaxGridY;
-    gates_join_kernel<<<dim3((s.d + 31) / 32, static_cast<unsigned>(n)), kSlices * 32, 0, st>>>(
-        gates, s.rows, s.seq, static_cast<int64_t>(s.blocks) * s.groups, at, s.d, a.grad_gate, a.gate_dtype);
+    OPUS_CUDA_TRY(launch_early(gates_join_kernel, dim3((s.d + 31) / 32, static_cast<unsigned>(n)), kSlices * 32, 0, st,
+                               gates, s.rows, s.seq, static_cast<int64_t>(s.blocks) * s.groups, at, s.d, a.grad_gate,
+                               a.gate_dtype));
     note_launch();
-    OPUS_CUDA_TRY(cudaGetLastError());
   }
   return OPUS_OK;
 }
