@@ -636,25 +636,27 @@ def _type_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _same_device(ref: torch.Tensor, **others: torch.Tensor | None) -> None:
-    """CUDA tensors of one device (checked after shapes and types, so those are checked without a GPU too)."""
-    for name, t in others.items():
-        if t is None:
-            continue
-        _cuda(t, name)
-        if t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
+def _device_index(ref: torch.Tensor, name: str, *others: torch.Tensor | None) -> int:
+    """The CUDA device of ref and of every other tensor (looked at after shapes and types, which need no GPU)."""
+    index = ref.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {ref.device}, another argument on {t.device}")
+    if index < 0:
+        _cuda(ref, name)
+    return index
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """Call an entry point on the device's current stream, with the device current."""
+def _call(name: str, index: int, *args) -> None:
+    """Call an entry point on device `index`, made current, and its current stream; addresses are plain integers."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
-    _lib.check(rc, name)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -699,12 +701,12 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     shape = (*tokens.shape, d)
     if out is not None and (out.shape != shape or out.dtype != weight.dtype or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {weight.dtype} tensor of shape {shape}")
-    _same_device(weight, weight=weight, tokens=tokens, out=out)
-    weight, stride = _rows(weight)
+    index = _device_index(weight, "weight", tokens, out)
+    rows, stride = _rows(weight)
     if out is None:
-        out = torch.empty(shape, dtype=weight.dtype, device=weight.device)
-    _call("opus_embedding", weight.device, _ptr(tokens), bits, tokens.numel(), _ptr(weight), code, V, stride, d,
-          float(scale), _ptr(out))
+        out = weight.new_empty(shape)
+    _call("opus_embedding", index, tokens.data_ptr(), bits, tokens.numel(), rows.data_ptr(), code, V, stride, d,
+          float(scale), out.data_ptr())
     return out
 
 
@@ -742,16 +744,16 @@ def embedding_grad(grad_out: torch.Tensor, tokens: torch.Tensor, num_embeddings:
     dtype = out.dtype if out is not None else out_dtype or grad_out.dtype
     if dtype not in (grad_out.dtype, torch.float32):
         raise ValueError(f"the gradient is {grad_out.dtype} or float32, not {dtype}")
-    _same_device(grad_out, grad_out=grad_out, tokens=tokens, out=out)
-    grad_out, stride = _rows(grad_out)
+    index = _device_index(grad_out, "grad_out", tokens, out)
+    rows, stride = _rows(grad_out)
     if out is None:
-        out = torch.empty(V, d, dtype=dtype, device=grad_out.device)
+        out = grad_out.new_empty((V, d), dtype=dtype)
     n = tokens.numel()
     ws_bytes = int(_lib.load().opus_embedding_grad_workspace_bytes(n, V, d))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=out.device)
-    _call("opus_embedding_grad", out.device, _ptr(grad_out), code, stride, _ptr(tokens), bits, n, V, d, float(scale),
-          -1 if padding_idx is None else int(padding_idx), _ptr(out), _type_code(out, "out"), int(accumulate), _ptr(ws),
-          ws_bytes)
+    ws = tokens.new_empty(ws_bytes, dtype=torch.uint8)
+    _call("opus_embedding_grad", index, rows.data_ptr(), code, stride, tokens.data_ptr(), bits, n, V, d, float(scale),
+          -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _TYPE_CODES[dtype], int(accumulate),
+          ws.data_ptr(), ws_bytes)
     return out
 
 
@@ -760,42 +762,40 @@ _NORM_KINDS = {"rms": 0, "layer": 1}
 _NORM_PARAMS = ("weight", "bias", "post_weight", "post_bias", "gate")
 
 
-def _norm_args(like: torch.Tensor, y: torch.Tensor | None, y_dtype: torch.dtype, params: dict, post: bool, kind: str,
-               residual_scale: float) -> tuple[_lib.ResidualNormArgs, dict]:
-    """The C arguments that forward and backward share, and the contiguous parameters they point to."""
+def _norm_args(like: torch.Tensor, y: torch.Tensor | None, y_dtype: torch.dtype, params: Sequence[torch.Tensor | None],
+               post: bool, kind: str, eps: float, residual_scale: float) -> tuple[_lib.ResidualNormArgs, list]:
+    """The C arguments that forward and backward share, and the contiguous parameters that they point to."""
     if kind not in _NORM_KINDS:
         raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
-    if like.dim() < 1 or like.shape[-1] < 1:
-        raise ValueError(f"rows of at least one element expected, got {tuple(like.shape)}")
-    d = like.shape[-1]
-    a = _lib.ResidualNormArgs()
-    a.rows, a.d, a.kind, a.post = like.numel() // d, d, _NORM_KINDS[kind], int(post)
-    a.x_dtype = _type_code(like, "x")
-    if y_dtype not in _TYPE_CODES or (y_dtype != like.dtype and like.dtype != torch.float32):
+    shape = like.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"rows of at least one element expected, got {tuple(shape)}")
+    d = shape[-1]
+    x_code, y_code = _type_code(like, "x"), _TYPE_CODES.get(y_dtype)
+    if y_code is None or (y_code != x_code and x_code != _lib.DTYPE_F32):
         raise ValueError(f"x must be of y's type (bfloat16, float16 or float32) or float32, got {like.dtype} with "
                          f"{y_dtype}")
-    a.y_dtype = _TYPE_CODES[y_dtype]
-    a.residual_scale = float(residual_scale)
-    if y is not None and y.shape != like.shape:
-        raise ValueError(f"y must have x's shape {tuple(like.shape)}, got {tuple(y.shape)}")
-    if y is None and (post or params.get("gate") is not None):
-        raise ValueError("a gate or a norm after the block needs y")
-    if not post and (params.get("post_weight") is not None or params.get("post_bias") is not None):
+    if y is None:
+        if post or params[4] is not None:
+            raise ValueError("a gate or a norm after the block needs y")
+    elif y.shape != shape:
+        raise ValueError(f"y must have x's shape {tuple(shape)}, got {tuple(y.shape)}")
+    if not post and (params[2] is not None or params[3] is not None):
         raise ValueError("post_weight and post_bias belong to post=True")
-    kept = {}
-    for name in _NORM_PARAMS:
-        p = params.get(name)
+    kept, ptrs, codes, gate_rows = [], [None] * 5, [0] * 5, 0
+    for i, p in enumerate(params):
         if p is None:
             continue
-        code = _type_code(p, name)
-        if name == "gate":
-            a.gate_rows = _gate_rows(p, like)
-        elif p.shape != (d,):
-            raise ValueError(f"{name} must be [{d}], got {tuple(p.shape)}")
-        kept[name] = p = _contig(p.detach())
-        setattr(a, name, p.data_ptr())
-        setattr(a, name + "_dtype", code)
-    return a, kept
+        codes[i] = _type_code(p, _NORM_PARAMS[i])
+        if i == 4:
+            gate_rows = _gate_rows(p, like)
+        elif p.dim() != 1 or p.shape[0] != d:
+            raise ValueError(f"{_NORM_PARAMS[i]} must be [{d}], got {tuple(p.shape)}")
+        p = _contig(p)
+        kept.append(p)
+        ptrs[i] = p.data_ptr()
+    return _lib.ResidualNormArgs(like.numel() // d, d, _NORM_KINDS[kind], int(post), x_code, y_code, eps, residual_scale,
+                                 None, None, 0, 0, *ptrs, *codes, gate_rows), kept
 
 
 def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
@@ -836,22 +836,20 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, weight: tor
         if y is not None:
             raise ValueError(f"out_dtype is y's type where y is given ({y.dtype}), got {out_dtype}")
         n_dtype = out_dtype
-    params = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias, "gate": gate}
-    a, kept = _norm_args(x, y, n_dtype, params, post, kind, residual_scale)
-    a.eps = float(eps)
-    _same_device(x, x=x, y=y, **params)
+    a, kept = _norm_args(x, y, n_dtype, (weight, bias, post_weight, post_bias, gate), post, kind, float(eps),
+                         float(residual_scale))
+    index = _device_index(x, "x", y, *kept)
     xr, a.x_stride = _rows(x)
     a.x = xr.data_ptr()
     if y is not None:
         yr, a.y_stride = _rows(y)
         a.y = yr.data_ptr()
     plain = y is None and a.residual_scale == 1.0
-    h = x if plain else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = torch.empty(x.shape, dtype=n_dtype, device=x.device)
-    stats = torch.empty(a.rows, 4, dtype=torch.float32, device=x.device)
-    a.h, a.h_stride = None if plain else h.data_ptr(), a.d
-    a.n, a.stats = n.data_ptr(), stats.data_ptr()
-    _call("opus_residual_norm", x.device, ctypes.byref(a))
+    h = x if plain else x.new_empty(x.shape)
+    n = x.new_empty(x.shape, dtype=n_dtype)
+    stats = x.new_empty((a.rows, 4), dtype=torch.float32)
+    a.h, a.h_stride, a.n, a.stats = None if plain else h.data_ptr(), a.d, n.data_ptr(), stats.data_ptr()
+    _call("opus_residual_norm", index, ctypes.byref(a))
     return n, h, stats
 
 
@@ -873,42 +871,39 @@ def residual_norm_grad(grad_n: torch.Tensor | None, grad_h: torch.Tensor | None,
     if grad_n is None and grad_h is None:
         raise ValueError("grad_n or grad_h must be given")
     n_dtype = y.dtype if y is not None else grad_n.dtype if grad_n is not None else h.dtype
-    params = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias, "gate": gate}
-    a, kept = _norm_args(h, y, n_dtype, params, post, kind, residual_scale)
+    params = (weight, bias, post_weight, post_bias, gate)
+    a, kept = _norm_args(h, y, n_dtype, params, post, kind, 0.0, float(residual_scale))
     for name, t, dtype in (("grad_n", grad_n, n_dtype), ("grad_h", grad_h, h.dtype)):
         if t is not None and (t.shape != h.shape or t.dtype != dtype):
             raise ValueError(f"{name} must be {dtype} {tuple(h.shape)}, got {t.dtype} {tuple(t.shape)}")
     if stats.shape != (a.rows, 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError(f"stats must be the forward's, a contiguous float32 [{a.rows}, 4]")
-    names = set(kept) if wanted is None else set(wanted)
-    if not names <= set(_NORM_PARAMS):
-        raise ValueError(f"wanted names {sorted(names - set(_NORM_PARAMS))}, parameters are {_NORM_PARAMS}")
-    _same_device(h, h=h, stats=stats, y=y, grad_n=grad_n, grad_h=grad_h, **params)
-    keep = []
-
-    def rows(t):
-        r, stride = _rows(t)
-        keep.append(r)
-        return r.data_ptr(), stride
-
-    a.h, a.h_stride = rows(h)
-    out = {"x": torch.empty(h.shape, dtype=h.dtype, device=h.device)}
+    if wanted is not None:
+        wanted = set(wanted)
+        if not wanted <= set(_NORM_PARAMS):
+            raise ValueError(f"wanted names {sorted(wanted - set(_NORM_PARAMS))}, parameters are {_NORM_PARAMS}")
+    index = _device_index(h, "h", stats, y, grad_n, grad_h, *kept)
+    hr, a.h_stride = _rows(h)
+    grad_x = h.new_empty(h.shape)
+    a.h, a.grad_x, a.stats = hr.data_ptr(), grad_x.data_ptr(), stats.data_ptr()
+    out = {"x": grad_x}
     if y is not None:
-        a.y, a.y_stride = rows(y)
-        out["y"] = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        a.grad_y = out["y"].data_ptr()
+        yr, a.y_stride = _rows(y)
+        out["y"] = grad_y = y.new_empty(y.shape)
+        a.y, a.grad_y = yr.data_ptr(), grad_y.data_ptr()
     if grad_n is not None:
-        a.grad_n, a.grad_n_stride = rows(grad_n)
+        nr, a.grad_n_stride = _rows(grad_n)
+        a.grad_n = nr.data_ptr()
     if grad_h is not None:
-        a.grad_h, a.grad_h_stride = rows(grad_h)
-    a.grad_x, a.stats = out["x"].data_ptr(), stats.data_ptr()
-    for name in _NORM_PARAMS:
-        if name in names and name in kept:
-            out[name] = torch.empty(params[name].shape, dtype=params[name].dtype, device=h.device)
-            setattr(a, "grad_" + name, out[name].data_ptr())
+        dr, a.grad_h_stride = _rows(grad_h)
+        a.grad_h = dr.data_ptr()
+    for name, p in zip(_NORM_PARAMS, params):
+        if p is not None and (wanted is None or name in wanted):
+            out[name] = g = p.new_empty(p.shape)
+            setattr(a, "grad_" + name, g.data_ptr())
     ws_bytes = int(_lib.load().opus_residual_norm_grad_workspace_bytes(ctypes.byref(a)))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=h.device)
-    _call("opus_residual_norm_grad", h.device, ctypes.byref(a), _ptr(ws), ws_bytes)
+    ws = stats.new_empty(ws_bytes, dtype=torch.uint8)
+    _call("opus_residual_norm_grad", index, ctypes.byref(a), ws.data_ptr(), ws_bytes)
     return out
 
 
@@ -945,27 +940,33 @@ class _TensorList:
         dtypes = {t.dtype for t in tensors}
         if not dtypes <= _TYPE_CODES.keys():
             raise ValueError(f"{name} must be bfloat16, float16 or float32 tensors, got {dtypes - _TYPE_CODES.keys()}")
-        if {t.layout for t in tensors} - {torch.strided}:
-            raise ValueError(f"{name} must be dense tensors")
         devices = set(map(torch.Tensor.get_device, tensors))
         if len(devices) > 1:
             raise ValueError(f"{name} are on several devices: {sorted({str(t.device) for t in tensors})}")
-        self.device_index = devices.pop() if devices else -1
+        self.index = devices.pop() if devices else -1
         self.copied = []
-        if not all(map(torch.Tensor.is_contiguous, tensors)):
-            for i, t in enumerate(tensors):
-                if not (t.is_contiguous() if contiguous else _dense(t)):
-                    self.copied.append(t)
-                    tensors[i] = t.contiguous()
+        try:
+            if not all(map(torch.Tensor.is_contiguous, tensors)):
+                for i, t in enumerate(tensors):
+                    if not (t.is_contiguous() if contiguous else _dense(t)):
+                        self.copied.append(t)
+                        tensors[i] = t.contiguous()
+            self.ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
+        except RuntimeError as e:  # a layout without one memory
+            raise ValueError(f"{name} must be dense tensors: {e}") from e
         self.tensors = tensors
-        self.ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
         self.numels = array("q", map(torch.Tensor.numel, tensors))
-        self.types = array("i", [_TYPE_CODES[t.dtype] for t in tensors] if len(dtypes) > 1 else
-                           [_TYPE_CODES[t] for t in dtypes] * self.count)
+        self.types = array("i", [_TYPE_CODES[t] for t in dtypes] * self.count if len(dtypes) <= 1 else
+                           [_TYPE_CODES[t.dtype] for t in tensors])
+
+    def cuda(self, name: str) -> int:
+        if self.index < 0:
+            _cuda(self.tensors[0], name)
+        return self.index
 
 
-def _p(a: array) -> ctypes.c_void_p:
-    return ctypes.c_void_p(a.buffer_info()[0])
+def _p(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
@@ -979,11 +980,12 @@ def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2
     g = _TensorList(grads, "grads")
     if not g.count:
         return torch.tensor(0.0)
-    device = _cuda(g.tensors[0], "grads").device
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    ws = torch.empty(int(_lib.load().opus_grad_norm_workspace_bytes(g.count)), dtype=torch.uint8, device=device)
-    _call("opus_grad_norm", device, _p(g.ptrs), _p(g.numels), _p(g.types), g.count, kind, _ptr(ws), ws.numel(),
-          _ptr(norm))
+    index = g.cuda("grads")
+    norm = g.tensors[0].new_empty((), dtype=torch.float32)
+    ws_bytes = int(_lib.load().opus_grad_norm_workspace_bytes(g.count))
+    ws = norm.new_empty(ws_bytes, dtype=torch.uint8)
+    _call("opus_grad_norm", index, _p(g.ptrs), _p(g.numels), _p(g.types), g.count, kind, ws.data_ptr(), ws_bytes,
+          norm.data_ptr())
     return norm
 
 
@@ -1003,7 +1005,7 @@ def _clip_targets(grads, out, name: str) -> tuple[_TensorList, _TensorList, list
         raise ValueError(f"{name}: out must be contiguous tensors")
     if g.numels != o.numels:
         raise ValueError(f"{name}: out must have a tensor of as many elements for each gradient")
-    if g.count and g.device_index != o.device_index:
+    if g.count and g.index != o.index:
         raise ValueError(f"{name}: out and grads are on different devices")
     return g, o, []
 
@@ -1026,11 +1028,12 @@ def clip_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, no
     g, o, back = _clip_targets(grads, out, "clip_grads")
     if not g.count:
         return torch.tensor(0.0)
-    device = _cuda(g.tensors[0], "grads").device
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    ws = torch.empty(int(_lib.load().opus_grad_norm_workspace_bytes(g.count)), dtype=torch.uint8, device=device)
-    _call("opus_clip_grads", device, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels), g.count, kind,
-          float(max_norm), _ptr(ws), ws.numel(), _ptr(norm))
+    index = g.cuda("grads")
+    norm = g.tensors[0].new_empty((), dtype=torch.float32)
+    ws_bytes = int(_lib.load().opus_grad_norm_workspace_bytes(g.count))
+    ws = norm.new_empty(ws_bytes, dtype=torch.uint8)
+    _call("opus_clip_grads", index, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels), g.count, kind,
+          float(max_norm), ws.data_ptr(), ws_bytes, norm.data_ptr())
     for t, c in back:
         t.copy_(c)
     return norm
@@ -1047,8 +1050,8 @@ def scale_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, n
         raise ValueError(f"norm must be a float32 scalar, got {norm.dtype} {tuple(norm.shape)}")
     if not g.count:
         return
-    _same_device(g.tensors[0], grads=g.tensors[0], norm=norm)
-    _call("opus_scale_grads", g.tensors[0].device, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels),
-          g.count, float(max_norm), _ptr(norm))
+    index = _device_index(g.tensors[0], "grads", norm)
+    _call("opus_scale_grads", index, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels),
+          g.count, float(max_norm), norm.data_ptr())
     for t, c in back:
         t.copy_(c)
