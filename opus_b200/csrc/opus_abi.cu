@@ -51,9 +51,18 @@ int* device_error_word() {
   if (dev < 0 || dev >= kMaxDevices) return nullptr;
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_dev_err[dev] == nullptr) {
+    // the first call may come while a stream is captured: the allocation and the clearing, on a stream of their
+    // own, are not part of what is captured
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
     int* p = nullptr;
-    if (cudaMalloc(&p, sizeof(int) * 4) != cudaSuccess) return nullptr;
-    if (cudaMemset(p, 0, sizeof(int) * 4) != cudaSuccess) return nullptr;
+    cudaStream_t st = nullptr;
+    const bool ok = cudaMalloc(&p, sizeof(int) * 4) == cudaSuccess &&
+                    cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                    cudaMemsetAsync(p, 0, sizeof(int) * 4, st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+    if (st != nullptr) cudaStreamDestroy(st);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) return nullptr;
     g_dev_err[dev] = p;
   }
   return g_dev_err[dev];

@@ -6,10 +6,14 @@ once is off by at most e |v| + K u M: M is the same formula over magnitudes
 (every subtraction an addition), K the length of the longest chain of f32
 operations behind a value.  Each test states its K.
 """
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
 
+from conftest import ROOT
 from opus_b200 import ops
 from opus_b200.layers import GCLinear, ResidualNorm, ScaledEmbedding, residual_norm, scaled_embedding
 from opus_b200.train import clip_grad_norm_, find_GClayers, get_batch_opus, initialize_projector
@@ -725,6 +729,33 @@ def test_captured_and_replayed():
     ops.check_device_error()
 
 
+FIRST_CALL_CAPTURED = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from opus_b200 import ops
+w, t = torch.randn(100, 64, device="cuda"), torch.arange(50, device="cuda") % 7
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.embedding(t, w, scale=2.0)
+    dw = ops.embedding_grad(y, t, 100)
+    n, h, stats = ops.residual_norm(y, y)
+    g = ops.residual_norm_grad(n, h, h, stats, y)
+    norm = ops.grad_norm([dw, n])
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, w[t] * 2) and float(norm) > 0 and bool(g["x"].isfinite().all())
+ops.check_device_error()
+print("captured")
+"""
+
+
+def test_first_call_may_be_captured():
+    """A process whose first use of the library is inside a captured graph (its error word is made there)."""
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED, str(ROOT)], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
 def test_on_other_streams_at_once():
     states = [training_state(s) for s in range(4)]
     want = [[t.clone() for t in training_ops(s)] for s in states]
@@ -802,7 +833,7 @@ def test_training_step_of_the_layers(kind):
     ref = torch.nn.functional.cross_entropy(plain_logits(model, tokens[:, :-1], params).view(-1, 300), tokens[:, 1:].reshape(-1))
     grads = dict(zip(params, torch.autograd.grad(ref, list(params.values()))))
     grads["embed.weight"][0] = 0.0  # the padding row
-    assert abs(float(loss) - float(ref)) < 1e-4 * float(ref)
+    assert abs(float(loss.detach()) - float(ref.detach())) < 1e-4 * float(ref.detach())
     for k, p in model.named_parameters():
         assert float((p.grad.double() - grads[k]).abs().max()) <= 1e-4 * float(grads[k].abs().max()), k
     before = {k: p.grad.clone() for k, p in model.named_parameters()}
