@@ -97,6 +97,7 @@ SIGNATURES: dict[str, tuple] = {
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 _timer = None  # the active KernelTimer, if any
+_tensor_list = None
 
 # entry points that launch no kernel of their own or only query state
 _UNTIMED = {"opus_abi_version", "opus_last_error", "opus_device_error", "opus_sketch_table_entries",
@@ -189,6 +190,19 @@ def _load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+def tensor_list():
+    """The compiled module that walks lists of tensors (built beside the library)."""
+    global _tensor_list
+    if _tensor_list is None:
+        try:
+            from . import _tensor_list as module
+        except ImportError as e:
+            raise ImportError("opus_b200/_tensor_list.so is not built for this Python and torch; run `python -m "
+                              "opus_b200.csrc.build`") from e
+        _tensor_list = module
+    return _tensor_list
 
 
 def last_error() -> str:

@@ -5,16 +5,19 @@ Usage: python -m opus_b200.csrc.build [--verbose]
 Each .cu file is compiled to an object under opus_b200/_build/ (in parallel,
 skipped when up to date) and linked into opus_b200/libopus_b200.so with the
 CUDA runtime linked statically, so the library has no dependency on the
-Python environment.
+Python environment.  tensor_list.cpp becomes the extension module
+opus_b200/_tensor_list.so, against this Python's and torch's headers.
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -22,6 +25,7 @@ PKG = CSRC.parent
 ROOT = PKG.parent
 BUILD = PKG / "_build"
 LIB = PKG / "libopus_b200.so"
+MODULE = PKG / "_tensor_list.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -74,15 +78,40 @@ def _compile(src: Path, verbose: bool, extra: list[str]) -> Path:
     return obj
 
 
+def build_module(verbose: bool = False, force: bool = False) -> Path:
+    """The extension module that walks lists of torch tensors."""
+    src = CSRC / "tensor_list.cpp"
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        raise RuntimeError("torch not found: cannot build _tensor_list.so")
+    torch_dir = Path(spec.origin).resolve().parent
+    cuda_include = Path(nvcc()).resolve().parent.parent / "include"
+    if not force and not _stale(MODULE, src, [ROOT / "include" / "opus_b200.h", torch_dir / "version.py"]):
+        return MODULE
+    tmp = MODULE.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden", f"-I{sysconfig.get_paths()['include']}", "-isystem", str(torch_dir / "include"),
+           "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda_include),
+           str(src), f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"c++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, MODULE)
+    return MODULE
+
+
 def build(verbose: bool = False, force: bool = False, extra: list[str] | None = None) -> Path:
     extra = list(extra or [])
     BUILD.mkdir(parents=True, exist_ok=True)
     deps = headers()
     srcs = sources()
     todo = [s for s in srcs if force or extra or _stale(BUILD / (s.stem + ".o"), s, deps)]
-    if todo:
-        with cf.ThreadPoolExecutor(max_workers=min(8, len(todo))) as ex:
-            list(ex.map(lambda s: _compile(s, verbose, extra), todo))
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        module = ex.submit(build_module, verbose, force)
+        list(ex.map(lambda s: _compile(s, verbose, extra), todo))
+        module.result()
     objs = [BUILD / (s.stem + ".o") for s in srcs]
     if todo or not LIB.exists() or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs):
         tmp = LIB.with_suffix(".so.tmp")

@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from array import array
 from collections.abc import Iterable, Sequence
 
 import torch
@@ -936,37 +935,21 @@ class _TensorList:
 
     def __init__(self, tensors: torch.Tensor | Iterable[torch.Tensor], name: str, contiguous: bool = False):
         tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-        self.count = len(tensors)
-        dtypes = {t.dtype for t in tensors}
-        if not dtypes <= _TYPE_CODES.keys():
-            raise ValueError(f"{name} must be bfloat16, float16 or float32 tensors, got {dtypes - _TYPE_CODES.keys()}")
-        devices = set(map(torch.Tensor.get_device, tensors))
-        if len(devices) > 1:
-            raise ValueError(f"{name} are on several devices: {sorted({str(t.device) for t in tensors})}")
-        self.index = devices.pop() if devices else -1
-        self.copied = []
-        try:
-            if not all(map(torch.Tensor.is_contiguous, tensors)):
-                for i, t in enumerate(tensors):
-                    if not (t.is_contiguous() if contiguous else _dense(t)):
-                        self.copied.append(t)
-                        tensors[i] = t.contiguous()
-            self.ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
-        except RuntimeError as e:  # a layout without one memory
-            raise ValueError(f"{name} must be dense tensors: {e}") from e
-        self.tensors = tensors
-        self.numels = array("q", map(torch.Tensor.numel, tensors))
-        self.types = array("i", [_TYPE_CODES[t] for t in dtypes] * self.count if len(dtypes) <= 1 else
-                           [_TYPE_CODES[t.dtype] for t in tensors])
+        self.count, self.tensors, self.copied = len(tensors), tensors, []
+        scan = _lib.tensor_list().scan
+        self.ptrs, self.numels, self.types, self.index, odd = scan(tensors, name)
+        for i in odd:
+            t = tensors[i]
+            if contiguous or not _dense(t):
+                self.copied.append(t)
+                tensors[i] = t.contiguous()
+        if self.copied:
+            self.ptrs = scan(tensors, name)[0]
 
     def cuda(self, name: str) -> int:
         if self.index < 0:
             _cuda(self.tensors[0], name)
         return self.index
-
-
-def _p(a: array) -> int:
-    return a.buffer_info()[0]
 
 
 def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
@@ -984,7 +967,7 @@ def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2
     norm = g.tensors[0].new_empty((), dtype=torch.float32)
     ws_bytes = int(_lib.load().opus_grad_norm_workspace_bytes(g.count))
     ws = norm.new_empty(ws_bytes, dtype=torch.uint8)
-    _call("opus_grad_norm", index, _p(g.ptrs), _p(g.numels), _p(g.types), g.count, kind, ws.data_ptr(), ws_bytes,
+    _call("opus_grad_norm", index, g.ptrs, g.numels, g.types, g.count, kind, ws.data_ptr(), ws_bytes,
           norm.data_ptr())
     return norm
 
@@ -1000,8 +983,8 @@ def _clip_targets(grads, out, name: str) -> tuple[_TensorList, _TensorList, list
             if any(stride == 0 and size > 1 for stride, size in zip(t.stride(), t.shape)):
                 raise ValueError(f"{name}: a gradient's elements overlap in memory (an expanded tensor)")
         return g, g, [(t, c) for t, c in zip(grads, g.tensors) if t is not c]
-    g, o = _TensorList(grads, "grads", contiguous=True), _TensorList(out, "out")
-    if o.copied or not all(map(torch.Tensor.is_contiguous, o.tensors)):
+    g, o = _TensorList(grads, "grads", contiguous=True), _TensorList(out, "out", contiguous=True)
+    if o.copied:
         raise ValueError(f"{name}: out must be contiguous tensors")
     if g.numels != o.numels:
         raise ValueError(f"{name}: out must have a tensor of as many elements for each gradient")
@@ -1032,7 +1015,7 @@ def clip_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, no
     norm = g.tensors[0].new_empty((), dtype=torch.float32)
     ws_bytes = int(_lib.load().opus_grad_norm_workspace_bytes(g.count))
     ws = norm.new_empty(ws_bytes, dtype=torch.uint8)
-    _call("opus_clip_grads", index, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels), g.count, kind,
+    _call("opus_clip_grads", index, g.ptrs, g.types, o.ptrs, o.types, g.numels, g.count, kind,
           float(max_norm), ws.data_ptr(), ws_bytes, norm.data_ptr())
     for t, c in back:
         t.copy_(c)
@@ -1051,7 +1034,7 @@ def scale_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, n
     if not g.count:
         return
     index = _device_index(g.tensors[0], "grads", norm)
-    _call("opus_scale_grads", index, _p(g.ptrs), _p(g.types), _p(o.ptrs), _p(o.types), _p(g.numels),
+    _call("opus_scale_grads", index, g.ptrs, g.types, o.ptrs, o.types, g.numels,
           g.count, float(max_norm), norm.data_ptr())
     for t, c in back:
         t.copy_(c)
