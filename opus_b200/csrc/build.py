@@ -38,10 +38,6 @@ NVCC_FLAGS = ARCH_FLAGS + [
     f"-I{ROOT / 'include'}",
 ]
 
-# Files of many template instances: their functions are compiled in parallel.
-SPLIT = ["--split-compile=0", "-Xptxas", "-split-compile=0"]
-FILE_FLAGS = {"residual_norm.cu": SPLIT, "residual_norm_grad.cu": SPLIT}
-
 
 def nvcc() -> str:
     for cand in (os.environ.get("NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
@@ -67,7 +63,7 @@ def _stale(obj: Path, src: Path, deps: list[Path]) -> bool:
 
 def _compile(src: Path, verbose: bool, extra: list[str]) -> Path:
     obj = BUILD / (src.stem + ".o")
-    cmd = [nvcc(), *NVCC_FLAGS, *FILE_FLAGS.get(src.name, []), *extra, "-c", str(src), "-o", str(obj)]
+    cmd = [nvcc(), *NVCC_FLAGS, *extra, "-c", str(src), "-o", str(obj)]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

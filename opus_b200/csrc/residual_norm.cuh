@@ -21,10 +21,16 @@ namespace opus {
 constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxWidth = 16384;
 
-// Rows of up to kNormNarrow elements take up to 16 elements a thread and 256 threads; wider ones 32 elements and
-// 512 threads, or 16 and 1024 where vectors have one element.
-constexpr int kNormNarrow = 4096;
-constexpr int wide_vectors(int V) { return V == 1 ? 16 : 32 / V; }
+// Narrow rows (up to 4096 elements) take up to 16 elements a thread and 256 threads, wider ones 32 elements and 512
+// threads.  Vectors of one element need more registers each (an address, a predicate): with a norm of y or a gate
+// narrow rows end at 2048 and take 8 elements a thread, and wide ones take 1024 threads with 8 elements up to 8192 and
+// 16 beyond.  Registers that spill cost more than anything else here: 50000 x 771 f32 with both norms took 335 us
+// forward with 16 elements a thread and 820 bytes spilled, 157 us with 8; without them 128 us with 8, 107 with 16.
+constexpr int narrow_vectors(int V, bool full) { return V == 1 && full ? 8 : 16 / V; }
+constexpr int norm_narrow(int V, bool full) { return 256 * narrow_vectors(V, full) * V; }
+// the smaller choice for shorter rows (vectors of 8: one vector)
+constexpr int fewer_vectors(int V, bool full) { return V == 1 ? 4 : narrow_vectors(V, full) / 2; }
+constexpr int kNormScalarMiddle = 8192;
 constexpr int norm_threads(int V, bool wide) { return !wide ? 256 : V == 1 ? 1024 : 512; }
 
 struct NormShape {
@@ -275,6 +281,47 @@ constexpr int kNormSharedParams = 160 * 1024;
 int norm_shape(const char* what, const opus_residual_norm_args* a, int V, int most, NormShape* s, int* nv);
 int check_norm(const char* what, const opus_residual_norm_args* a);
 bool norm_params_aligned(const opus_residual_norm_args* a);
+
+// ---- the backward's sums over rows
+enum Column : int { kWeight = 0, kBias, kPostWeight, kPostBias, kGate, kColumns };
+
+struct ColumnOutputs {
+  void* p[kColumns];
+  int dtype[kColumns];
+};
+
+constexpr int kRun = 64;  // rows of a run at least
+struct Runs {
+  int64_t seq, run;
+  int64_t samples;
+  int per_seq;
+};
+// Runs of rows that stay inside `seq` neighbours: at least kRun rows each, and about a thousand in all.
+inline Runs runs_of(int64_t rows, int64_t seq) {
+  Runs r;
+  r.seq = seq;
+  r.samples = seq > 0 ? rows / seq : 0;
+  int64_t run = (rows + 1023) / 1024;
+  r.run = run > kRun ? run : kRun;
+  r.per_seq = static_cast<int>((seq + r.run - 1) / r.run);
+  return r;
+}
+
+inline int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+constexpr int kGradBlocksPerSm = 4;  // of the one-pass kernel at most: bounds the workspace
+
+// The kernels of one pair of types are compiled in a file of their own (residual_norm_<types>.cu).
+#define OPUS_NORM_LAUNCHES(NAME)                                                                                       \
+  int residual_norm_##NAME(const opus_residual_norm_args& a, bool vec, cudaStream_t st);                               \
+  int residual_norm_grad_##NAME(const opus_residual_norm_args& a, bool vec, int wanted, const ColumnOutputs& out,      \
+                                uint8_t* ws, cudaStream_t st);
+OPUS_NORM_LAUNCHES(bf16)
+OPUS_NORM_LAUNCHES(f16)
+OPUS_NORM_LAUNCHES(f32)
+OPUS_NORM_LAUNCHES(f32_bf16)
+OPUS_NORM_LAUNCHES(f32_f16)
+#undef OPUS_NORM_LAUNCHES
 
 // Sets a kernel's dynamic shared memory limit where it needs more than the default.
 template <auto Kernel>

@@ -1,4 +1,4 @@
-// Residual norm, backward.
+// Residual norm, backward: kernels and their launch, for one pair of types (included by residual_norm_<types>.cu).
 //
 // With hh = (h - mean) / sd the normed row, a = dn o w and <.> the mean over a
 // row (<a> for layer norms only):
@@ -8,7 +8,7 @@
 //   dy = dz, or through the norm of y: c = dz o w_post,
 //   dy = (c - <c> - yh <c yh>) / sd_y;  dw_post = sum dz o yh;  db_post = sum dz
 //
-// d up to 4096: one kernel reads each row once, writes dx and dy, and keeps a
+// Narrow rows (norm_narrow: d up to 4096 or 2048): one kernel reads each row once, writes dx and dy, and keeps a
 // column's sums over its run of rows in registers (16 columns a thread, five
 // sums each); a second kernel joins the runs.  Wider rows would need more
 // than 256 threads and leave them too few registers for that: one kernel for
@@ -16,12 +16,12 @@
 // join.  Every sum has a fixed order.
 //
 // Bound: HBM bandwidth (h, dn, dh_in and y read once, dx and dy written once).
+#pragma once
+
 #include "residual_norm.cuh"
 
 namespace opus {
 namespace {
-
-enum Column : int { kWeight = 0, kBias, kPostWeight, kPostBias, kGate, kColumns };
 
 // The worker (group of threads) whose run of rows holds `row`: RowRun's split, inverted.
 __device__ __forceinline__ int64_t worker_of(int64_t row, int64_t rows, int64_t n) {
@@ -299,7 +299,6 @@ __global__ void __launch_bounds__(norm_threads(V, true))
 }
 
 constexpr int kColWarps = 8;
-constexpr int kRun = 64;  // rows of a run at least
 
 template <int V>
 __device__ __forceinline__ void column_param(const void* p, int dtype, int64_t at, float other, float (&r)[V]) {
@@ -384,11 +383,6 @@ __global__ void __launch_bounds__(kColWarps * 32)
   }
 }
 
-struct ColumnOutputs {
-  void* p[kColumns];
-  int dtype[kColumns];
-};
-
 constexpr int kSlices = 32;
 
 // Sums v[first + r * stride + col] over r in [0, count) for 32 columns by the block's 32 slices; warp 0 has the result.
@@ -409,28 +403,26 @@ __device__ __forceinline__ float join_parts(const float* v, int64_t count, int64
   return x;  // of column `slice`, in every lane
 }
 
-// blockIdx.y: an array of parts[run][array][d] (its sums over all runs).
+// blockIdx.y < kColumns: an array of parts[run][array][d] (its sums over all runs).  Behind them the gates of samples
+// first + blockIdx.y - kColumns, from gates[worker + sample][d] of `workers` groups of threads.
 __global__ void __launch_bounds__(kSlices * 32) columns_join_kernel(const float* __restrict__ parts, int64_t runs, int d,
-                                                                    const __grid_constant__ ColumnOutputs out) {
+                                                                    const __grid_constant__ ColumnOutputs out,
+                                                                    const float* __restrict__ gates, int64_t rows,
+                                                                    int64_t seq, int64_t workers, int64_t first, void* gate) {
   wait_for_predecessors();
-  const int c = blockIdx.y;
-  if (out.p[c] == nullptr) return;
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
-  const float v = join_parts(parts + static_cast<int64_t>(c) * d + col, runs, static_cast<int64_t>(kColumns) * d, col < d);
-  const int at = blockIdx.x * 32 + (threadIdx.x >> 5);
-  if ((threadIdx.x & 31) == 0 && at < d) store_any(out.p[c], out.dtype[c], at, v);
-}
-
-// The gates of samples first + blockIdx.y: from gates[worker + sample][d] of `workers` groups of threads.
-__global__ void __launch_bounds__(kSlices * 32) gates_join_kernel(const float* __restrict__ gates, int64_t rows, int64_t seq,
-                                                                  int64_t workers, int64_t first, int d, void* out, int dtype) {
-  wait_for_predecessors();
-  const int64_t sample = first + blockIdx.y;
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), at = blockIdx.x * 32 + (threadIdx.x >> 5);
+  const bool writes = (threadIdx.x & 31) == 0 && at < d;
+  if (blockIdx.y < kColumns) {
+    const int c = blockIdx.y;
+    if (out.p[c] == nullptr) return;
+    const float v = join_parts(parts + static_cast<int64_t>(c) * d + col, runs, static_cast<int64_t>(kColumns) * d, col < d);
+    if (writes) store_any(out.p[c], out.dtype[c], at, v);
+    return;
+  }
+  const int64_t sample = first + blockIdx.y - kColumns;
   const int64_t a = worker_of(sample * seq, rows, workers), b = worker_of((sample + 1) * seq - 1, rows, workers);
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
   const float v = join_parts(gates + (a + sample) * d + col, b - a + 1, d, col < d);
-  const int at = blockIdx.x * 32 + (threadIdx.x >> 5);
-  if ((threadIdx.x & 31) == 0 && at < d) store_any(out, dtype, sample * d + at, v);
+  if (writes) store_any(gate, out.dtype[kGate], sample * d + at, v);
 }
 
 // The gates of wide rows: runs per_seq of each sample, array kGate of parts[run][array][d].
@@ -444,33 +436,24 @@ __global__ void __launch_bounds__(kSlices * 32) gate_runs_join_kernel(const floa
   if ((threadIdx.x & 31) == 0 && at < d) store_any(out, dtype, sample * d + at, v);
 }
 
-struct Runs {
-  int64_t seq, run;
-  int64_t samples;
-  int per_seq;
-};
-// Runs of rows that stay inside `seq` neighbours: at least kRun rows each, and about a thousand in all.
-Runs runs_of(int64_t rows, int64_t seq) {
-  Runs r;
-  r.seq = seq;
-  r.samples = seq > 0 ? rows / seq : 0;
-  int64_t run = (rows + 1023) / 1024;
-  r.run = run > kRun ? run : kRun;
-  r.per_seq = static_cast<int>((seq + r.run - 1) / r.run);
-  return r;
-}
+constexpr int64_t kMaxSamples = 65535 - kColumns;  // of one launch: the grid's y limit
 
-int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
-
-constexpr int kGradBlocksPerSm = 4;  // of the one-pass kernel at most: bounds the workspace
-constexpr int64_t kMaxGridY = 65535;
-
-int launch_columns_join(const float* parts, int64_t runs, int d, int wanted, ColumnOutputs out, cudaStream_t st) {
+// Joins the arrays in `wanted`, and the gates of `samples` samples into gate.
+int launch_columns_join(const float* parts, int64_t runs, const NormShape& s, int wanted, ColumnOutputs out,
+                        const float* gates, int64_t samples, void* gate, cudaStream_t st) {
   for (int c = 0; c < kColumns; ++c)
     if ((wanted & (1 << c)) == 0) out.p[c] = nullptr;
-  if (wanted == 0) return OPUS_OK;
-  OPUS_CUDA_TRY(launch_early(columns_join_kernel, dim3((d + 31) / 32, kColumns), kSlices * 32, 0, st, parts, runs, d, out));
-  note_launch();
+  const int64_t workers = static_cast<int64_t>(s.blocks) * s.groups;
+  int64_t at = 0;
+  do {
+    const int64_t n = samples - at < kMaxSamples ? samples - at : kMaxSamples;
+    const dim3 grid((s.d + 31) / 32, static_cast<unsigned>(kColumns + n));
+    OPUS_CUDA_TRY(launch_early(columns_join_kernel, grid, kSlices * 32, 0, st, parts, runs, s.d, out, gates, s.rows, s.seq,
+                               workers, at, gate));
+    note_launch();
+    for (int c = 0; c < kColumns; ++c) out.p[c] = nullptr;  // joined
+    at += kMaxSamples;
+  } while (at < samples);
   return OPUS_OK;
 }
 
@@ -494,16 +477,9 @@ int launch_one_pass(NormShape s, const opus_residual_norm_args& a, int wanted, c
   note_launch();
   OPUS_CUDA_TRY(cudaGetLastError());
   const bool per_sample = s.seq != s.rows && (wanted & (1 << kGate)) != 0;
-  const int rc = launch_columns_join(parts, s.blocks, s.d, per_sample ? wanted & ~(1 << kGate) : wanted, out, st);
-  if (rc || !per_sample) return rc;
-  for (int64_t at = 0; at < a.gate_rows; at += kMaxGridY) {
-    const int64_t n = a.gate_rows - at < kMaxGridY ? a.gate_rows - at : kMaxGridY;
-    OPUS_CUDA_TRY(launch_early(gates_join_kernel, dim3((s.d + 31) / 32, static_cast<unsigned>(n)), kSlices * 32, 0, st,
-                               gates, s.rows, s.seq, static_cast<int64_t>(s.blocks) * s.groups, at, s.d, a.grad_gate,
-                               a.gate_dtype));
-    note_launch();
-  }
-  return OPUS_OK;
+  const int whole = per_sample ? wanted & ~(1 << kGate) : wanted;
+  if (wanted == 0) return OPUS_OK;
+  return launch_columns_join(parts, s.blocks, s, whole, out, gates, per_sample ? a.gate_rows : 0, a.grad_gate, st);
 }
 
 template <typename TX, typename TY, int V>
@@ -517,8 +493,11 @@ int launch_columns(const NormShape& s, const opus_residual_norm_args& a, const f
 }
 
 template <typename TX, typename TY, int V, int NV>
-int launch_wide(NormShape s, const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws,
-                cudaStream_t st) {
+int backward_wide(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
+  NormShape s;
+  int nv;
+  const int shaped = norm_shape("residual_norm_grad", &a, V, NV, &s, &nv);
+  if (shaped) return shaped;
   float2* means = reinterpret_cast<float2*>(ws);
   float* parts = reinterpret_cast<float*>(ws + align256(s.rows * 8));
   constexpr auto kernel = rows_kernel<TX, TY, V, NV>;
@@ -537,13 +516,13 @@ int launch_wide(NormShape s, const opus_residual_norm_args& a, int wanted, const
   if (whole != 0) {
     const Runs r = runs_of(s.rows, s.rows);
     rc = launch_columns<TX, TY, V>(s, a, means, whole, r, parts, st);
-    if (rc == OPUS_OK) rc = launch_columns_join(parts, r.per_seq, s.d, whole, out, st);
+    if (rc == OPUS_OK) rc = launch_columns_join(parts, r.per_seq, s, whole, out, nullptr, 0, nullptr, st);
   }
   if (rc || !per_sample) return rc;
   const Runs r = runs_of(s.rows, s.seq);
   rc = launch_columns<TX, TY, V>(s, a, means, 1 << kGate, r, parts, st);
-  for (int64_t at = 0; rc == OPUS_OK && at < r.samples; at += kMaxGridY) {
-    const int64_t n = r.samples - at < kMaxGridY ? r.samples - at : kMaxGridY;
+  for (int64_t at = 0; rc == OPUS_OK && at < r.samples; at += kMaxSamples) {
+    const int64_t n = r.samples - at < kMaxSamples ? r.samples - at : kMaxSamples;
     gate_runs_join_kernel<<<dim3((s.d + 31) / 32, static_cast<unsigned>(n)), kSlices * 32, 0, st>>>(
         parts, r.per_seq, at, s.d, a.grad_gate, a.gate_dtype);
     note_launch();
@@ -553,129 +532,50 @@ int launch_wide(NormShape s, const opus_residual_norm_args& a, int wanted, const
 }
 
 template <typename TX, typename TY, int V, bool Full, bool Bias>
-int launch_by_width(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
-  // 16 elements a thread, 8 where the sums of 16 columns would not leave registers enough and 8 reach the row's end
-  constexpr bool kLean = V < 8 && Full && (Bias || V == 1);
-  constexpr int kMost = 16 / V, kLess = 8 / V;
+int backward_by_width(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
+  // 16 elements a thread, 8 where the sums of 16 f32 columns would not leave registers enough (with biases) and 8
+  // reach the row's end
+  constexpr int kMost = narrow_vectors(V, Full), kFewer = fewer_vectors(V, Full);
+  constexpr bool kLean = V == 4 && Full && Bias;
   NormShape s;
   int nv;
-  const bool lean = kLean && a.d <= kNormNarrow / 2;
-  const int rc = norm_shape("residual_norm_grad", &a, V, lean ? kLess : kMost, &s, &nv);
+  const bool lean = kLean && a.d <= norm_narrow(V, Full) / 2;
+  const int rc = norm_shape("residual_norm_grad", &a, V, lean ? kFewer : kMost, &s, &nv);
   if (rc) return rc;
   if constexpr (V > 1) {
     if (nv == 1) return launch_one_pass<TX, TY, V, 1, Full, Bias>(s, a, wanted, out, ws, st);
   }
-  if constexpr (V == 4) {
-    if (nv == 2) return launch_one_pass<TX, TY, V, 2, Full, Bias>(s, a, wanted, out, ws, st);
-  }
-  if constexpr (V == 1) {
-    if (nv <= 4) return launch_one_pass<TX, TY, V, 4, Full, Bias>(s, a, wanted, out, ws, st);
-    if constexpr (kLean) {
-      if (nv == 8) return launch_one_pass<TX, TY, V, 8, Full, Bias>(s, a, wanted, out, ws, st);
-    }
+  if constexpr (V < 8) {
+    if (nv <= kFewer) return launch_one_pass<TX, TY, V, kFewer, Full, Bias>(s, a, wanted, out, ws, st);
   }
   return launch_one_pass<TX, TY, V, kMost, Full, Bias>(s, a, wanted, out, ws, st);
 }
 
 template <typename TX, typename TY, int V>
-int launch_by_form(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
-  if (a.d > kNormNarrow) {
-    NormShape s;
-    int nv;
-    const int rc = norm_shape("residual_norm_grad", &a, V, wide_vectors(V), &s, &nv);
-    if (rc) return rc;
-    return launch_wide<TX, TY, V, wide_vectors(V)>(s, a, wanted, out, ws, st);
+int backward_by_form(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
+  const bool full = a.post || a.gate != nullptr;
+  if (a.d > norm_narrow(V, full)) {
+    if constexpr (V == 1) {
+      if (a.d <= kNormScalarMiddle) return backward_wide<TX, TY, V, 8>(a, wanted, out, ws, st);
+      return backward_wide<TX, TY, V, 16>(a, wanted, out, ws, st);
+    } else {
+      return backward_wide<TX, TY, V, 32 / V>(a, wanted, out, ws, st);
+    }
   }
   const bool bias = a.post_bias != nullptr || (wanted & (1 << kBias)) != 0;
-  if (a.post || a.gate != nullptr)
-    return bias ? launch_by_width<TX, TY, V, true, true>(a, wanted, out, ws, st)
-                : launch_by_width<TX, TY, V, true, false>(a, wanted, out, ws, st);
-  return bias ? launch_by_width<TX, TY, V, false, true>(a, wanted, out, ws, st)
-              : launch_by_width<TX, TY, V, false, false>(a, wanted, out, ws, st);
+  if (full)
+    return bias ? backward_by_width<TX, TY, V, true, true>(a, wanted, out, ws, st)
+                : backward_by_width<TX, TY, V, true, false>(a, wanted, out, ws, st);
+  return bias ? backward_by_width<TX, TY, V, false, true>(a, wanted, out, ws, st)
+              : backward_by_width<TX, TY, V, false, false>(a, wanted, out, ws, st);
 }
 
 template <typename TX, typename TY>
-int launch_by_alignment(const opus_residual_norm_args& a, bool vec, int wanted, const ColumnOutputs& out, uint8_t* ws,
+int backward_by_alignment(const opus_residual_norm_args& a, bool vec, int wanted, const ColumnOutputs& out, uint8_t* ws,
                         cudaStream_t st) {
-  return vec ? launch_by_form<TX, TY, 16 / sizeof(TX)>(a, wanted, out, ws, st)
-             : launch_by_form<TX, TY, 1>(a, wanted, out, ws, st);
+  return vec ? backward_by_form<TX, TY, 16 / sizeof(TX)>(a, wanted, out, ws, st)
+             : backward_by_form<TX, TY, 1>(a, wanted, out, ws, st);
 }
-
-bool on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 }  // namespace
 }  // namespace opus
-
-using namespace opus;
-
-extern "C" int64_t opus_residual_norm_grad_workspace_bytes(const opus_residual_norm_args* a) {
-  if (a == nullptr || a->rows <= 0 || a->d < 1) return 256;
-  const int64_t samples = a->gate != nullptr && a->gate_rows > 1 && a->rows % a->gate_rows == 0 ? a->gate_rows : 0;
-  const Runs whole = runs_of(a->rows, a->rows);
-  int64_t runs = whole.samples * whole.per_seq;
-  if (samples > 0) {
-    const Runs r = runs_of(a->rows, a->rows / samples);
-    if (r.samples * r.per_seq > runs) runs = r.samples * r.per_seq;
-  }
-  const int64_t wide = align256(a->rows * 8) + align256(runs * kColumns * a->d * 4);
-  // the one-pass kernel: a block holds at most 256 rows, and no more blocks run than there are rows
-  int64_t blocks = static_cast<int64_t>(sm_count()) * kGradBlocksPerSm;
-  blocks = blocks < a->rows ? blocks : a->rows;
-  int64_t workers = 0;
-  if (samples > 0) {
-    workers = blocks * (a->d > 2048 ? 1 : a->d > 256 ? 8 : 256);
-    workers = (workers < a->rows + 256 ? workers : a->rows + 256) + samples;
-  }
-  const int64_t one_pass = align256((blocks * kColumns + workers) * a->d * 4);
-  return wide > one_pass ? wide : one_pass;
-}
-
-extern "C" int opus_residual_norm_grad(const opus_residual_norm_args* args, void* workspace, int64_t workspace_bytes,
-                                       void* stream) {
-  int rc = check_norm("residual_norm_grad", args);
-  if (rc) return rc;
-  const opus_residual_norm_args& a = *args;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  void* outs[kColumns] = {a.grad_weight, a.grad_bias, a.grad_post_weight, a.grad_post_bias, a.grad_gate};
-  const void* of[kColumns] = {a.weight, a.bias, a.post_weight, a.post_bias, a.gate};
-  const int types[kColumns] = {a.weight_dtype, a.bias_dtype, a.post_weight_dtype, a.post_bias_dtype, a.gate_dtype};
-  int wanted = 0;
-  for (int c = 0; c < kColumns; ++c) {
-    if (outs[c] == nullptr) continue;
-    if (of[c] == nullptr) return set_error(OPUS_ERR_INVALID, "residual_norm_grad: a gradient of no parameter");
-    if (!on(outs[c], dtype_bytes(types[c])))
-      return set_error(OPUS_ERR_INVALID, "residual_norm_grad: a pointer is not aligned to its elements");
-    wanted |= 1 << c;
-    if (a.rows == 0)
-      OPUS_CUDA_TRY(cudaMemsetAsync(outs[c], 0, (c == kGate ? a.gate_rows : 1) * static_cast<int64_t>(a.d) * dtype_bytes(types[c]), st));
-  }
-  if (a.rows == 0) return OPUS_OK;
-  if (!a.h || !a.stats || !a.grad_x || (!a.grad_n && !a.grad_h) || (a.y != nullptr && a.grad_y == nullptr) ||
-      (a.y == nullptr && a.grad_y != nullptr) || !workspace)
-    return set_error(OPUS_ERR_INVALID, "residual_norm_grad: NULL pointer");
-  if (workspace_bytes < opus_residual_norm_grad_workspace_bytes(&a))
-    return set_error(OPUS_ERR_INVALID, "residual_norm_grad: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
-                     (long long)opus_residual_norm_grad_workspace_bytes(&a));
-  if (!on(workspace, 256)) return set_error(OPUS_ERR_INVALID, "residual_norm_grad: workspace must be 256-byte aligned");
-  const int xb = dtype_bytes(a.x_dtype), yb = dtype_bytes(a.y_dtype);
-  if (a.h_stride < a.d || (a.y && a.y_stride < a.d) || (a.grad_n && a.grad_n_stride < a.d) ||
-      (a.grad_h && a.grad_h_stride < a.d))
-    return set_error(OPUS_ERR_INVALID, "residual_norm_grad: row stride < d");
-  if (!on(a.h, xb) || !on(a.grad_h, xb) || !on(a.grad_x, xb) || !on(a.y, yb) || !on(a.grad_n, yb) ||
-      !on(a.grad_y, yb) || !on(a.stats, 16))
-    return set_error(OPUS_ERR_INVALID, "residual_norm_grad: a pointer is not aligned to its elements");
-  const int V = 16 / xb;
-  const bool vec = norm_params_aligned(&a) && a.d % V == 0 && a.h_stride % V == 0 && on(a.h, 16) && on(a.grad_x, 16) && on(a.grad_y, V * yb) &&
-                   (!a.y || (a.y_stride % V == 0 && on(a.y, V * yb))) &&
-                   (!a.grad_n || (a.grad_n_stride % V == 0 && on(a.grad_n, V * yb))) &&
-                   (!a.grad_h || (a.grad_h_stride % V == 0 && on(a.grad_h, 16)));
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const ColumnOutputs out{{outs[0], outs[1], outs[2], outs[3], outs[4]}, {types[0], types[1], types[2], types[3], types[4]}};
-  if (a.x_dtype == OPUS_DTYPE_F32) {
-    if (a.y_dtype == OPUS_DTYPE_F32) return launch_by_alignment<float, float>(a, vec, wanted, out, ws, st);
-    if (a.y_dtype == OPUS_DTYPE_F16) return launch_by_alignment<float, __half>(a, vec, wanted, out, ws, st);
-    return launch_by_alignment<float, __nv_bfloat16>(a, vec, wanted, out, ws, st);
-  }
-  if (a.x_dtype == OPUS_DTYPE_F16) return launch_by_alignment<__half, __half>(a, vec, wanted, out, ws, st);
-  return launch_by_alignment<__nv_bfloat16, __nv_bfloat16>(a, vec, wanted, out, ws, st);
-}

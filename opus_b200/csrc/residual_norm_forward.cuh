@@ -1,0 +1,185 @@
+// Residual norm, forward: kernels and their launch, for one pair of types (included by residual_norm_<types>.cu).
+//
+//   z = y or N(y) w_post + b_post;  h = r x + g z;  n = N(h) w + b
+//
+// N(v) = v / sqrt(mean v^2 + eps), or (v - mean) / sqrt(var + eps) with the
+// variance summed about the mean (two sums over the registers, so no
+// cancellation).  n is the norm of the h that is stored: what the next block
+// sees is the norm of the residual stream as the backward will read it.
+//
+// Bound: HBM bandwidth; x and y are read once, h and n written once, nothing
+// else but 16 bytes of statistics a row.
+#pragma once
+
+#include "residual_norm.cuh"
+
+namespace opus {
+namespace {
+
+enum Form : int { kAlone, kJoin, kFull };  // no y; y; y with a norm or a gate
+
+template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
+__global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull || V < 8 ? 2 : 3)
+    residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
+  extern __shared__ __align__(16) float shared[];
+  const int t = threadIdx.x % s.group;
+  const int g = threadIdx.x / s.group;
+  const RowRun run(s.rows, static_cast<int64_t>(blockIdx.x) * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
+  const Columns<V, NV> c(s, t);
+  const TX* x = static_cast<const TX*>(a.x) + run.first * a.x_stride;
+  const TY* y = static_cast<const TY*>(a.y) + (F != kAlone ? run.first * a.y_stride : 0);
+  TX* hp = static_cast<TX*>(a.h) + run.first * s.d;
+  TY* np = static_cast<TY*>(a.n) + run.first * s.d;
+  RawRow<TX, V, NV> xr;
+  RawRow<TY, V, NV> yr;
+  xr.zero();
+  yr.zero();
+  if (run.first < run.last) {
+    xr.load(x, c);
+    if constexpr (F != kAlone) yr.load(y, c);
+  }
+  GroupSum<norm_sub_warp(V, NV)> sum(shared, s.group, s.groups);
+  float* place = shared + group_floats(s.group, s.groups);
+  Param<NV, V, Near> w(a.weight, a.weight_dtype, 1.f), b(a.bias, a.bias_dtype, 0.f);
+  Param<NV, V, Near> pw(a.post_weight, a.post_weight_dtype, 1.f), pb(a.post_bias, a.post_bias_dtype, 0.f);
+  Param<NV, V, Near> q(a.gate, a.gate_dtype, 1.f);
+  w.fill(&place, s);
+  b.fill(&place, s);
+  const bool one_gate = s.seq == s.rows;
+  if constexpr (F == kFull) {
+    pw.fill(&place, s);
+    pb.fill(&place, s);
+    if (one_gate) q.fill(&place, s);
+  }
+  __syncthreads();
+  int64_t until = 0, gate_at = 0;  // the first row of the next sample, this sample's gate
+  for (int64_t row = run.first; row < run.last; ++row) {
+    float h[NV][V], u[NV][V];
+    xr.get(h);
+    if constexpr (F != kAlone) yr.get(u);
+    x += a.x_stride;
+    if constexpr (F != kAlone) y += a.y_stride;
+    if (row + 1 < run.last) {
+      xr.load(x, c);
+      if constexpr (F != kAlone) yr.load(y, c);
+    }
+    float2 ys = make_float2(0.f, 1.f);
+    if constexpr (F == kFull) {
+      float p[NV][V];
+      if (a.post) {
+        ys = row_stats(u, s, c, t, sum);
+        float o[NV][V];
+        pw.row(c, p);
+        pb.row(c, o);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) u[k][j] = fmaf((u[k][j] - ys.x) * ys.y, p[k][j], o[k][j]);
+      }
+      if (one_gate) {
+        q.row(c, p);
+      } else {
+        if (row >= until) {
+          gate_at = row / s.seq * s.d;
+          until = (row / s.seq + 1) * s.seq;
+        }
+        load_param_row(a.gate, a.gate_dtype, gate_at, 1.f, c, p);
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[k][j] *= p[k][j];
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[k][j] = F == kAlone ? a.residual_scale * h[k][j] : fmaf(a.residual_scale, h[k][j], u[k][j]);
+      Vec<TX, V> stored;
+      stored.set(h[k]);
+      stored.get(h[k]);  // what is normed is what is stored
+      if (c.own[k] && (F != kAlone || a.h != nullptr)) *reinterpret_cast<Vec<TX, V>*>(hp + c.at[k]) = stored;
+    }
+    hp += s.d;
+    const float2 hs = row_stats(h, s, c, t, sum);
+    float o[NV][V];
+    w.row(c, u);
+    b.row(c, o);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[k][j] = fmaf((h[k][j] - hs.x) * hs.y, u[k][j], o[k][j]);
+    store_row(np, c, h);
+    np += s.d;
+    if (t == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
+  }
+}
+
+template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
+int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t st) {
+  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Near, Wide>;
+  const int threads = s.group * s.groups;
+  const int arrays = F != kFull ? 2 : s.seq == s.rows ? 5 : 4;
+  const int shared = (group_floats(s.group, s.groups) + arrays * Param<NV, V, Near>::size(s.group)) * static_cast<int>(sizeof(float));
+  const int rc = allow_shared<kernel>(shared);
+  if (rc) return rc;
+  const int64_t need = (s.rows + s.groups - 1) / s.groups;
+  const int64_t most = static_cast<int64_t>(sm_count()) * resident_blocks<kernel>(threads, shared);
+  s.blocks = static_cast<int>(need < most ? need : most);
+  kernel<<<s.blocks, threads, shared, st>>>(s, a);
+  note_launch();
+  OPUS_CUDA_TRY(cudaGetLastError());
+  return OPUS_OK;
+}
+
+template <typename TX, typename TY, int V, int NV, int F>
+int forward_wide(const opus_residual_norm_args& a, cudaStream_t st) {
+  NormShape s;
+  int nv;
+  const int rc = norm_shape("residual_norm", &a, V, NV, &s, &nv);
+  if (rc) return rc;
+  if constexpr (F == kFull) {
+    if (5 * Param<NV, V, true>::size(s.group) * static_cast<int>(sizeof(float)) > kNormSharedParams)
+      return launch_forward<TX, TY, V, NV, F, false, true>(s, a, st);
+  }
+  return launch_forward<TX, TY, V, NV, F, true, true>(s, a, st);
+}
+
+template <typename TX, typename TY, int V, int F>
+int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
+  NormShape s;
+  int nv;
+  constexpr bool kBoth = F == kFull;
+  if (a.d > norm_narrow(V, kBoth)) {
+    if constexpr (V == 1) {
+      if (a.d <= kNormScalarMiddle) return forward_wide<TX, TY, V, 8, F>(a, st);
+      return forward_wide<TX, TY, V, 16, F>(a, st);
+    } else {
+      return forward_wide<TX, TY, V, 32 / V, F>(a, st);
+    }
+  }
+  constexpr int kMost = narrow_vectors(V, kBoth), kFewer = fewer_vectors(V, kBoth);
+  const int rc = norm_shape("residual_norm", &a, V, kMost, &s, &nv);
+  if (rc) return rc;
+  if constexpr (V > 1) {
+    if (nv == 1) return launch_forward<TX, TY, V, 1, F, true, false>(s, a, st);
+  }
+  if constexpr (V < 8) {
+    if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, true, false>(s, a, st);
+  }
+  return launch_forward<TX, TY, V, kMost, F, true, false>(s, a, st);
+}
+
+template <typename TX, typename TY, int V>
+int forward_by_form(const opus_residual_norm_args& a, cudaStream_t st) {
+  if (a.post || a.gate != nullptr) return forward_by_width<TX, TY, V, kFull>(a, st);
+  if (a.y != nullptr) return forward_by_width<TX, TY, V, kJoin>(a, st);
+  return forward_by_width<TX, TY, V, kAlone>(a, st);
+}
+
+template <typename TX, typename TY>
+int forward_by_alignment(const opus_residual_norm_args& a, bool vec, cudaStream_t st) {
+  return vec ? forward_by_form<TX, TY, 16 / sizeof(TX)>(a, st) : forward_by_form<TX, TY, 1>(a, st);
+}
+
+}  // namespace
+}  // namespace opus
