@@ -109,6 +109,119 @@ __device__ __forceinline__ void store_vec(T* p, const float (&r)[V]) {
   *reinterpret_cast<Vec<T, V>*>(p) = x;
 }
 
+// Arithmetic on vectors of f32; Pairs: two elements to an instruction, for kernels that are bound by the instructions
+// they issue and have registers to spare (pairs lie in neighbouring ones).  The roundings are those of one by one.
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+// (a, b) = (a x0 + y0, b x1 + y1)
+__device__ __forceinline__ void fma2(float& a, float& b, float x0, float x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
+}
+// (a, b) += (x0 y0, x1 y1)
+__device__ __forceinline__ void mac2(float& a, float& b, float x0, float x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
+}
+// r += s, r *= s, r += a, r *= a, r = r a + b, r = r s + b, r += a b, elementwise
+template <bool Pairs, int V>
+__device__ __forceinline__ void vadd(float (&r)[V], float s) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] += s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) add2(r[i], r[i + 1], s, s);
+  }
+}
+template <bool Pairs, int V>
+__device__ __forceinline__ void vmul(float (&r)[V], float s) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] *= s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) mul2(r[i], r[i + 1], s, s);
+  }
+}
+template <bool Pairs, int V>
+__device__ __forceinline__ void vadd(float (&r)[V], const float (&a)[V]) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] += a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) add2(r[i], r[i + 1], a[i], a[i + 1]);
+  }
+}
+template <bool Pairs, int V>
+__device__ __forceinline__ void vmul(float (&r)[V], const float (&a)[V]) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] *= a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) mul2(r[i], r[i + 1], a[i], a[i + 1]);
+  }
+}
+template <bool Pairs, int V>
+__device__ __forceinline__ void vfma(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = fmaf(r[i], a[i], b[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) fma2(r[i], r[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+  }
+}
+template <bool Pairs, int V>
+__device__ __forceinline__ void vfma(float (&r)[V], float s, const float (&b)[V]) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = fmaf(r[i], s, b[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) fma2(r[i], r[i + 1], s, s, b[i], b[i + 1]);
+  }
+}
+template <bool Pairs, int V>
+__device__ __forceinline__ void vmac(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = fmaf(a[i], b[i], r[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) mac2(r[i], r[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+  }
+}
+// (s0, s1) += the vector's elements (products) in two chains
+template <bool Pairs, int V>
+__device__ __forceinline__ void vsum(float (&s)[2], const float (&a)[V]) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i & 1] += a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) add2(s[0], s[1], a[i], a[i + 1]);
+  }
+}
+template <bool Pairs, int V>
+__device__ __forceinline__ void vdot(float (&s)[2], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (!Pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i & 1] = fmaf(a[i], b[i], s[i & 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) mac2(s[0], s[1], a[i], a[i + 1], b[i], b[i + 1]);
+  }
+}
+
 // One element of an array whose type is known at run time (parameters: read once per block or row).
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   if (dtype == OPUS_DTYPE_F32) return static_cast<const float*>(p)[i];

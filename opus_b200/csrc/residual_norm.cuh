@@ -21,16 +21,18 @@ namespace opus {
 constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxWidth = 16384;
 
-// Narrow rows (up to 4096 elements) take up to 16 elements a thread and 256 threads, wider ones 32 elements and 512
-// threads.  Vectors of one element need more registers each (an address, a predicate): with a norm of y or a gate
-// narrow rows end at 2048 and take 8 elements a thread, and wide ones take 1024 threads with 8 elements up to 8192 and
-// 16 beyond.  Registers that spill cost more than anything else here: 50000 x 771 f32 with both norms took 335 us
-// forward with 16 elements a thread and 820 bytes spilled, 157 us with 8; without them 128 us with 8, 107 with 16.
+// Narrow rows (up to 4096 elements) take up to 16 elements a thread and 256 threads; wider ones 512 threads, with 16
+// elements up to 8192 and 32 beyond.  Vectors of one element need more registers each (an address, a predicate): with
+// a norm of y or a gate narrow rows end at 2048 and take 8 elements a thread, and wide ones take 1024 threads with 8
+// elements up to 8192 and 16 beyond.  Registers that spill cost more than anything else here: 50000 x 771 f32 with
+// both norms took 335 us forward with 16 elements a thread and 820 bytes spilled, 155 us with 8; without them 128 us
+// with 8, 107 with 16.
 constexpr int narrow_vectors(int V, bool full) { return V == 1 && full ? 8 : 16 / V; }
 constexpr int norm_narrow(int V, bool full) { return 256 * narrow_vectors(V, full) * V; }
+constexpr int middle_vectors(int V) { return V == 1 ? 8 : 16 / V; }
 // the smaller choice for shorter rows (vectors of 8: one vector)
 constexpr int fewer_vectors(int V, bool full) { return V == 1 ? 4 : narrow_vectors(V, full) / 2; }
-constexpr int kNormScalarMiddle = 8192;
+constexpr int kNormMiddle = 8192;  // wide rows up to here take half the elements a thread of wider ones
 constexpr int norm_threads(int V, bool wide) { return !wide ? 256 : V == 1 ? 1024 : 512; }
 
 struct NormShape {
@@ -150,29 +152,46 @@ __device__ __forceinline__ void store_row(T* row, const Columns<V, NV>& c, const
 }
 
 // mean (0 for an RMS norm) and 1 / sqrt(mean square about it + eps) of a row (zeros beyond it)
-template <int V, int NV, typename Sum>
+template <bool Pairs, int V, int NV, typename Sum>
 __device__ __forceinline__ float2 row_stats(const float (&r)[NV][V], const NormShape& s, const Columns<V, NV>& c, int t, Sum& sum) {
   const float inv_d = 1.0f / static_cast<float>(s.d);
   float mean = 0.f;
+  float q[2] = {0.f, 0.f};  // two chains
   if (s.layer) {
-    float a[1] = {0.f};
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) a[0] += r[k][i];
+    for (int k = 0; k < NV; ++k) vsum<Pairs>(q, r[k]);
+    float a[1] = {q[0] + q[1]};
     sum(a, t);
     mean = a[0] * inv_d;
+    q[0] = q[1] = 0.f;
   }
-  float q[2] = {0.f, 0.f};  // two chains
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const float m = c.own[k] ? mean : 0.f;
+    if constexpr (Pairs) {
+      float v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) q[i & 1] = fmaf(r[k][i] - m, r[k][i] - m, q[i & 1]);
+      for (int i = 0; i < V; ++i) v[i] = r[k][i];
+      vadd<true>(v, -m);
+      vdot<true>(q, v, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) q[i & 1] = fmaf(r[k][i] - m, r[k][i] - m, q[i & 1]);
+    }
   }
   float whole[1] = {q[0] + q[1]};
   sum(whole, t);
   return make_float2(mean, rsqrtf(whole[0] * inv_d + s.eps));
+}
+
+// r = (r - mean) / sd of a row with those statistics (an RMS norm's mean is 0)
+template <bool Pairs, int V, int NV>
+__device__ __forceinline__ void normalize(float (&r)[NV][V], float mean, float rstd) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    vadd<Pairs>(r[k], -mean);
+    vmul<Pairs>(r[k], rstd);
+  }
 }
 
 // V neighbours of an array whose type is known at run time, in accesses of up to 16 bytes (V > 1: aligned arrays).

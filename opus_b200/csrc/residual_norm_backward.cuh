@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(norm_threads(V, false))
     grad_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a, int wanted,
                 float* __restrict__ parts, float* __restrict__ gates) {
   extern __shared__ __align__(16) float shared[];
+  constexpr bool kPairs = V == 8;
   const int t = threadIdx.x % s.group;
   const int g = threadIdx.x / s.group;
   const int64_t worker = static_cast<int64_t>(blockIdx.x) * s.groups + g;
@@ -101,30 +102,31 @@ __global__ void __launch_bounds__(norm_threads(V, false))
     if constexpr (Full) yr.get(y);
     const float4 st = ahead;
     if (row + 1 < run.last) fetch();
-    float m[2] = {0.f, 0.f};
+    float m[2], m0[2] = {0.f, 0.f}, m1[2] = {0.f, 0.f};
     w.row(c, f);
+    normalize<kPairs>(hat, st.x, st.y);
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        hat[k][j] = (hat[k][j] - st.x) * st.y;
-        acc_w[k][j] = fmaf(u[k][j], hat[k][j], acc_w[k][j]);
-        if constexpr (Bias) acc_b[k][j] += u[k][j];
-        u[k][j] *= f[k][j];
-        m[0] += u[k][j];
-        m[1] = fmaf(u[k][j], hat[k][j], m[1]);
-      }
+    for (int k = 0; k < NV; ++k) {
+      vmac<kPairs>(acc_w[k], u[k], hat[k]);
+      if constexpr (Bias) vadd<kPairs>(acc_b[k], u[k]);
+      vmul<kPairs>(u[k], f[k]);
+      if (s.layer) vsum<kPairs>(m0, u[k]);
+      vdot<kPairs>(m1, u[k], hat[k]);
+    }
+    m[0] = m0[0] + m0[1];
+    m[1] = m1[0] + m1[1];
     sum(m, t);
-    m[0] = s.layer ? m[0] * inv_d : 0.f;
-    m[1] *= inv_d;
     // dh in u
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      vmul<kPairs>(hat[k], -m[1] * inv_d);
+      vadd<kPairs>(u[k], hat[k]);
+      if (s.layer) vadd<kPairs>(u[k], -m[0] * inv_d);
+      vfma<kPairs>(u[k], st.y, r[k]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        u[k][j] = fmaf(st.y, u[k][j] - m[0] - hat[k][j] * m[1], r[k][j]);
-        r[k][j] = a.residual_scale * u[k][j];
-      }
+      for (int j = 0; j < V; ++j) r[k][j] = u[k][j];
+      vmul<kPairs>(r[k], a.residual_scale);
+    }
     store_row(dx, c, r);
     dx += s.d;
     if constexpr (Full) {
@@ -140,36 +142,40 @@ __global__ void __launch_bounds__(norm_threads(V, false))
       }
       if (!a.post) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            acc_g[k][j] = fmaf(u[k][j], y[k][j], acc_g[k][j]);
-            u[k][j] *= r[k][j];
-          }
+        for (int k = 0; k < NV; ++k) {
+          vmac<kPairs>(acc_g[k], u[k], y[k]);
+          vmul<kPairs>(u[k], r[k]);
+        }
       } else {
         pw.row(c, f);
         if constexpr (Bias) pb.row(c, hat);
-        float p[2] = {0.f, 0.f};
+        normalize<kPairs>(y, st.z, st.w);
+        float p[2], p0[2] = {0.f, 0.f}, p1[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+          float z[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            y[k][j] = (y[k][j] - st.z) * st.w;  // normed y
-            acc_g[k][j] = fmaf(u[k][j], Bias ? fmaf(y[k][j], f[k][j], hat[k][j]) : y[k][j] * f[k][j], acc_g[k][j]);
-            const float dz = u[k][j] * r[k][j];
-            acc_pw[k][j] = fmaf(dz, y[k][j], acc_pw[k][j]);
-            if constexpr (Bias) acc_pb[k][j] += dz;
-            u[k][j] = dz * f[k][j];
-            p[0] += u[k][j];
-            p[1] = fmaf(u[k][j], y[k][j], p[1]);
-          }
+          for (int j = 0; j < V; ++j) z[j] = y[k][j];
+          if constexpr (Bias) vfma<kPairs>(z, f[k], hat[k]);
+          else vmul<kPairs>(z, f[k]);
+          vmac<kPairs>(acc_g[k], u[k], z);
+          vmul<kPairs>(u[k], r[k]);  // dz
+          vmac<kPairs>(acc_pw[k], u[k], y[k]);
+          if constexpr (Bias) vadd<kPairs>(acc_pb[k], u[k]);
+          vmul<kPairs>(u[k], f[k]);
+          if (s.layer) vsum<kPairs>(p0, u[k]);
+          vdot<kPairs>(p1, u[k], y[k]);
+        }
+        p[0] = p0[0] + p0[1];
+        p[1] = p1[0] + p1[1];
         sum(p, t);
-        p[0] = s.layer ? p[0] * inv_d : 0.f;
-        p[1] *= inv_d;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) u[k][j] = st.w * (u[k][j] - p[0] - y[k][j] * p[1]);
+        for (int k = 0; k < NV; ++k) {
+          vmul<kPairs>(y[k], -p[1] * inv_d);
+          vadd<kPairs>(u[k], y[k]);
+          if (s.layer) vadd<kPairs>(u[k], -p[0] * inv_d);
+          vmul<kPairs>(u[k], st.w);
+        }
       }
     }
     if (a.grad_y != nullptr) store_row(dy, c, u);
@@ -555,12 +561,8 @@ template <typename TX, typename TY, int V>
 int backward_by_form(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
   const bool full = a.post || a.gate != nullptr;
   if (a.d > norm_narrow(V, full)) {
-    if constexpr (V == 1) {
-      if (a.d <= kNormScalarMiddle) return backward_wide<TX, TY, V, 8>(a, wanted, out, ws, st);
-      return backward_wide<TX, TY, V, 16>(a, wanted, out, ws, st);
-    } else {
-      return backward_wide<TX, TY, V, 32 / V>(a, wanted, out, ws, st);
-    }
+    return a.d <= kNormMiddle ? backward_wide<TX, TY, V, middle_vectors(V)>(a, wanted, out, ws, st)
+                              : backward_wide<TX, TY, V, 2 * middle_vectors(V)>(a, wanted, out, ws, st);
   }
   const bool bias = a.post_bias != nullptr || (wanted & (1 << kBias)) != 0;
   if (full)

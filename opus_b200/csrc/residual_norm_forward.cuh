@@ -22,6 +22,7 @@ template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
 __global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull || V < 8 ? 2 : 3)
     residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
   extern __shared__ __align__(16) float shared[];
+  constexpr bool kPairs = V == 8 && F == kFull;
   const int t = threadIdx.x % s.group;
   const int g = threadIdx.x / s.group;
   const RowRun run(s.rows, static_cast<int64_t>(blockIdx.x) * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
@@ -67,14 +68,13 @@ __global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull |
     if constexpr (F == kFull) {
       float p[NV][V];
       if (a.post) {
-        ys = row_stats(u, s, c, t, sum);
+        ys = row_stats<kPairs>(u, s, c, t, sum);
         float o[NV][V];
         pw.row(c, p);
         pb.row(c, o);
+        normalize<kPairs>(u, ys.x, ys.y);
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) u[k][j] = fmaf((u[k][j] - ys.x) * ys.y, p[k][j], o[k][j]);
+        for (int k = 0; k < NV; ++k) vfma<kPairs>(u[k], p[k], o[k]);
       }
       if (one_gate) {
         q.row(c, p);
@@ -86,28 +86,25 @@ __global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull |
         load_param_row(a.gate, a.gate_dtype, gate_at, 1.f, c, p);
       }
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) u[k][j] *= p[k][j];
+      for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) h[k][j] = F == kAlone ? a.residual_scale * h[k][j] : fmaf(a.residual_scale, h[k][j], u[k][j]);
+      if constexpr (F == kAlone) vmul<kPairs>(h[k], a.residual_scale);
+      else vfma<kPairs>(h[k], a.residual_scale, u[k]);
       Vec<TX, V> stored;
       stored.set(h[k]);
       stored.get(h[k]);  // what is normed is what is stored
       if (c.own[k] && (F != kAlone || a.h != nullptr)) *reinterpret_cast<Vec<TX, V>*>(hp + c.at[k]) = stored;
     }
     hp += s.d;
-    const float2 hs = row_stats(h, s, c, t, sum);
+    const float2 hs = row_stats<kPairs>(h, s, c, t, sum);
     float o[NV][V];
     w.row(c, u);
     b.row(c, o);
+    normalize<kPairs>(h, hs.x, hs.y);
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) h[k][j] = fmaf((h[k][j] - hs.x) * hs.y, u[k][j], o[k][j]);
+    for (int k = 0; k < NV; ++k) vfma<kPairs>(h[k], u[k], o[k]);
     store_row(np, c, h);
     np += s.d;
     if (t == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
@@ -150,12 +147,8 @@ int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   int nv;
   constexpr bool kBoth = F == kFull;
   if (a.d > norm_narrow(V, kBoth)) {
-    if constexpr (V == 1) {
-      if (a.d <= kNormScalarMiddle) return forward_wide<TX, TY, V, 8, F>(a, st);
-      return forward_wide<TX, TY, V, 16, F>(a, st);
-    } else {
-      return forward_wide<TX, TY, V, 32 / V, F>(a, st);
-    }
+    return a.d <= kNormMiddle ? forward_wide<TX, TY, V, middle_vectors(V), F>(a, st)
+                              : forward_wide<TX, TY, V, 2 * middle_vectors(V), F>(a, st);
   }
   constexpr int kMost = narrow_vectors(V, kBoth), kFewer = fewer_vectors(V, kBoth);
   const int rc = norm_shape("residual_norm", &a, V, kMost, &s, &nv);
