@@ -20,8 +20,15 @@
 // recorded in the device error word.  Tokens equal to padding_idx add to no
 // gradient.
 //
-// Bound: HBM bandwidth; dY is read once (whole rows, in sorted order) and dW
-// written once.
+// Bound: HBM bandwidth.  The lookup is a stream of writes: 147456 rows of 1600
+// bf16 elements in 96 to 105 us, 4.5 to 4.9 TB/s written (a memset on the same
+// device writes 3.9, a copy moves 6.5).  The gradient reads dY once, whole rows in sorted
+// order, and writes dW, the named rows twice (zeros, then sums: the zeroing
+// hides behind the sort, which leaves HBM idle): 81920 x 768 f32 tokens of a
+// 50257-row table in 102 us (a profile gives 35 to sort and zero, 50 to sum and
+// 16 to join); 16384 x 2048 bf16 of a 151936-row table in 121 to 137 us, where a
+// memset of dW alone takes 160.  Short lists are bound by the chain of three
+// launches: 23 us for 300 tokens.
 #include "elements.cuh"
 
 namespace opus {
@@ -111,8 +118,7 @@ __device__ __forceinline__ uint2 load_item(const KeySource& s, int64_t i, int* e
   return item;
 }
 
-// The lanes whose digit is this lane's, among those in `live` (match_any takes many more cycles where a warp's
-// digits differ).
+// The lanes whose digit is this lane's, among those in `live`, by a ballot for each bit.
 __device__ __forceinline__ unsigned same_digit(uint32_t digit, int bits, unsigned live) {
   unsigned same = live;
 #pragma unroll
@@ -239,7 +245,9 @@ constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kMostBlocks = 16;
 constexpr int kMostItems = 11776;  // of a block: four arrays of them and the counts fit its shared memory
 constexpr int kItemRounds = (kMostItems + kClusterThreads - 1) / kClusterThreads;
-constexpr int kBlockItems = 2048;  // of a block, while there are blocks to share them
+constexpr int kBlockItems = 2048;  // of a block, while there are blocks to share them: 10 to 12 us for one block
+                                   // (zeros of a 51 MB table with it), 14 for 16384 on eight, 24 for 81920 and 36 for
+                                   // 147456 on sixteen
 
 struct ClusterSort {
   const void* tokens;

@@ -16,6 +16,11 @@
 // join.  Every sum has a fixed order.
 //
 // Bound: HBM bandwidth (h, dn, dh_in and y read once, dx and dy written once).
+// 65536 x 2048 bf16: RMS joints 210 us, 6.4 TB/s; layer norms with biases 267 us,
+// 5.0 TB/s (161 registers: one block an SM); both norms and a gate 369 us, 4.4
+// TB/s (241 registers: eight warps an SM, a third of the issue slots).  8 elements
+// a thread would leave room for twice the warps and took 535 us.  32768 x 2048 f32:
+// 213 us, 6.3 TB/s.  Wide rows are read twice: 8192 x 8192 f32 356 us, 3.8 TB/s.
 #pragma once
 
 #include "residual_norm.cuh"

@@ -8,7 +8,11 @@
 // sees is the norm of the residual stream as the backward will read it.
 //
 // Bound: HBM bandwidth; x and y are read once, h and n written once, nothing
-// else but 16 bytes of statistics a row.
+// else but 16 bytes of statistics a row.  65536 x 2048 bf16: 185 us, 5.8 TB/s;
+// 32768 x 2048 f32 185 us, 5.8 TB/s.  With norms on both sides and a gate 16-bit
+// rows are bound by the instructions they issue (26 an element, 49% of the
+// issue slots at the 16 warps that their registers leave): 213 us, 5.0 TB/s; f32
+// ones are not: 175 us, 6.1 TB/s.
 #pragma once
 
 #include "residual_norm.cuh"
