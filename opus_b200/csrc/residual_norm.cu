@@ -39,28 +39,39 @@ bool norm_params_aligned(const opus_residual_norm_args* a) {
 }
 
 // The launch's shape for vectors of V elements, at most `most` of them (a power of two) a thread: as few threads
-// a row as that allows, and as few vectors a thread as those threads need.
-int norm_shape(const char* what, const opus_residual_norm_args* a, int V, int most, NormShape* s, int* nv) {
+// a row as that allows.  Returns how many vectors a thread (a power of two) those threads need.
+int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s) {
   const int full = (a->d + V - 1) / V;
   int group = 1;
   while (group < 32 && group * most < full) group <<= 1;
   if (group * most < full) group = ((full + most - 1) / most + 31) / 32 * 32;
   // rows of less than a warp: a vector for each lane, so that its loads are neighbours
   while (group < 32 && group < full) group <<= 1;
-  if (group > kNormMaxThreads) return set_error(OPUS_ERR_UNSUPPORTED, "%s: d = %d is too wide", what, a->d);
   int k = 1;
   while (k * group < full) k <<= 1;
-  *nv = k;
   s->rows = a->rows;
   s->seq = a->gate != nullptr && a->gate_rows > 1 ? a->rows / a->gate_rows : a->rows;
   if (s->seq < 1) s->seq = 1;
   s->d = a->d;
   s->group = group;
-  s->groups = group >= 256 ? 1 : 256 / group;
+  s->groups = group >= kNormThreads ? 1 : kNormThreads / group;
+  s->ranks = 1;
   s->layer = a->kind;
   s->eps = a->eps;
   s->blocks = 0;
-  return OPUS_OK;
+  return k;
+}
+
+// Of rows wider than a block of NV vectors a thread: a cluster of as few blocks (2, 4 or 8) as hold a row, and as few
+// threads in each as share it evenly (more than 64, since half as many full blocks would not have held it).
+void norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape* s) {
+  norm_shape(a, V, NV, s);
+  const int full = (a->d + V - 1) / V;
+  int ranks = 2;
+  while (ranks * kNormThreads * NV < full) ranks *= 2;
+  s->group = ((full + ranks * NV - 1) / (ranks * NV) + 31) / 32 * 32;
+  s->groups = 1;
+  s->ranks = ranks;
 }
 
 namespace {
@@ -100,14 +111,7 @@ extern "C" int opus_residual_norm(const opus_residual_norm_args* args, void* str
 extern "C" int64_t opus_residual_norm_grad_workspace_bytes(const opus_residual_norm_args* a) {
   if (a == nullptr || a->rows <= 0 || a->d < 1) return 256;
   const int64_t samples = a->gate != nullptr && a->gate_rows > 1 && a->rows % a->gate_rows == 0 ? a->gate_rows : 0;
-  const Runs whole = runs_of(a->rows, a->rows);
-  int64_t runs = whole.samples * whole.per_seq;
-  if (samples > 0) {
-    const Runs r = runs_of(a->rows, a->rows / samples);
-    if (r.samples * r.per_seq > runs) runs = r.samples * r.per_seq;
-  }
-  const int64_t wide = align256(a->rows * 8) + align256(runs * kColumns * a->d * 4);
-  // the one-pass kernel: a block holds at most 256 rows, and no more blocks run than there are rows
+  // a block holds at most 256 rows, and no more blocks run than there are rows
   int64_t blocks = static_cast<int64_t>(sm_count()) * kGradBlocksPerSm;
   blocks = blocks < a->rows ? blocks : a->rows;
   int64_t workers = 0;
@@ -115,8 +119,7 @@ extern "C" int64_t opus_residual_norm_grad_workspace_bytes(const opus_residual_n
     workers = blocks * (a->d > 2048 ? 1 : a->d > 256 ? 8 : 256);
     workers = (workers < a->rows + 256 ? workers : a->rows + 256) + samples;
   }
-  const int64_t one_pass = align256((blocks * kColumns + workers) * a->d * 4);
-  return wide > one_pass ? wide : one_pass;
+  return align256((blocks * kColumns + workers) * a->d * 4);
 }
 
 extern "C" int opus_residual_norm_grad(const opus_residual_norm_args* args, void* workspace, int64_t workspace_bytes,

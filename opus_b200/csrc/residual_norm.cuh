@@ -18,31 +18,28 @@
 
 namespace opus {
 
-constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxWidth = 16384;
 
-// Narrow rows (up to 4096 elements) take up to 16 elements a thread and 256 threads; wider ones 512 threads, with 16
-// elements up to 8192 and 32 beyond.  Vectors of one element need more registers each (an address, a predicate): with
-// a norm of y or a gate narrow rows end at 2048 and take 8 elements a thread, and wide ones take 1024 threads with 8
-// elements up to 8192 and 16 beyond.  Registers that spill cost more than anything else here: 50000 x 771 f32 with
-// both norms took 335 us forward with 16 elements a thread and 820 bytes spilled, 155 us with 8; without them 128 us
-// with 8, 107 with 16.
+// A block is 256 threads at most, with up to 16 elements a thread.  Vectors of one element need more registers each
+// (an address, a predicate): with a norm of y or a gate they are 8 at most.  Registers that spill cost more than
+// anything else here: 50000 x 771 f32 with both norms took 335 us forward with 16 elements a thread and 820 bytes
+// spilled, 155 us with 8; without them 128 us with 8, 107 with 16.  Rows wider than a block are split among the
+// blocks of a cluster, which have the same registers each and share the row's sums.
+constexpr int kNormThreads = 256;
 constexpr int narrow_vectors(int V, bool full) { return V == 1 && full ? 8 : 16 / V; }
-constexpr int norm_narrow(int V, bool full) { return 256 * narrow_vectors(V, full) * V; }
-constexpr int middle_vectors(int V) { return V == 1 ? 8 : 16 / V; }
+constexpr int norm_narrow(int V, bool full) { return kNormThreads * narrow_vectors(V, full) * V; }
 // the smaller choice for shorter rows (vectors of 8: one vector)
 constexpr int fewer_vectors(int V, bool full) { return V == 1 ? 4 : narrow_vectors(V, full) / 2; }
-constexpr int kNormMiddle = 8192;  // wide rows up to here take half the elements a thread of wider ones
-constexpr int norm_threads(int V, bool wide) { return !wide ? 256 : V == 1 ? 1024 : 512; }
 
 struct NormShape {
   int64_t rows;
   int64_t seq;  // rows that share a row of the gate (rows of a sample); `rows` for one gate
   int d;
-  int group, groups;  // threads of a row, rows of a block
+  int group, groups;  // threads of a row in a block, rows of a block
+  int ranks;          // blocks of a row: 1, or a cluster's (with groups = 1)
   int layer;          // LayerNorm (1) or RMS norm (0)
   float eps;
-  int blocks;  // of the launch
+  int blocks;  // of the launch, or clusters of them
 };
 
 // The rows [first, last) of worker w among n.
@@ -55,32 +52,40 @@ struct RowRun {
   }
 };
 
-// Shared memory of a group's sums: slots of its warps (a multiple of 4), twice for two values, twice for two turns.
+// Shared memory of a group's sums: slots of its warps (a multiple of 4; of every block of the row), twice for two
+// values, twice for two turns.
 __host__ __device__ constexpr int group_slots(int group) { return group <= 32 ? 0 : ((group >> 5) + 3) / 4 * 4; }
-__host__ __device__ constexpr int group_floats(int group, int groups) { return 4 * groups * group_slots(group); }
+__host__ __device__ constexpr int group_floats(int group, int groups, int ranks) {
+  return 4 * groups * ranks * group_slots(group);
+}
 
 // Whether a thread's group may be less than a warp (norm_shape's smallest vector counts).
 constexpr bool norm_sub_warp(int V, int NV) { return NV == 1 || (V == 1 && NV == 4); }
 
 // Sums over the group of up to two values each, in a fixed order; the result is in every thread of the group.
-// A call takes one barrier of the group's own: `turn` alternates between two buffers.
-template <bool SubWarp>
+// A call takes one barrier of the group's own, or of the cluster, whose blocks write their warps' sums to each
+// other: `turn` alternates between two buffers, so that one is written while the other may still be read.
+template <bool SubWarp, bool Cluster>
 struct GroupSum {
   float* buf;
   int slots, span, barrier, threads;
   unsigned lanes;
   int turn;
+  int ranks, rank;
 
   // every thread of the block calls it once
-  __device__ GroupSum(float* shared, int group, int groups) : threads(group), lanes(0xffffffffu), turn(0) {
-    slots = group_slots(group);  // of the group's warps, zeros behind them
-    span = groups * slots;
-    const int g = static_cast<int>(threadIdx.x) / group;
+  __device__ GroupSum(float* shared, const NormShape& s, int rank_)
+      : threads(s.group), lanes(0xffffffffu), turn(0), ranks(Cluster ? s.ranks : 1), rank(rank_) {
+    slots = group_slots(s.group) * ranks;  // of the row's warps, zeros behind each block's
+    span = s.groups * slots;
+    const int g = static_cast<int>(threadIdx.x) / s.group;
     buf = shared + g * slots;
     barrier = 1 + g;  // named barriers 1 to 15: a block has at most 4 groups of more than a warp
-    if (SubWarp && group < 32) lanes = ((1u << group) - 1) << ((threadIdx.x & 31) / group * group);
+    if (SubWarp && s.group < 32) lanes = ((1u << s.group) - 1) << ((threadIdx.x & 31) / s.group * s.group);
     for (int i = threadIdx.x; i < 4 * span; i += blockDim.x) shared[i] = 0.f;
-    __syncthreads();
+    __syncwarp();
+    if constexpr (Cluster) cluster_sync();  // before another block writes here
+    else __syncthreads();
   }
   template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N], int t) {
@@ -93,11 +98,22 @@ struct GroupSum {
     if (slots == 0) return;
     float* b = buf + turn;
     turn = 2 * span - turn;
-    if ((t & 31) == 0) {
+    if constexpr (Cluster) {
+      const int lane = t & 31;
+      if (lane < ranks) {
+        float* own = b + rank * (slots / ranks) + (t >> 5);
 #pragma unroll
-      for (int i = 0; i < N; ++i) b[i * span + (t >> 5)] = v[i];
+        for (int i = 0; i < N; ++i) store_peer(own + i * span, lane, v[i]);
+      }
+      __syncwarp();
+      cluster_sync();
+    } else {
+      if ((t & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) b[i * span + (t >> 5)] = v[i];
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float4 q = *reinterpret_cast<const float4*>(b + i * span);
@@ -109,6 +125,13 @@ struct GroupSum {
       v[i] = s;
     }
   }
+
+ private:
+  // *p = v in the shared memory of the cluster's block `peer`
+  static __device__ __forceinline__ void store_peer(float* p, int peer, float v) {
+    const uint32_t to = mapa_shared(smem_u32(p), static_cast<uint32_t>(peer));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+  }
 };
 
 // Which columns a thread holds.
@@ -116,10 +139,10 @@ template <int V, int NV>
 struct Columns {
   int at[NV];
   bool own[NV];
-  __device__ Columns(const NormShape& s, int t) {
+  __device__ Columns(const NormShape& s, int t, int base) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      at[k] = (k * s.group + t) * V;
+      at[k] = base + (k * s.group + t) * V;
       own[k] = at[k] < s.d;
     }
   }
@@ -234,57 +257,60 @@ __device__ __forceinline__ void load_param_row(const void* p, int dtype, int64_t
   else load_param_row_as<__nv_bfloat16>(p, at, c, r);
 }
 
-// A parameter of d elements that rows share.  Near: as f32 in shared memory, `other` where there is none and 0
-// beyond the row; vectors of 8 lie in two planes of 4, so that neighbouring lanes read neighbouring 16 bytes.
-// Otherwise read from where it is.
-template <int NV, int V, bool Near>
+// A parameter of d elements that rows share, as f32 in shared memory: `other` where there is none and 0 beyond the
+// row; vectors of 8 lie in two planes of 4, so that neighbouring lanes read neighbouring 16 bytes.  A block of a
+// cluster has the columns from `base`.
+template <int NV, int V>
 struct Param {
   const void* p;
-  int dtype;
+  int dtype, base;
   float other;
   float *near, *far;  // the two planes
-  __device__ __forceinline__ Param(const void* p_, int dtype_, float other_)
-      : p(p_), dtype(dtype_), other(other_), near(nullptr), far(nullptr) {}
-  static __host__ __device__ int size(int group) { return Near ? group * NV * V : 0; }
+  __device__ __forceinline__ Param(const void* p_, int dtype_, float other_, int base_)
+      : p(p_), dtype(dtype_), base(base_), other(other_), near(nullptr), far(nullptr) {}
+  static __host__ __device__ int size(int group) { return group * NV * V; }
   // by every thread; a barrier has to follow
   __device__ __forceinline__ void fill(float** shared, const NormShape& s) {
-    if constexpr (Near) {
-      near = *shared;
-      const int whole = size(s.group);
-      far = near + whole / 2;
-      *shared += whole;
-      for (int col = threadIdx.x * V; col < whole; col += blockDim.x * V) {
-        float r[V];
+    near = *shared;
+    const int whole = size(s.group);
+    far = near + whole / 2;
+    *shared += whole;
+    for (int col = threadIdx.x * V; col < whole; col += blockDim.x * V) {
+      const bool own = base + col < s.d;
+      float r[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) r[i] = col < s.d ? other : 0.f;
-        if (p != nullptr && col < s.d) load_param_vec<V>(p, dtype, col, r);
-        if constexpr (V == 8) {
-          *reinterpret_cast<float4*>(near + col / 2) = make_float4(r[0], r[1], r[2], r[3]);
-          *reinterpret_cast<float4*>(far + col / 2) = make_float4(r[4], r[5], r[6], r[7]);
-        } else {
-          store_vec<float, V>(near + col, r);
-        }
+      for (int i = 0; i < V; ++i) r[i] = own ? other : 0.f;
+      if (p != nullptr && own) load_param_vec<V>(p, dtype, base + col, r);
+      if constexpr (V == 8) {
+        *reinterpret_cast<float4*>(near + col / 2) = make_float4(r[0], r[1], r[2], r[3]);
+        *reinterpret_cast<float4*>(far + col / 2) = make_float4(r[4], r[5], r[6], r[7]);
+      } else {
+        store_vec<float, V>(near + col, r);
       }
     }
   }
   __device__ __forceinline__ void row(const Columns<V, NV>& c, float (&r)[NV][V]) const {
-    if constexpr (!Near) {
-      load_param_row(p, dtype, 0, other, c, r);
-    } else {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        if constexpr (V == 8) {
-          const float4 a = *reinterpret_cast<const float4*>(near + c.at[k] / 2);
-          const float4 b = *reinterpret_cast<const float4*>(far + c.at[k] / 2);
-          r[k][0] = a.x, r[k][1] = a.y, r[k][2] = a.z, r[k][3] = a.w;
-          r[k][4] = b.x, r[k][5] = b.y, r[k][6] = b.z, r[k][7] = b.w;
-        } else {
-          load_vec<float, V>(near + c.at[k], r[k]);
-        }
+    for (int k = 0; k < NV; ++k) {
+      const int at = c.at[k] - base;
+      if constexpr (V == 8) {
+        const float4 a = *reinterpret_cast<const float4*>(near + at / 2);
+        const float4 b = *reinterpret_cast<const float4*>(far + at / 2);
+        r[k][0] = a.x, r[k][1] = a.y, r[k][2] = a.z, r[k][3] = a.w;
+        r[k][4] = b.x, r[k][5] = b.y, r[k][6] = b.z, r[k][7] = b.w;
+      } else {
+        load_vec<float, V>(near + at, r[k]);
       }
     }
   }
 };
+
+// Sets a kernel's dynamic shared memory limit where it needs more than the default.
+template <auto Kernel>
+int allow_shared(int bytes) {
+  if (bytes > 48 * 1024) OPUS_CUDA_TRY(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return OPUS_OK;
+}
 
 // Blocks of a kernel that one multiprocessor holds.
 template <auto Kernel>
@@ -294,10 +320,47 @@ int resident_blocks(int threads, int shared_bytes) {
   return n;
 }
 
-// Shared memory that the parameters may take; above it they are read from where they are.
-constexpr int kNormSharedParams = 160 * 1024;
+// A launch of s.blocks rows' blocks or clusters: as many as the device holds at once and the rows can use, at most
+// `cap` blocks a multiprocessor.
+struct NormLaunch {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute cluster[1];
+  int shared;
 
-int norm_shape(const char* what, const opus_residual_norm_args* a, int V, int most, NormShape* s, int* nv);
+  template <auto Kernel>
+  int plan(NormShape* s, int shared_floats, int cap, cudaStream_t st) {
+    const int threads = s->group * s->groups;
+    shared = shared_floats * static_cast<int>(sizeof(float));
+    const int rc = allow_shared<Kernel>(shared);
+    if (rc) return rc;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(shared);
+    cfg.stream = st;
+    int64_t most;
+    if (s->ranks == 1) {
+      const int held = resident_blocks<Kernel>(threads, shared);
+      most = static_cast<int64_t>(sm_count()) * (held < cap ? held : cap);
+    } else {
+      cluster[0].id = cudaLaunchAttributeClusterDimension;
+      cluster[0].val.clusterDim.x = static_cast<unsigned>(s->ranks);
+      cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+      cfg.attrs = cluster;
+      cfg.numAttrs = 1;
+      cfg.gridDim = dim3(static_cast<unsigned>(s->ranks));
+      int held = 0;
+      if (cudaOccupancyMaxActiveClusters(&held, Kernel, &cfg) != cudaSuccess || held < 1) held = 1;
+      const int64_t bound = static_cast<int64_t>(sm_count()) * cap / s->ranks;
+      most = held < bound ? held : bound;
+    }
+    const int64_t need = (s->rows + s->groups - 1) / s->groups;
+    s->blocks = static_cast<int>(need < most ? need : most);
+    cfg.gridDim = dim3(static_cast<unsigned>(s->blocks * s->ranks));
+    return OPUS_OK;
+  }
+};
+
+int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s);
+void norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape* s);
 int check_norm(const char* what, const opus_residual_norm_args* a);
 bool norm_params_aligned(const opus_residual_norm_args* a);
 
@@ -309,26 +372,9 @@ struct ColumnOutputs {
   int dtype[kColumns];
 };
 
-constexpr int kRun = 64;  // rows of a run at least
-struct Runs {
-  int64_t seq, run;
-  int64_t samples;
-  int per_seq;
-};
-// Runs of rows that stay inside `seq` neighbours: at least kRun rows each, and about a thousand in all.
-inline Runs runs_of(int64_t rows, int64_t seq) {
-  Runs r;
-  r.seq = seq;
-  r.samples = seq > 0 ? rows / seq : 0;
-  int64_t run = (rows + 1023) / 1024;
-  r.run = run > kRun ? run : kRun;
-  r.per_seq = static_cast<int>((seq + r.run - 1) / r.run);
-  return r;
-}
-
 inline int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
-constexpr int kGradBlocksPerSm = 4;  // of the one-pass kernel at most: bounds the workspace
+constexpr int kGradBlocksPerSm = 4;  // of the backward at most: bounds the workspace
 
 // The kernels of one pair of types are compiled in a file of their own (residual_norm_<types>.cu).
 #define OPUS_NORM_LAUNCHES(NAME)                                                                                       \
@@ -341,12 +387,5 @@ OPUS_NORM_LAUNCHES(f32)
 OPUS_NORM_LAUNCHES(f32_bf16)
 OPUS_NORM_LAUNCHES(f32_f16)
 #undef OPUS_NORM_LAUNCHES
-
-// Sets a kernel's dynamic shared memory limit where it needs more than the default.
-template <auto Kernel>
-int allow_shared(int bytes) {
-  if (bytes > 48 * 1024) OPUS_CUDA_TRY(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  return OPUS_OK;
-}
 
 }  // namespace opus

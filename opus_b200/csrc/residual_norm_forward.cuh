@@ -22,15 +22,19 @@ namespace {
 
 enum Form : int { kAlone, kJoin, kFull };  // no y; y; y with a norm or a gate
 
-template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
-__global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull || V < 8 ? 2 : 3)
+// Wide: the blocks of a cluster share a row, each holding a range of its columns.
+template <typename TX, typename TY, int V, int NV, int F, bool Wide>
+__global__ void __launch_bounds__(kNormThreads, F == kFull || V < 8 ? 2 : 3)
     residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
   extern __shared__ __align__(16) float shared[];
   constexpr bool kPairs = V == 8 && F == kFull;
   const int t = threadIdx.x % s.group;
   const int g = threadIdx.x / s.group;
-  const RowRun run(s.rows, static_cast<int64_t>(blockIdx.x) * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
-  const Columns<V, NV> c(s, t);
+  const int rank = Wide ? static_cast<int>(cluster_ctarank()) : 0;
+  const int base = Wide ? rank * s.group * NV * V : 0;
+  const int64_t unit = Wide ? blockIdx.x / s.ranks : blockIdx.x;
+  const RowRun run(s.rows, unit * s.groups + g, static_cast<int64_t>(s.blocks) * s.groups);
+  const Columns<V, NV> c(s, t, base);
   const TX* x = static_cast<const TX*>(a.x) + run.first * a.x_stride;
   const TY* y = static_cast<const TY*>(a.y) + (F != kAlone ? run.first * a.y_stride : 0);
   TX* hp = static_cast<TX*>(a.h) + run.first * s.d;
@@ -43,11 +47,11 @@ __global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull |
     xr.load(x, c);
     if constexpr (F != kAlone) yr.load(y, c);
   }
-  GroupSum<norm_sub_warp(V, NV)> sum(shared, s.group, s.groups);
-  float* place = shared + group_floats(s.group, s.groups);
-  Param<NV, V, Near> w(a.weight, a.weight_dtype, 1.f), b(a.bias, a.bias_dtype, 0.f);
-  Param<NV, V, Near> pw(a.post_weight, a.post_weight_dtype, 1.f), pb(a.post_bias, a.post_bias_dtype, 0.f);
-  Param<NV, V, Near> q(a.gate, a.gate_dtype, 1.f);
+  GroupSum<norm_sub_warp(V, NV), Wide> sum(shared, s, rank);
+  float* place = shared + group_floats(s.group, s.groups, Wide ? s.ranks : 1);
+  Param<NV, V> w(a.weight, a.weight_dtype, 1.f, base), b(a.bias, a.bias_dtype, 0.f, base);
+  Param<NV, V> pw(a.post_weight, a.post_weight_dtype, 1.f, base), pb(a.post_bias, a.post_bias_dtype, 0.f, base);
+  Param<NV, V> q(a.gate, a.gate_dtype, 1.f, base);
   w.fill(&place, s);
   b.fill(&place, s);
   const bool one_gate = s.seq == s.rows;
@@ -111,59 +115,39 @@ __global__ void __launch_bounds__(norm_threads(V, Wide), Wide ? 1 : F == kFull |
     for (int k = 0; k < NV; ++k) vfma<kPairs>(h[k], u[k], o[k]);
     store_row(np, c, h);
     np += s.d;
-    if (t == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
+    if (t == 0 && rank == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
   }
 }
 
-template <typename TX, typename TY, int V, int NV, int F, bool Near, bool Wide>
+template <typename TX, typename TY, int V, int NV, int F, bool Wide>
 int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t st) {
-  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Near, Wide>;
-  const int threads = s.group * s.groups;
+  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Wide>;
   const int arrays = F != kFull ? 2 : s.seq == s.rows ? 5 : 4;
-  const int shared = (group_floats(s.group, s.groups) + arrays * Param<NV, V, Near>::size(s.group)) * static_cast<int>(sizeof(float));
-  const int rc = allow_shared<kernel>(shared);
+  NormLaunch launch;
+  const int rc = launch.plan<kernel>(&s, group_floats(s.group, s.groups, s.ranks) + arrays * Param<NV, V>::size(s.group), 32, st);
   if (rc) return rc;
-  const int64_t need = (s.rows + s.groups - 1) / s.groups;
-  const int64_t most = static_cast<int64_t>(sm_count()) * resident_blocks<kernel>(threads, shared);
-  s.blocks = static_cast<int>(need < most ? need : most);
-  kernel<<<s.blocks, threads, shared, st>>>(s, a);
+  OPUS_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, kernel, s, a));
   note_launch();
-  OPUS_CUDA_TRY(cudaGetLastError());
   return OPUS_OK;
-}
-
-template <typename TX, typename TY, int V, int NV, int F>
-int forward_wide(const opus_residual_norm_args& a, cudaStream_t st) {
-  NormShape s;
-  int nv;
-  const int rc = norm_shape("residual_norm", &a, V, NV, &s, &nv);
-  if (rc) return rc;
-  if constexpr (F == kFull) {
-    if (5 * Param<NV, V, true>::size(s.group) * static_cast<int>(sizeof(float)) > kNormSharedParams)
-      return launch_forward<TX, TY, V, NV, F, false, true>(s, a, st);
-  }
-  return launch_forward<TX, TY, V, NV, F, true, true>(s, a, st);
 }
 
 template <typename TX, typename TY, int V, int F>
 int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   NormShape s;
-  int nv;
   constexpr bool kBoth = F == kFull;
-  if (a.d > norm_narrow(V, kBoth)) {
-    return a.d <= kNormMiddle ? forward_wide<TX, TY, V, middle_vectors(V), F>(a, st)
-                              : forward_wide<TX, TY, V, 2 * middle_vectors(V), F>(a, st);
-  }
   constexpr int kMost = narrow_vectors(V, kBoth), kFewer = fewer_vectors(V, kBoth);
-  const int rc = norm_shape("residual_norm", &a, V, kMost, &s, &nv);
-  if (rc) return rc;
+  if (a.d > norm_narrow(V, kBoth)) {
+    norm_shape_wide(&a, V, kMost, &s);
+    return launch_forward<TX, TY, V, kMost, F, true>(s, a, st);
+  }
+  const int nv = norm_shape(&a, V, kMost, &s);
   if constexpr (V > 1) {
-    if (nv == 1) return launch_forward<TX, TY, V, 1, F, true, false>(s, a, st);
+    if (nv == 1) return launch_forward<TX, TY, V, 1, F, false>(s, a, st);
   }
   if constexpr (V < 8) {
-    if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, true, false>(s, a, st);
+    if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, false>(s, a, st);
   }
-  return launch_forward<TX, TY, V, kMost, F, true, false>(s, a, st);
+  return launch_forward<TX, TY, V, kMost, F, false>(s, a, st);
 }
 
 template <typename TX, typename TY, int V>

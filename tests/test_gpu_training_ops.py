@@ -243,7 +243,7 @@ def check_norm(c, p, dn, dh, kind="rms", post=False, r=1.0, eps=1e-5):
     """Forward against 64 bits, backward against the formulas in 64 bits at the stored h.
 
     K = 192 for the forward: the longest chain is a row's sum (16 elements a
-    thread, 5 shuffles, up to 32 warps), twice for a layer norm and twice
+    thread, 5 shuffles, up to 64 warps by fours), twice for a layer norm and twice
     again with a norm of y.  K = 768 + rows for the backward: four such sums
     in a row, and sums over rows.
     """
@@ -374,6 +374,27 @@ def test_residual_norm_many_rows(rows):
     check_norm(*norm_case(rows, (rows,), 136, torch.bfloat16, post=True, gate="channel", bias=True), kind="layer", post=True)
     check_norm(*norm_case(rows, (2, rows), 136, post=True, gate="sample"), post=True)
     check_norm(*norm_case(rows, (rows, 2), 24, post=False, gate="sample"))
+
+
+@pytest.mark.parametrize("dtype,x_dtype", [(torch.bfloat16, None), (torch.float32, None), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("d", [2047, 2048, 2049, 2056, 4095, 4096, 4097, 4100, 4104, 8191, 8192, 8193, 8200, 16383])
+def test_residual_norm_where_rows_are_split(d, dtype, x_dtype):
+    """Widths at which a row passes from one block to a cluster of two, four and eight."""
+    for kind, post, gate in (("rms", False, None), ("layer", True, "sample")):
+        check_norm(*norm_case(d, (3, 3), d, dtype, x_dtype, post=post, gate=gate, bias=kind == "layer"), kind=kind, post=post)
+
+
+@pytest.mark.parametrize("shape,d", [((3, 133), 4104), ((2, 200), 8193), ((5, 40), 16384), ((301, 2), 5001)])
+def test_residual_norm_many_wide_rows(shape, d):
+    """More rows than clusters run at once: several rows a cluster, whose runs cross samples."""
+    check_norm(*norm_case(d, shape, d, torch.bfloat16, post=True, gate="sample", bias=True), kind="layer", post=True)
+    check_norm(*norm_case(d, shape, d, post=True, gate="channel"), post=True)
+    check_norm(*norm_case(d, shape, d, torch.bfloat16))
+
+
+def test_residual_norm_more_gates_than_one_launch_joins():
+    check_norm(*norm_case(3, (70000,), 24, gate="sample"))
+    check_norm(*norm_case(4, (140000, 1), 8, torch.bfloat16, gate="sample", post=True, bias=True), kind="layer", post=True)
 
 
 def test_residual_norm_no_rows():
