@@ -62,6 +62,7 @@ enum DeviceError : int {
   kDevTimeoutGroup = 0x104,
   kDevTimeoutDrain = 0x105,
   kDevTimeoutSelftest = 0x106,  // opus_selftest_stalled_wait: a wait that nothing releases
+  kDevTimeoutRow = 0x107,  // opus_residual_norm(_grad): a wide row's sums from another block
   kDevBadBucket = 0x201,
   kDevBadToken = 0x202,  // opus_embedding(_grad): a token outside [0, vocab)
 };

@@ -56,6 +56,7 @@ int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s) 
   s->group = group;
   s->groups = group >= kNormThreads ? 1 : kNormThreads / group;
   s->ranks = 1;
+  s->err = nullptr;
   s->layer = a->kind;
   s->eps = a->eps;
   s->blocks = 0;
@@ -64,7 +65,7 @@ int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s) 
 
 // Of rows wider than a block of NV vectors a thread: a cluster of as few blocks (2, 4 or 8) as hold a row, and as few
 // threads in each as share it evenly (more than 64, since half as many full blocks would not have held it).
-void norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape* s) {
+int norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape* s) {
   norm_shape(a, V, NV, s);
   const int full = (a->d + V - 1) / V;
   int ranks = 2;
@@ -72,6 +73,8 @@ void norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape*
   s->group = ((full + ranks * NV - 1) / (ranks * NV) + 31) / 32 * 32;
   s->groups = 1;
   s->ranks = ranks;
+  s->err = device_error_word();
+  return s->err != nullptr ? OPUS_OK : set_error(OPUS_ERR_CUDA, "device error word unavailable");
 }
 
 namespace {

@@ -40,6 +40,7 @@ struct NormShape {
   int layer;          // LayerNorm (1) or RMS norm (0)
   float eps;
   int blocks;  // of the launch, or clusters of them
+  int* err;    // the device error word (clusters)
 };
 
 // The rows [first, last) of worker w among n.
@@ -53,39 +54,53 @@ struct RowRun {
 };
 
 // Shared memory of a group's sums: slots of its warps (a multiple of 4; of every block of the row), twice for two
-// values, twice for two turns.
+// values, twice for two turns; two mbarriers behind them for a cluster.
 __host__ __device__ constexpr int group_slots(int group) { return group <= 32 ? 0 : ((group >> 5) + 3) / 4 * 4; }
 __host__ __device__ constexpr int group_floats(int group, int groups, int ranks) {
-  return 4 * groups * ranks * group_slots(group);
+  return 4 * groups * ranks * group_slots(group) + (ranks > 1 ? 4 : 0);
 }
 
 // Whether a thread's group may be less than a warp (norm_shape's smallest vector counts).
 constexpr bool norm_sub_warp(int V, int NV) { return NV == 1 || (V == 1 && NV == 4); }
 
 // Sums over the group of up to two values each, in a fixed order; the result is in every thread of the group.
-// A call takes one barrier of the group's own, or of the cluster, whose blocks write their warps' sums to each
-// other: `turn` alternates between two buffers, so that one is written while the other may still be read.
+// A call takes one barrier of the group's own.  The blocks of a cluster send their warps' sums to each other, counted
+// on the receiver's mbarrier: a barrier of the cluster would wait for the row's stores to HBM too (8192 x 8192 bf16
+// backward with both norms: 340 us, 250 so).
+// `turn` alternates between two buffers: a block sends the sums after next only when it has had the next ones of
+// every warp, and those are sent after the warp has read the buffer.
 template <bool SubWarp, bool Cluster>
 struct GroupSum {
   float* buf;
   int slots, span, barrier, threads;
   unsigned lanes;
   int turn;
-  int ranks, rank;
+  const NormShape& shape;
+  uint32_t phases;  // bit 0 or 1: the parity that the turn's mbarrier completes next; bit 2: a wait ran out (the sums
+                    // are wrong from there, and the error word says so)
 
   // every thread of the block calls it once
-  __device__ GroupSum(float* shared, const NormShape& s, int rank_)
-      : threads(s.group), lanes(0xffffffffu), turn(0), ranks(Cluster ? s.ranks : 1), rank(rank_) {
-    slots = group_slots(s.group) * ranks;  // of the row's warps, zeros behind each block's
+  __device__ GroupSum(float* shared, const NormShape& s)
+      : threads(s.group), lanes(0xffffffffu), turn(0), shape(s), phases(0) {
+    slots = group_slots(s.group) * (Cluster ? s.ranks : 1);  // of the row's warps, zeros behind each block's
     span = s.groups * slots;
     const int g = static_cast<int>(threadIdx.x) / s.group;
     buf = shared + g * slots;
     barrier = 1 + g;  // named barriers 1 to 15: a block has at most 4 groups of more than a warp
     if (SubWarp && s.group < 32) lanes = ((1u << s.group) - 1) << ((threadIdx.x & 31) / s.group * s.group);
     for (int i = threadIdx.x; i < 4 * span; i += blockDim.x) shared[i] = 0.f;
-    __syncwarp();
-    if constexpr (Cluster) cluster_sync();  // before another block writes here
-    else __syncthreads();
+    if constexpr (Cluster) {
+      uint64_t* bars = reinterpret_cast<uint64_t*>(shared + 4 * span);
+      if (threadIdx.x == 0) {
+        mbar_init(bars, 1);
+        mbar_init(bars + 1, 1);
+        fence_mbar_init();
+      }
+      __syncwarp();
+      cluster_sync();  // before another block writes here
+    } else {
+      __syncthreads();
+    }
   }
   template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N], int t) {
@@ -99,14 +114,20 @@ struct GroupSum {
     float* b = buf + turn;
     turn = 2 * span - turn;
     if constexpr (Cluster) {
+      const int which = turn == 0;  // of the turn that b is
+      uint64_t* bar = reinterpret_cast<uint64_t*>(buf + 4 * span) + which;
       const int lane = t & 31;
-      if (lane < ranks) {
-        float* own = b + rank * (slots / ranks) + (t >> 5);
+      if (phases < 4) {
+        if (t == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(shape.ranks * (threads >> 5) * N * sizeof(float)));
+        if (lane < shape.ranks) {
+          float* own = b + cluster_ctarank() * group_slots(threads) + (t >> 5);
 #pragma unroll
-        for (int i = 0; i < N; ++i) store_peer(own + i * span, lane, v[i]);
+          for (int i = 0; i < N; ++i) send(own + i * span, bar, lane, v[i]);
+        }
+        if (!mbar_wait(bar, phases >> which & 1, nullptr, shape.err, kDevTimeoutRow)) phases |= 4;
+        phases ^= 1u << which;
       }
       __syncwarp();
-      cluster_sync();
     } else {
       if ((t & 31) == 0) {
 #pragma unroll
@@ -126,11 +147,21 @@ struct GroupSum {
     }
   }
 
+  // at the kernel's end, by every thread: no block leaves while another may still send to it
+  __device__ __forceinline__ void leave() {
+    if constexpr (Cluster) {
+      __syncwarp();
+      cluster_sync();
+    }
+  }
+
  private:
-  // *p = v in the shared memory of the cluster's block `peer`
-  static __device__ __forceinline__ void store_peer(float* p, int peer, float v) {
+  // *p = v in the shared memory of the cluster's block `peer`, counted on its mbarrier
+  static __device__ __forceinline__ void send(float* p, uint64_t* bar, int peer, float v) {
     const uint32_t to = mapa_shared(smem_u32(p), static_cast<uint32_t>(peer));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+    const uint32_t on = mapa_shared(smem_u32(bar), static_cast<uint32_t>(peer));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(to), "f"(v), "r"(on)
+                 : "memory");
   }
 };
 
@@ -360,7 +391,7 @@ struct NormLaunch {
 };
 
 int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s);
-void norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape* s);
+int norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape* s);
 int check_norm(const char* what, const opus_residual_norm_args* a);
 bool norm_params_aligned(const opus_residual_norm_args* a);
 

@@ -20,7 +20,9 @@
 // 5.0 TB/s (161 registers: one block an SM); both norms and a gate 369 us, 4.4
 // TB/s (241 registers: eight warps an SM, a third of the issue slots).  8 elements
 // a thread would leave room for twice the warps and took 535 us.  32768 x 2048 f32:
-// 213 us, 6.3 TB/s.  Wide rows are read twice: 8192 x 8192 f32 356 us, 3.8 TB/s.
+// 213 us, 6.3 TB/s.  Wide rows, 8192 x 8192: bf16 RMS 115 us (5.8 TB/s), both
+// norms and a gate 250 (3.2); f32 219 us (6.1 TB/s).  A kernel for dx and dy and
+// a second read of the rows for the sums took 256, 445 and 356.
 #pragma once
 
 #include "residual_norm.cuh"
@@ -34,12 +36,23 @@ __device__ __forceinline__ int64_t worker_of(int64_t row, int64_t rows, int64_t 
   return row < cut ? row / (each + 1) : more + (row - cut) / each;
 }
 
+// Blocks that a multiprocessor's registers have to hold: two where the sums of a thread's columns leave room for them
+// (16384 x 4096 bf16 RMS 111 us, 138 with the registers of one; 500000 x 128 with layer norms 136 and 185), three for
+// 4 elements a thread, otherwise one, which may then use all that it needs (8192 x 8192 f32 with both layer norms
+// 593 us, 674 where the compiler chose).
+constexpr int grad_blocks(int V, int NV, bool full, bool bias) {
+  const int elements = V * NV;
+  if (elements <= 4) return full ? 2 : 3;
+  if (elements <= 8) return !full || (V == 8 && !bias) ? 2 : 1;
+  return V == 8 && !full && !bias ? 2 : 1;
+}
+
 // parts[block or cluster][array][d]: sums over its rows.  gates[worker + sample][d]: sums over the worker's rows of
 // one sample, where each sample has a gate (a step to the next worker or sample is a step to the next slot).
 // Full: with a norm of y or a gate.  Bias: sums for bias and post_bias too.
 // Wide: the blocks of a cluster share a row, each holding a range of its columns.
 template <typename TX, typename TY, int V, int NV, bool Full, bool Bias, bool Wide>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Full, Bias))
     grad_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a, int wanted,
                 float* __restrict__ parts, float* __restrict__ gates) {
   extern __shared__ __align__(16) float shared[];
@@ -72,7 +85,7 @@ __global__ void __launch_bounds__(kNormThreads)
     hp += a.h_stride, dhp += a.grad_h_stride, dnp += a.grad_n_stride, yp += a.y_stride, ++stats;
   };
   if (run.first < run.last) fetch();
-  GroupSum<norm_sub_warp(V, NV), Wide> sum(shared, s, rank);
+  GroupSum<norm_sub_warp(V, NV), Wide> sum(shared, s);
   float* meet = shared + group_floats(s.group, s.groups, Wide ? s.ranks : 1);
   float* place = meet + (s.groups > 1 ? blockDim.x * V * NV : 0);
   const bool one_gate = s.seq == s.rows;
@@ -222,6 +235,7 @@ __global__ void __launch_bounds__(kNormThreads)
     if constexpr (Bias) finish(acc_pb, kPostBias);
     if (one_gate) finish(acc_g, kGate);
   }
+  sum.leave();
 }
 
 constexpr int kSlices = 32;
@@ -316,8 +330,8 @@ int backward_by_width(const opus_residual_norm_args& a, int wanted, const Column
   NormShape s;
   if (a.d > norm_narrow(V, Full)) {
     constexpr int kWide = kLean ? kFewer : kMost;
-    norm_shape_wide(&a, V, kWide, &s);
-    return launch_backward<TX, TY, V, kWide, Full, Bias, true>(s, a, wanted, out, ws, st);
+    const int rc = norm_shape_wide(&a, V, kWide, &s);
+    return rc ? rc : launch_backward<TX, TY, V, kWide, Full, Bias, true>(s, a, wanted, out, ws, st);
   }
   const bool lean = kLean && a.d <= norm_narrow(V, Full) / 2;
   const int nv = norm_shape(&a, V, lean ? kFewer : kMost, &s);

@@ -22,14 +22,21 @@ namespace {
 
 enum Form : int { kAlone, kJoin, kFull };  // no y; y; y with a norm or a gate
 
-// Wide: the blocks of a cluster share a row, each holding a range of its columns.
-template <typename TX, typename TY, int V, int NV, int F, bool Wide>
-__global__ void __launch_bounds__(kNormThreads, F == kFull || V < 8 ? 2 : 3)
+// What holds a row: a block (or a group of its threads), a block of twice the threads, which has no parameter sums to
+// keep in registers and needs no other block, or the blocks of a cluster, each with a range of the columns.  At 8192
+// columns the larger block takes 129 us where a cluster of two takes 134 (8192 rows, bf16, both norms and a gate; 167
+// and 206 for layer norms with biases).
+enum Split : int { kBlock, kLargeBlock, kCluster };
+
+template <typename TX, typename TY, int V, int NV, int F, int By>
+__global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormThreads,
+                                  By == kLargeBlock ? 1 : F == kFull || V < 8 ? 2 : 3)
     residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
   extern __shared__ __align__(16) float shared[];
   constexpr bool kPairs = V == 8 && F == kFull;
   const int t = threadIdx.x % s.group;
   const int g = threadIdx.x / s.group;
+  constexpr bool Wide = By == kCluster;
   const int rank = Wide ? static_cast<int>(cluster_ctarank()) : 0;
   const int base = Wide ? rank * s.group * NV * V : 0;
   const int64_t unit = Wide ? blockIdx.x / s.ranks : blockIdx.x;
@@ -47,7 +54,7 @@ __global__ void __launch_bounds__(kNormThreads, F == kFull || V < 8 ? 2 : 3)
     xr.load(x, c);
     if constexpr (F != kAlone) yr.load(y, c);
   }
-  GroupSum<norm_sub_warp(V, NV), Wide> sum(shared, s, rank);
+  GroupSum<norm_sub_warp(V, NV), Wide> sum(shared, s);
   float* place = shared + group_floats(s.group, s.groups, Wide ? s.ranks : 1);
   Param<NV, V> w(a.weight, a.weight_dtype, 1.f, base), b(a.bias, a.bias_dtype, 0.f, base);
   Param<NV, V> pw(a.post_weight, a.post_weight_dtype, 1.f, base), pb(a.post_bias, a.post_bias_dtype, 0.f, base);
@@ -117,11 +124,12 @@ __global__ void __launch_bounds__(kNormThreads, F == kFull || V < 8 ? 2 : 3)
     np += s.d;
     if (t == 0 && rank == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
   }
+  sum.leave();
 }
 
-template <typename TX, typename TY, int V, int NV, int F, bool Wide>
+template <typename TX, typename TY, int V, int NV, int F, int By>
 int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t st) {
-  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Wide>;
+  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, By>;
   const int arrays = F != kFull ? 2 : s.seq == s.rows ? 5 : 4;
   NormLaunch launch;
   const int rc = launch.plan<kernel>(&s, group_floats(s.group, s.groups, s.ranks) + arrays * Param<NV, V>::size(s.group), 32, st);
@@ -136,18 +144,24 @@ int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   NormShape s;
   constexpr bool kBoth = F == kFull;
   constexpr int kMost = narrow_vectors(V, kBoth), kFewer = fewer_vectors(V, kBoth);
+  if constexpr (V > 1) {  // single elements would need 1024 threads of 64 registers
+    if (a.d > norm_narrow(V, kBoth) && a.d <= 2 * norm_narrow(V, kBoth)) {
+      norm_shape(&a, V, kMost, &s);
+      return launch_forward<TX, TY, V, kMost, F, kLargeBlock>(s, a, st);
+    }
+  }
   if (a.d > norm_narrow(V, kBoth)) {
-    norm_shape_wide(&a, V, kMost, &s);
-    return launch_forward<TX, TY, V, kMost, F, true>(s, a, st);
+    const int rc = norm_shape_wide(&a, V, kMost, &s);
+    return rc ? rc : launch_forward<TX, TY, V, kMost, F, kCluster>(s, a, st);
   }
   const int nv = norm_shape(&a, V, kMost, &s);
   if constexpr (V > 1) {
-    if (nv == 1) return launch_forward<TX, TY, V, 1, F, false>(s, a, st);
+    if (nv == 1) return launch_forward<TX, TY, V, 1, F, kBlock>(s, a, st);
   }
   if constexpr (V < 8) {
-    if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, false>(s, a, st);
+    if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, kBlock>(s, a, st);
   }
-  return launch_forward<TX, TY, V, kMost, F, false>(s, a, st);
+  return launch_forward<TX, TY, V, kMost, F, kBlock>(s, a, st);
 }
 
 template <typename TX, typename TY, int V>
