@@ -982,6 +982,8 @@ def _clip_targets(grads, out, name: str) -> tuple[_TensorList, _TensorList, list
         for t in g.copied:
             if any(stride == 0 and size > 1 for stride, size in zip(t.stride(), t.shape)):
                 raise ValueError(f"{name}: a gradient's elements overlap in memory (an expanded tensor)")
+        if len({(t.data_ptr(), t.shape, t.stride()) for t in g.copied if t.numel()}) < sum(t.numel() > 0 for t in g.copied):
+            raise ValueError(f"{name}: an element would be written twice (a tensor listed twice)")
         return g, g, [(t, c) for t, c in zip(grads, g.tensors) if t is not c]
     g, o = _TensorList(grads, "grads", contiguous=True), _TensorList(out, "out", contiguous=True)
     if o.copied:
@@ -1004,7 +1006,8 @@ def clip_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, no
     product rounded once.  Gradients whose norm is within the bound are not
     written in place.  A list that would write an element twice (a gradient
     listed twice, overlapping views, an out that overlaps the gradients) is
-    refused.  A NaN norm makes every gradient NaN.  The norm is a
+    refused; of views with gaps between their elements only equal ones are,
+    and elements that several share are scaled once.  A NaN norm makes every gradient NaN.  The norm is a
     float32 scalar on the device, and nothing waits for the host.
     """
     kind = _norm_kind(norm_type)

@@ -686,6 +686,16 @@ def test_clip_grads_refuses_what_it_would_write_twice():
     with pytest.raises(ValueError, match="twice"):
         clip_grad_norm_([p, p], 1.0)
     assert bool((a == 1).all()) and bool((b == 1).all()) and bool((p.grad == 1).all())
+    gaps = torch.full((6, 8), 2.0, device=DEV)
+    for grads in ([gaps[:, :3], gaps[:, :3]], [a, gaps[:, 1::2], gaps[:, 1::2]]):
+        with pytest.raises(ValueError, match="twice"):
+            ops.clip_grads(grads, 1.0)
+        with pytest.raises(ValueError, match="twice"):
+            ops.scale_grads(grads, 1.0, torch.ones((), device=DEV))
+    assert bool((gaps == 2).all())
+    ops.scale_grads([gaps[:, :3], gaps[:, 2:5], gaps[:0, :3], gaps[:0, :3]], 1.0, torch.full((), 4.0, device=DEV))
+    c = np.float32(1.0) / (np.float32(4.0) + np.float32(1e-6))
+    assert bool((gaps[:, :5] == float(np.float32(2.0) * c)).all()) and bool((gaps[:, 5:] == 2).all())  # scaled once
     assert float(ops.grad_norm([b, b])) == float(np.float32(80 ** 0.5))  # reading twice is fine
     assert float(ops.clip_grads([a[:300], a[300:]], 1.0)) > 1  # neighbours share no element
 
@@ -769,6 +779,33 @@ assert torch.equal(y, w[t] * 2) and float(norm) > 0 and bool(g["x"].isfinite().a
 ops.check_device_error()
 print("captured")
 """
+
+
+@pytest.mark.parametrize("d", [5120, 4099])
+def test_wide_rows_captured_and_on_streams_at_once(d):
+    """Rows split among clusters: replayed in a graph, and from several streams together, with the eager results."""
+    c, p, dn, dh = norm_case(d, (3, 100), d, torch.bfloat16, post=True, gate="sample", bias=True)
+
+    def run():
+        n, h, stats = ops.residual_norm(c["x"], c["y"], **p, kind="layer")
+        got = ops.residual_norm_grad(dn, dh, h, stats, c["y"], **p, kind="layer")
+        return [n, h, stats, *(got[k] for k in sorted(got))]
+
+    want = run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(3):
+        graph.replay()
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for x in (captured, *got) for a, b in zip(x, want))
+    ops.check_device_error()
 
 
 def test_first_call_may_be_captured():
