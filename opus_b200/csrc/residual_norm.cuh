@@ -300,8 +300,8 @@ struct Param {
   __device__ __forceinline__ Param(const void* p_, int dtype_, float other_, int base_)
       : p(p_), dtype(dtype_), base(base_), other(other_), near(nullptr), far(nullptr) {}
   static __host__ __device__ int size(int group) { return group * NV * V; }
-  // by every thread; a barrier has to follow
-  __device__ __forceinline__ void fill(float** shared, const NormShape& s) {
+  // by every thread; a barrier has to follow.  times: another parameter to multiply by, or NULL
+  __device__ __forceinline__ void fill(float** shared, const NormShape& s, const void* times = nullptr, int times_dtype = 0) {
     near = *shared;
     const int whole = size(s.group);
     far = near + whole / 2;
@@ -312,6 +312,12 @@ struct Param {
 #pragma unroll
       for (int i = 0; i < V; ++i) r[i] = own ? other : 0.f;
       if (p != nullptr && own) load_param_vec<V>(p, dtype, base + col, r);
+      if (times != nullptr && own) {
+        float m[V];
+        load_param_vec<V>(times, times_dtype, base + col, m);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] *= m[i];
+      }
       if constexpr (V == 8) {
         *reinterpret_cast<float4*>(near + col / 2) = make_float4(r[0], r[1], r[2], r[3]);
         *reinterpret_cast<float4*>(far + col / 2) = make_float4(r[4], r[5], r[6], r[7]);

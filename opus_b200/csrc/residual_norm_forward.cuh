@@ -9,10 +9,11 @@
 //
 // Bound: HBM bandwidth; x and y are read once, h and n written once, nothing
 // else but 16 bytes of statistics a row.  65536 x 2048 bf16: 185 us, 5.8 TB/s;
-// 32768 x 2048 f32 185 us, 5.8 TB/s.  With norms on both sides and a gate 16-bit
-// rows are bound by the instructions they issue (26 an element, 49% of the
-// issue slots at the 16 warps that their registers leave): 213 us, 5.0 TB/s; f32
-// ones are not: 175 us, 6.1 TB/s.
+// 32768 x 2048 f32 185 us, 5.8 TB/s.  With norms on both sides and a gate 181 us,
+// 5.9 TB/s (f32 186): the gate that all rows share is folded into post_weight and
+// post_bias once a block, and biases that are not there are not read.  Reading
+// all five arrays from shared memory for every row took 213 us, its warps
+// waiting for that memory most.
 #pragma once
 
 #include "residual_norm.cuh"
@@ -24,11 +25,12 @@ enum Form : int { kAlone, kJoin, kFull };  // no y; y; y with a norm or a gate
 
 // What holds a row: a block (or a group of its threads), a block of twice the threads, which has no parameter sums to
 // keep in registers and needs no other block, or the blocks of a cluster, each with a range of the columns.  At 8192
-// columns the larger block takes 129 us where a cluster of two takes 134 (8192 rows, bf16, both norms and a gate; 167
-// and 206 for layer norms with biases).
+// columns the larger block takes 100 us where a cluster of two takes 109 (8192 rows, bf16, layer norms; 167 and 206 with
+// both norms and a gate).
 enum Split : int { kBlock, kLargeBlock, kCluster };
 
-template <typename TX, typename TY, int V, int NV, int F, int By>
+// Bias: with a bias or post_bias.
+template <typename TX, typename TY, int V, int NV, int F, bool Bias, int By>
 __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormThreads,
                                   By == kLargeBlock ? 1 : F == kFull || V < 8 ? 2 : 3)
     residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
@@ -58,14 +60,13 @@ __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormTh
   float* place = shared + group_floats(s.group, s.groups, Wide ? s.ranks : 1);
   Param<NV, V> w(a.weight, a.weight_dtype, 1.f, base), b(a.bias, a.bias_dtype, 0.f, base);
   Param<NV, V> pw(a.post_weight, a.post_weight_dtype, 1.f, base), pb(a.post_bias, a.post_bias_dtype, 0.f, base);
-  Param<NV, V> q(a.gate, a.gate_dtype, 1.f, base);
   w.fill(&place, s);
-  b.fill(&place, s);
-  const bool one_gate = s.seq == s.rows;
+  if constexpr (Bias) b.fill(&place, s);
+  const bool one_gate = s.seq == s.rows;  // it is folded into the norm's weight and bias
   if constexpr (F == kFull) {
-    pw.fill(&place, s);
-    pb.fill(&place, s);
-    if (one_gate) q.fill(&place, s);
+    const void* gate = one_gate ? a.gate : nullptr;
+    pw.fill(&place, s, gate, a.gate_dtype);
+    if constexpr (Bias) pb.fill(&place, s, gate, a.gate_dtype);
   }
   __syncthreads();
   int64_t until = 0, gate_at = 0;  // the first row of the next sample, this sample's gate
@@ -84,24 +85,27 @@ __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormTh
       float p[NV][V];
       if (a.post) {
         ys = row_stats<kPairs>(u, s, c, t, sum);
-        float o[NV][V];
-        pw.row(c, p);
-        pb.row(c, o);
         normalize<kPairs>(u, ys.x, ys.y);
+      }
+      pw.row(c, p);
+      if constexpr (Bias) {
+        float o[NV][V];
+        pb.row(c, o);
 #pragma unroll
         for (int k = 0; k < NV; ++k) vfma<kPairs>(u[k], p[k], o[k]);
-      }
-      if (one_gate) {
-        q.row(c, p);
       } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
+      }
+      if (!one_gate) {
         if (row >= until) {
           gate_at = row / s.seq * s.d;
           until = (row / s.seq + 1) * s.seq;
         }
         load_param_row(a.gate, a.gate_dtype, gate_at, 1.f, c, p);
-      }
 #pragma unroll
-      for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
+        for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
+      }
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -114,12 +118,17 @@ __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormTh
     }
     hp += s.d;
     const float2 hs = row_stats<kPairs>(h, s, c, t, sum);
-    float o[NV][V];
     w.row(c, u);
-    b.row(c, o);
     normalize<kPairs>(h, hs.x, hs.y);
+    if constexpr (Bias) {
+      float o[NV][V];
+      b.row(c, o);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) vfma<kPairs>(h[k], u[k], o[k]);
+      for (int k = 0; k < NV; ++k) vfma<kPairs>(h[k], u[k], o[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) vmul<kPairs>(h[k], u[k]);
+    }
     store_row(np, c, h);
     np += s.d;
     if (t == 0 && rank == 0) reinterpret_cast<float4*>(a.stats)[row] = make_float4(hs.x, hs.y, ys.x, ys.y);
@@ -127,10 +136,10 @@ __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormTh
   sum.leave();
 }
 
-template <typename TX, typename TY, int V, int NV, int F, int By>
+template <typename TX, typename TY, int V, int NV, int F, bool Bias, int By>
 int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t st) {
-  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, By>;
-  const int arrays = F != kFull ? 2 : s.seq == s.rows ? 5 : 4;
+  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Bias, By>;
+  const int arrays = (F == kFull ? 2 : 1) * (Bias ? 2 : 1);
   NormLaunch launch;
   const int rc = launch.plan<kernel>(&s, group_floats(s.group, s.groups, s.ranks) + arrays * Param<NV, V>::size(s.group), 32, st);
   if (rc) return rc;
@@ -139,7 +148,7 @@ int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t s
   return OPUS_OK;
 }
 
-template <typename TX, typename TY, int V, int F>
+template <typename TX, typename TY, int V, int F, bool Bias>
 int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   NormShape s;
   constexpr bool kBoth = F == kFull;
@@ -147,28 +156,34 @@ int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   if constexpr (V > 1) {  // single elements would need 1024 threads of 64 registers
     if (a.d > norm_narrow(V, kBoth) && a.d <= 2 * norm_narrow(V, kBoth)) {
       norm_shape(&a, V, kMost, &s);
-      return launch_forward<TX, TY, V, kMost, F, kLargeBlock>(s, a, st);
+      return launch_forward<TX, TY, V, kMost, F, Bias, kLargeBlock>(s, a, st);
     }
   }
   if (a.d > norm_narrow(V, kBoth)) {
     const int rc = norm_shape_wide(&a, V, kMost, &s);
-    return rc ? rc : launch_forward<TX, TY, V, kMost, F, kCluster>(s, a, st);
+    return rc ? rc : launch_forward<TX, TY, V, kMost, F, Bias, kCluster>(s, a, st);
   }
   const int nv = norm_shape(&a, V, kMost, &s);
   if constexpr (V > 1) {
-    if (nv == 1) return launch_forward<TX, TY, V, 1, F, kBlock>(s, a, st);
+    if (nv == 1) return launch_forward<TX, TY, V, 1, F, Bias, kBlock>(s, a, st);
   }
   if constexpr (V < 8) {
-    if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, kBlock>(s, a, st);
+    if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, Bias, kBlock>(s, a, st);
   }
-  return launch_forward<TX, TY, V, kMost, F, kBlock>(s, a, st);
+  return launch_forward<TX, TY, V, kMost, F, Bias, kBlock>(s, a, st);
+}
+
+template <typename TX, typename TY, int V, int F>
+int forward_by_bias(const opus_residual_norm_args& a, cudaStream_t st) {
+  return a.bias != nullptr || a.post_bias != nullptr ? forward_by_width<TX, TY, V, F, true>(a, st)
+                                                     : forward_by_width<TX, TY, V, F, false>(a, st);
 }
 
 template <typename TX, typename TY, int V>
 int forward_by_form(const opus_residual_norm_args& a, cudaStream_t st) {
-  if (a.post || a.gate != nullptr) return forward_by_width<TX, TY, V, kFull>(a, st);
-  if (a.y != nullptr) return forward_by_width<TX, TY, V, kJoin>(a, st);
-  return forward_by_width<TX, TY, V, kAlone>(a, st);
+  if (a.post || a.gate != nullptr) return forward_by_bias<TX, TY, V, kFull>(a, st);
+  if (a.y != nullptr) return forward_by_bias<TX, TY, V, kJoin>(a, st);
+  return forward_by_bias<TX, TY, V, kAlone>(a, st);
 }
 
 template <typename TX, typename TY>
