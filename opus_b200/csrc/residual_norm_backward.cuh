@@ -9,7 +9,7 @@
 //   dy = (c - <c> - yh <c yh>) / sd_y;  dw_post = sum dz o yh;  db_post = sum dz
 //
 // One kernel reads each row once, writes dx and dy, and keeps a column's sums
-// over its run of rows in registers (16 columns a thread, five sums each); a
+// over its run of rows in registers (16 columns a thread, up to five sums each); a
 // second kernel joins the runs.  More than 256 threads would have too few
 // registers for that: rows wider than such a block holds (4096 elements, or
 // 2048) are split among the blocks of a cluster, which exchange the row's sums
@@ -17,11 +17,13 @@
 //
 // Bound: HBM bandwidth (h, dn, dh_in and y read once, dx and dy written once).
 // 65536 x 2048 bf16: RMS joints 210 us, 6.4 TB/s; layer norms with biases 267 us,
-// 5.0 TB/s (161 registers: one block an SM); both norms and a gate 369 us, 4.4
-// TB/s (241 registers: eight warps an SM, a third of the issue slots).  8 elements
-// a thread would leave room for twice the warps and took 535 us.  32768 x 2048 f32:
-// 213 us, 6.3 TB/s.  Wide rows, 8192 x 8192: bf16 RMS 115 us (5.8 TB/s), both
-// norms and a gate 250 (3.2); f32 219 us (6.1 TB/s).  A kernel for dx and dy and
+// 5.0 TB/s (161 registers: one block an SM); both norms and a gate 299 us, 5.4
+// TB/s (214 registers: eight warps an SM), 368 with a third sum a column for the
+// gate and five parameter arrays read for every row.  8 elements a thread would
+// leave room for twice the warps and took 535 us where 16 took 374.  32768 x 2048
+// f32: 213 us, 6.3 TB/s; both norms and a gate 252 us, 6.4 TB/s.  Wide rows, 8192
+// x 8192: bf16 RMS 115 us (5.8 TB/s), both norms and a gate 230 (3.5); f32 219 us
+// (6.1 TB/s).  A kernel for dx and dy and
 // a second read of the rows for the sums took 256, 445 and 356.
 #pragma once
 
@@ -40,7 +42,10 @@ __device__ __forceinline__ int64_t worker_of(int64_t row, int64_t rows, int64_t 
 // (16384 x 4096 bf16 RMS 111 us, 138 with the registers of one; 500000 x 128 with layer norms 136 and 185), three for
 // 4 elements a thread, otherwise one, which may then use all that it needs (8192 x 8192 f32 with both layer norms
 // 593 us, 674 where the compiler chose).
-constexpr int grad_blocks(int V, int NV, bool full, bool bias) {
+enum GradForm : int { kGradJoin, kGradFull, kGradSamples };  // y as it is; with a norm or one gate; a gate a sample
+
+constexpr int grad_blocks(int V, int NV, int form, bool bias) {
+  const bool full = form != kGradJoin;
   const int elements = V * NV;
   if (elements <= 4) return full ? 2 : 3;
   if (elements <= 8) return !full || (V == 8 && !bias) ? 2 : 1;
@@ -49,14 +54,15 @@ constexpr int grad_blocks(int V, int NV, bool full, bool bias) {
 
 // parts[block or cluster][array][d]: sums over its rows.  gates[worker + sample][d]: sums over the worker's rows of
 // one sample, where each sample has a gate (a step to the next worker or sample is a step to the next slot).
-// Full: with a norm of y or a gate.  Bias: sums for bias and post_bias too.
+// Bias: sums for bias and post_bias too.
 // Wide: the blocks of a cluster share a row, each holding a range of its columns.
-template <typename TX, typename TY, int V, int NV, bool Full, bool Bias, bool Wide>
-__global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Full, Bias))
+template <typename TX, typename TY, int V, int NV, int Form, bool Bias, bool Wide>
+__global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Form, Bias))
     grad_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a, int wanted,
                 float* __restrict__ parts, float* __restrict__ gates) {
   extern __shared__ __align__(16) float shared[];
   constexpr bool kPairs = V == 8;
+  constexpr bool Full = Form != kGradJoin, Samples = Form == kGradSamples;
   const int t = threadIdx.x % s.group;
   const int g = threadIdx.x / s.group;
   const int rank = Wide ? static_cast<int>(cluster_ctarank()) : 0;
@@ -88,18 +94,14 @@ __global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Full, Bias))
   GroupSum<norm_sub_warp(V, NV), Wide> sum(shared, s);
   float* meet = shared + group_floats(s.group, s.groups, Wide ? s.ranks : 1);
   float* place = meet + (s.groups > 1 ? blockDim.x * V * NV : 0);
-  const bool one_gate = s.seq == s.rows;
-  Param<NV, V> w(a.weight, a.weight_dtype, 1.f, base), q(a.gate, a.gate_dtype, 1.f, base);
+  Param<NV, V> w(a.weight, a.weight_dtype, 1.f, base);
   Param<NV, V> pw(a.post_weight, a.post_weight_dtype, 1.f, base), pb(a.post_bias, a.post_bias_dtype, 0.f, base);
   w.fill(&place, s);
-  if constexpr (Full) {
-    pw.fill(&place, s);
-    if constexpr (Bias) pb.fill(&place, s);
-    if (one_gate) q.fill(&place, s);
-  }
+  if constexpr (Full) pw.fill(&place, s, Samples ? nullptr : a.gate, a.gate_dtype);  // g o w_post for one gate
+  if constexpr (Samples && Bias) pb.fill(&place, s);
   __syncthreads();
   const float inv_d = 1.0f / static_cast<float>(s.d);
-  float acc_w[NV][V], acc_b[Bias ? NV : 1][V], acc_pw[Full ? NV : 1][V], acc_pb[Full && Bias ? NV : 1][V], acc_g[Full ? NV : 1][V];
+  float acc_w[NV][V], acc_b[Bias ? NV : 1][V], acc_pw[Full ? NV : 1][V], acc_pb[Full && Bias ? NV : 1][V], acc_g[Samples ? NV : 1][V];
   const auto clear = [](auto& acc) {
     for (auto& k : acc)
       for (float& v : k) v = 0.f;
@@ -107,13 +109,23 @@ __global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Full, Bias))
   clear(acc_w), clear(acc_b), clear(acc_pw), clear(acc_pb), clear(acc_g);
   int64_t sample = -1, until = -1;  // of the gate whose sums are held; the first row of the next sample
   const auto flush_gate = [&]() {
-    if constexpr (Full) {
+    if constexpr (Samples) {
       if (sample < 0 || (wanted & (1 << kGate)) == 0) return;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         if (c.own[k]) store_vec<float, V>(gates + (worker + sample) * s.d + c.at[k], acc_g[k]);
       }
       clear(acc_g);
+    }
+  };
+  // u = (u - <u> - yh <u yh>) / sd from the sums p; yh is overwritten
+  const auto through_norm = [&](float (&u)[NV][V], float (&yh)[NV][V], const float (&p)[2], float rstd) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      vmul<kPairs>(yh[k], -p[1] * inv_d);
+      vadd<kPairs>(u[k], yh[k]);
+      if (s.layer) vadd<kPairs>(u[k], -p[0] * inv_d);
+      vmul<kPairs>(u[k], rstd);
     }
   };
   for (int64_t row = run.first; row < run.last; ++row) {
@@ -151,17 +163,34 @@ __global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Full, Bias))
     }
     store_row(dx, c, r);
     dx += s.d;
-    if constexpr (Full) {
-      if (one_gate) {
-        q.row(c, r);
-      } else {
-        if (row >= until) {
-          flush_gate();
-          sample = row / s.seq;
-          until = (sample + 1) * s.seq;
-        }
-        load_param_row(a.gate, a.gate_dtype, sample * s.d, 1.f, c, r);
+    if constexpr (Form == kGradFull) {
+      // One gate: dw_post = g o A, dg = w_post o A + b_post o B and db_post = g o B with A = sum dh o yh (y itself
+      // without its norm) and B = sum dh, so that two sums are held, not three.
+      pw.row(c, f);
+      if (a.post) normalize<kPairs>(y, st.z, st.w);
+      float p[2], p0[2] = {0.f, 0.f}, p1[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        vmac<kPairs>(acc_pw[k], u[k], y[k]);
+        if constexpr (Bias) vadd<kPairs>(acc_pb[k], u[k]);
+        vmul<kPairs>(u[k], f[k]);
+        if (s.layer) vsum<kPairs>(p0, u[k]);
+        vdot<kPairs>(p1, u[k], y[k]);
       }
+      if (a.post) {
+        p[0] = p0[0] + p0[1];
+        p[1] = p1[0] + p1[1];
+        sum(p, t);
+        through_norm(u, y, p, st.w);
+      }
+    }
+    if constexpr (Samples) {
+      if (row >= until) {
+        flush_gate();
+        sample = row / s.seq;
+        until = (sample + 1) * s.seq;
+      }
+      load_param_row(a.gate, a.gate_dtype, sample * s.d, 1.f, c, r);
       if (!a.post) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -191,19 +220,13 @@ __global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Full, Bias))
         p[0] = p0[0] + p0[1];
         p[1] = p1[0] + p1[1];
         sum(p, t);
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          vmul<kPairs>(y[k], -p[1] * inv_d);
-          vadd<kPairs>(u[k], y[k]);
-          if (s.layer) vadd<kPairs>(u[k], -p[0] * inv_d);
-          vmul<kPairs>(u[k], st.w);
-        }
+        through_norm(u, y, p, st.w);
       }
     }
     if (a.grad_y != nullptr) store_row(dy, c, u);
     dy += s.d;
   }
-  if (!one_gate) flush_gate();
+  if constexpr (Samples) flush_gate();
   // the block's groups together, in order
   const auto finish = [&](auto& acc, int which) {
     if ((wanted & (1 << which)) == 0) return;
@@ -230,10 +253,34 @@ __global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Full, Bias))
   };
   finish(acc_w, kWeight);
   if constexpr (Bias) finish(acc_b, kBias);
+  if constexpr (Form == kGradFull) {
+    float g_row[NV][V], part[NV][V];
+    load_param_row(a.gate, a.gate_dtype, 0, 1.f, c, g_row);
+    if ((wanted & (1 << kGate)) != 0) {
+      float w_row[NV][V];
+      load_param_row(a.post_weight, a.post_weight_dtype, 0, 1.f, c, w_row);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) part[k][j] = w_row[k][j] * acc_pw[k][j];
+      if constexpr (Bias) {
+        load_param_row(a.post_bias, a.post_bias_dtype, 0, 0.f, c, w_row);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) part[k][j] = fmaf(w_row[k][j], acc_pb[k][j], part[k][j]);
+      }
+      finish(part, kGate);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      vmul<kPairs>(acc_pw[k], g_row[k]);
+      if constexpr (Bias) vmul<kPairs>(acc_pb[k], g_row[k]);
+    }
+  }
   if constexpr (Full) {
     finish(acc_pw, kPostWeight);
     if constexpr (Bias) finish(acc_pb, kPostBias);
-    if (one_gate) finish(acc_g, kGate);
   }
   sum.leave();
 }
@@ -301,11 +348,11 @@ int launch_columns_join(const float* parts, int64_t runs, const NormShape& s, in
   return OPUS_OK;
 }
 
-template <typename TX, typename TY, int V, int NV, bool Full, bool Bias, bool Wide>
+template <typename TX, typename TY, int V, int NV, int Form, bool Bias, bool Wide>
 int launch_backward(NormShape s, const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws,
                     cudaStream_t st) {
-  constexpr auto kernel = grad_kernel<TX, TY, V, NV, Full, Bias, Wide>;
-  const int arrays = !Full ? 1 : (Bias ? 3 : 2) + (s.seq == s.rows ? 1 : 0);
+  constexpr auto kernel = grad_kernel<TX, TY, V, NV, Form, Bias, Wide>;
+  const int arrays = Form == kGradJoin ? 1 : Form == kGradSamples && Bias ? 3 : 2;
   const int shared = group_floats(s.group, s.groups, s.ranks) + (s.groups > 1 ? s.group * s.groups * V * NV : 0) +
                      arrays * Param<NV, V>::size(s.group);
   NormLaunch launch;
@@ -321,38 +368,41 @@ int launch_backward(NormShape s, const opus_residual_norm_args& a, int wanted, c
   return launch_columns_join(parts, s.blocks, s, whole, out, gates, per_sample ? a.gate_rows : 0, a.grad_gate, st);
 }
 
-template <typename TX, typename TY, int V, bool Full, bool Bias>
+template <typename TX, typename TY, int V, int Form, bool Bias>
 int backward_by_width(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
   // 16 elements a thread, 8 where the sums of 16 f32 columns would not leave registers enough (with biases) and 8
   // reach the row's end
+  constexpr bool Full = Form != kGradJoin;
   constexpr int kMost = narrow_vectors(V, Full), kFewer = fewer_vectors(V, Full);
   constexpr bool kLean = V == 4 && Full && Bias;
   NormShape s;
   if (a.d > norm_narrow(V, Full)) {
     constexpr int kWide = kLean ? kFewer : kMost;
     const int rc = norm_shape_wide(&a, V, kWide, &s);
-    return rc ? rc : launch_backward<TX, TY, V, kWide, Full, Bias, true>(s, a, wanted, out, ws, st);
+    return rc ? rc : launch_backward<TX, TY, V, kWide, Form, Bias, true>(s, a, wanted, out, ws, st);
   }
   const bool lean = kLean && a.d <= norm_narrow(V, Full) / 2;
   const int nv = norm_shape(&a, V, lean ? kFewer : kMost, &s);
   if constexpr (V > 1) {
-    if (nv == 1) return launch_backward<TX, TY, V, 1, Full, Bias, false>(s, a, wanted, out, ws, st);
+    if (nv == 1) return launch_backward<TX, TY, V, 1, Form, Bias, false>(s, a, wanted, out, ws, st);
   }
   if constexpr (V < 8) {
-    if (nv <= kFewer) return launch_backward<TX, TY, V, kFewer, Full, Bias, false>(s, a, wanted, out, ws, st);
+    if (nv <= kFewer) return launch_backward<TX, TY, V, kFewer, Form, Bias, false>(s, a, wanted, out, ws, st);
   }
-  return launch_backward<TX, TY, V, kMost, Full, Bias, false>(s, a, wanted, out, ws, st);
+  return launch_backward<TX, TY, V, kMost, Form, Bias, false>(s, a, wanted, out, ws, st);
 }
 
 template <typename TX, typename TY, int V>
 int backward_by_form(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
-  const bool full = a.post || a.gate != nullptr;
   const bool bias = a.post_bias != nullptr || (wanted & (1 << kBias)) != 0;
-  if (full)
-    return bias ? backward_by_width<TX, TY, V, true, true>(a, wanted, out, ws, st)
-                : backward_by_width<TX, TY, V, true, false>(a, wanted, out, ws, st);
-  return bias ? backward_by_width<TX, TY, V, false, true>(a, wanted, out, ws, st)
-              : backward_by_width<TX, TY, V, false, false>(a, wanted, out, ws, st);
+  if (a.gate != nullptr && a.gate_rows > 1)
+    return bias ? backward_by_width<TX, TY, V, kGradSamples, true>(a, wanted, out, ws, st)
+                : backward_by_width<TX, TY, V, kGradSamples, false>(a, wanted, out, ws, st);
+  if (a.post || a.gate != nullptr)
+    return bias ? backward_by_width<TX, TY, V, kGradFull, true>(a, wanted, out, ws, st)
+                : backward_by_width<TX, TY, V, kGradFull, false>(a, wanted, out, ws, st);
+  return bias ? backward_by_width<TX, TY, V, kGradJoin, true>(a, wanted, out, ws, st)
+              : backward_by_width<TX, TY, V, kGradJoin, false>(a, wanted, out, ws, st);
 }
 
 template <typename TX, typename TY>
