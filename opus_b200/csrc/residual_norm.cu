@@ -39,8 +39,8 @@ bool norm_params_aligned(const opus_residual_norm_args* a) {
 }
 
 // The launch's shape for vectors of V elements, at most `most` of them (a power of two) a thread: as few threads
-// a row as that allows.  Returns how many vectors a thread (a power of two) those threads need.
-int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s) {
+// a row as that allows, and as many rows as a block of `threads` holds.  Returns how many vectors a thread (a power of two) those threads need.
+int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s, int threads) {
   const int full = (a->d + V - 1) / V;
   int group = 1;
   while (group < 32 && group * most < full) group <<= 1;
@@ -54,7 +54,7 @@ int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s) 
   if (s->seq < 1) s->seq = 1;
   s->d = a->d;
   s->group = group;
-  s->groups = group >= kNormThreads ? 1 : kNormThreads / group;
+  s->groups = group >= threads ? 1 : threads / group;
   s->ranks = 1;
   s->err = nullptr;
   s->layer = a->kind;

@@ -396,7 +396,7 @@ struct NormLaunch {
   }
 };
 
-int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s);
+int norm_shape(const opus_residual_norm_args* a, int V, int most, NormShape* s, int threads = kNormThreads);
 int norm_shape_wide(const opus_residual_norm_args* a, int V, int NV, NormShape* s);
 int check_norm(const char* what, const opus_residual_norm_args* a);
 bool norm_params_aligned(const opus_residual_norm_args* a);

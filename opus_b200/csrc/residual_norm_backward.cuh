@@ -16,8 +16,8 @@
 // through each other's shared memory.  Every sum has a fixed order.
 //
 // Bound: HBM bandwidth (h, dn, dh_in and y read once, dx and dy written once).
-// 65536 x 2048 bf16: RMS joints 210 us, 6.4 TB/s; layer norms with biases 267 us,
-// 5.0 TB/s (161 registers: one block an SM); both norms and a gate 299 us, 5.4
+// 65536 x 2048 bf16: RMS joints 210 us, 6.4 TB/s; layer norms with biases 227 us,
+// 5.9 TB/s; both norms and a gate 299 us, 5.4
 // TB/s (214 registers: eight warps an SM), 368 with a third sum a column for the
 // gate and five parameter arrays read for every row.  8 elements a thread would
 // leave room for twice the warps and took 535 us where 16 took 374.  32768 x 2048
@@ -38,12 +38,12 @@ __device__ __forceinline__ int64_t worker_of(int64_t row, int64_t rows, int64_t 
   return row < cut ? row / (each + 1) : more + (row - cut) / each;
 }
 
+enum GradForm : int { kGradJoin, kGradFull, kGradSamples };  // y as it is; with a norm or one gate; a gate a sample
+
 // Blocks that a multiprocessor's registers have to hold: two where the sums of a thread's columns leave room for them
 // (16384 x 4096 bf16 RMS 111 us, 138 with the registers of one; 500000 x 128 with layer norms 136 and 185), three for
 // 4 elements a thread, otherwise one, which may then use all that it needs (8192 x 8192 f32 with both layer norms
 // 593 us, 674 where the compiler chose).
-enum GradForm : int { kGradJoin, kGradFull, kGradSamples };  // y as it is; with a norm or one gate; a gate a sample
-
 constexpr int grad_blocks(int V, int NV, int form, bool bias) {
   const bool full = form != kGradJoin;
   const int elements = V * NV;
@@ -52,12 +52,18 @@ constexpr int grad_blocks(int V, int NV, int form, bool bias) {
   return V == 8 && !full && !bias ? 2 : 1;
 }
 
+// Threads of a block: 384 where their registers (168 a thread) fill a multiprocessor that a block of 256 would leave a
+// third of (24576 x 1600 bf16 layer norms 86 us, 98 with 256; 65536 x 2048 227 and 264).
+constexpr int grad_threads(int V, int NV, int form, bool bias, bool wide) {
+  return V == 8 && NV == 2 && form == kGradJoin && bias && !wide ? 384 : kNormThreads;
+}
+
 // parts[block or cluster][array][d]: sums over its rows.  gates[worker + sample][d]: sums over the worker's rows of
 // one sample, where each sample has a gate (a step to the next worker or sample is a step to the next slot).
 // Bias: sums for bias and post_bias too.
 // Wide: the blocks of a cluster share a row, each holding a range of its columns.
 template <typename TX, typename TY, int V, int NV, int Form, bool Bias, bool Wide>
-__global__ void __launch_bounds__(kNormThreads, grad_blocks(V, NV, Form, Bias))
+__global__ void __launch_bounds__(grad_threads(V, NV, Form, Bias, Wide), grad_blocks(V, NV, Form, Bias))
     grad_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a, int wanted,
                 float* __restrict__ parts, float* __restrict__ gates) {
   extern __shared__ __align__(16) float shared[];
@@ -389,6 +395,7 @@ int backward_by_width(const opus_residual_norm_args& a, int wanted, const Column
   if constexpr (V < 8) {
     if (nv <= kFewer) return launch_backward<TX, TY, V, kFewer, Form, Bias, false>(s, a, wanted, out, ws, st);
   }
+  norm_shape(&a, V, kMost, &s, grad_threads(V, kMost, Form, Bias, false));
   return launch_backward<TX, TY, V, kMost, Form, Bias, false>(s, a, wanted, out, ws, st);
 }
 
