@@ -377,12 +377,12 @@ int launch_backward(NormShape s, const opus_residual_norm_args& a, int wanted, c
 template <typename TX, typename TY, int V, int Form, bool Bias>
 int backward_by_width(const opus_residual_norm_args& a, int wanted, const ColumnOutputs& out, uint8_t* ws, cudaStream_t st) {
   // 16 elements a thread, 8 where the sums of 16 f32 columns would not leave registers enough (with biases) and 8
-  // reach the row's end
+  // reach the row's end.  Single elements 8: 32768 x 1601 bf16 189 us (16: 224), 16384 x 5001 327 us (506)
   constexpr bool Full = Form != kGradJoin;
-  constexpr int kMost = narrow_vectors(V, Full), kFewer = fewer_vectors(V, Full);
+  constexpr int kMost = V == 1 ? 8 : narrow_vectors(V, Full), kFewer = fewer_vectors(V, Full);
   constexpr bool kLean = V == 4 && Full && Bias;
   NormShape s;
-  if (a.d > norm_narrow(V, Full)) {
+  if (a.d > kNormThreads * kMost * V) {
     constexpr int kWide = kLean ? kFewer : kMost;
     const int rc = norm_shape_wide(&a, V, kWide, &s);
     return rc ? rc : launch_backward<TX, TY, V, kWide, Form, Bias, true>(s, a, wanted, out, ws, st);
