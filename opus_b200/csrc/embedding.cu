@@ -27,8 +27,8 @@
 // hides behind the sort, which leaves HBM idle): 81920 x 768 f32 tokens of a
 // 50257-row table in 102 us (a profile gives 35 to sort and zero, 50 to sum and
 // 16 to join); 16384 x 2048 bf16 of a 151936-row table in 121 to 137 us, where a
-// memset of dW alone takes 160.  Short lists are bound by the chain of three
-// launches: 23 us for 300 tokens.
+// memset of dW alone takes 160.  Lists between those and the short ones (below)
+// are bound by the chain of three launches: 19 to 25 us.
 #include "elements.cuh"
 
 namespace opus {
@@ -761,6 +761,149 @@ int launch_lookup_by_width(const void* tokens, int wide, int64_t n, const void* 
              : launch_lookup_by_token<T, 1>(tokens, wide, n, w, vocab, stride, d, scale, y, err, st);
 }
 
+// ---- short lists: one launch
+// Every block holds the whole list.  It zeroes its share of the rows that no token names, and sums the tokens that
+// occur first at its positions.  A token's few occurrences are summed by every warp for columns of its own; many are
+// cut among the warps, whose sums are joined in order.  No row is written twice.
+//
+// One launch instead of three: 300 tokens of 80 f32 columns 6 us instead of 19, 300 of 768 bf16 18 instead of 24 (a
+// table of 77 MB to zero).  What it does badly is a token that fills the list: 0.44 us for each 64 positions and each
+// 32 vectors of columns (2048 positions of 1600 f32 columns, two tokens: 185 us, 16 sorted), so lists are short while
+// that product is 32 at most (14 us, 19 sorted, at 2048 x 80).
+constexpr int kShortList = 2048;
+constexpr int64_t kShortWork = 32;
+constexpr int kShortThreads = 256, kShortWarps = kShortThreads / 32;
+constexpr int kShortFlags = 1024;    // words: a bit for each row of a block's share
+constexpr int kShortBlocksPerSm = 4;
+constexpr int kShortSerial = 32;     // occurrences that each warp sums alone
+
+template <typename T, int V>
+__device__ __forceinline__ void add_rows(const uint32_t* at, int count, const T* __restrict__ dy, int64_t stride,
+                                         float (&acc)[V]) {
+  constexpr int kBatch = 8;
+  for (int b = 0; b < count; b += kBatch) {
+    Vec<T, V> x[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (b + i < count) x[i] = *reinterpret_cast<const Vec<T, V>*>(dy + static_cast<int64_t>(at[b + i]) * stride);
+      else x[i].zero();
+    }
+    float part[V] = {};  // sums of sums: a chain of 8 + count / 8 additions
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (b + i >= count) break;
+      float r[V];
+      x[i].get(r);
+#pragma unroll
+      for (int k = 0; k < V; ++k) part[k] += r[k];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += part[k];
+  }
+}
+
+template <typename T, typename TO, int V, bool Add>
+__global__ void __launch_bounds__(kShortThreads)
+    short_kernel(const __grid_constant__ KeySource src, int n, int64_t share, const T* __restrict__ dy, int64_t stride,
+                 int d, float scale, TO* __restrict__ dw, int* err) {
+  __shared__ uint32_t keys[kShortList], list[kShortList];
+  __shared__ uint32_t flags[Add ? 1 : kShortFlags];
+  __shared__ float meet[kShortWarps][32 * V];
+  __shared__ int counts[kShortWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t none = static_cast<uint32_t>(src.vocab);
+  for (int i = threadIdx.x; i < n; i += kShortThreads) keys[i] = load_item(src, i, blockIdx.x == 0 ? err : nullptr).x;
+  if constexpr (!Add) {
+    for (int i = threadIdx.x; i < kShortFlags; i += kShortThreads) flags[i] = 0;
+  }
+  __syncthreads();
+  if constexpr (!Add) {
+    const int64_t first = blockIdx.x * share, left = src.vocab - first;
+    const int rows = static_cast<int>(left < share ? (left > 0 ? left : 0) : share);
+    for (int i = threadIdx.x; i < n; i += kShortThreads) {
+      const int64_t at = static_cast<int64_t>(keys[i]) - first;
+      if (at >= 0 && at < rows) atomicOr(&flags[at >> 5], 1u << (at & 31));
+    }
+    __syncthreads();
+    const float zeros[V] = {};
+    for (int r = warp; r < rows; r += kShortWarps) {
+      if (flags[r >> 5] >> (r & 31) & 1u) continue;
+      for (int col = lane * V; col < d; col += 32 * V) store_vec<TO, V>(dw + (first + r) * d + col, zeros);
+    }
+  }
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const uint32_t key = keys[i];
+    if (key == none) continue;
+    bool seen = false;
+    for (int j = threadIdx.x; j < i; j += kShortThreads) seen |= keys[j] == key;
+    if (__syncthreads_or(seen)) continue;
+    // the positions of the token from here on, in order: warps take neighbouring segments of them
+    const int segment = ((n - i + kShortWarps - 1) / kShortWarps + 31) / 32 * 32;
+    const int from = i + warp * segment, to = from + segment < n ? from + segment : n;
+    int count = 0;
+    for (int j = from; j < to; j += 32) count += __popc(__ballot_sync(0xffffffffu, j + lane < to && keys[j + lane] == key));
+    if (lane == 0) counts[warp] = count;
+    __syncthreads();
+    int place = 0, whole = 0;
+    for (int w = 0; w < kShortWarps; ++w) {
+      place += w < warp ? counts[w] : 0;
+      whole += counts[w];
+    }
+    for (int j = from; j < to; j += 32) {
+      const bool mine = j + lane < to && keys[j + lane] == key;
+      const unsigned all = __ballot_sync(0xffffffffu, mine);
+      if (mine) list[place + __popc(all & ((1u << lane) - 1))] = static_cast<uint32_t>(j + lane);
+      place += __popc(all);
+    }
+    __syncthreads();
+    TO* out = dw + static_cast<int64_t>(key) * d;
+    if (whole <= kShortSerial) {
+      for (int col = threadIdx.x * V; col < d; col += kShortThreads * V) {
+        float acc[V] = {};
+        add_rows<T, V>(list, whole, dy + col, stride, acc);
+        write_row<TO, V, Add>(out + col, acc, scale);
+      }
+    } else {
+      const int part = (whole + kShortWarps - 1) / kShortWarps, start = warp * part < whole ? warp * part : whole;
+      const int mine = start + part < whole ? part : whole - start;
+      for (int base = 0; base < d; base += 32 * V) {
+        const int col = base + lane * V;
+        float acc[V] = {};
+        if (col < d) add_rows<T, V>(list + start, mine, dy + col, stride, acc);
+#pragma unroll
+        for (int k = 0; k < V; ++k) meet[warp][k * 32 + lane] = acc[k];
+        __syncthreads();
+        if (warp == 0 && col < d) {
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            for (int w = 1; w < kShortWarps; ++w) acc[k] += meet[w][k * 32 + lane];
+          write_row<TO, V, Add>(out + col, acc, scale);
+        }
+        __syncthreads();
+      }
+    }
+    __syncthreads();  // list and counts are free again
+  }
+}
+
+template <typename T, typename TO, int V>
+int launch_short(const KeySource& src, int64_t n, const void* dy, int64_t stride, int d, float scale, bool accumulate,
+                 void* dw, int64_t grid, int64_t share, int* err, cudaStream_t st) {
+  const auto kernel = accumulate ? short_kernel<T, TO, V, true> : short_kernel<T, TO, V, false>;
+  kernel<<<static_cast<unsigned>(grid), kShortThreads, 0, st>>>(src, static_cast<int>(n), share, static_cast<const T*>(dy),
+                                                                stride, d, scale, static_cast<TO*>(dw), err);
+  note_launch();
+  OPUS_CUDA_TRY(cudaGetLastError());
+  return OPUS_OK;
+}
+
+template <typename T, typename TO>
+int launch_short_by_width(bool vec, const KeySource& src, int64_t n, const void* dy, int64_t stride, int d, float scale,
+                          bool accumulate, void* dw, int64_t grid, int64_t share, int* err, cudaStream_t st) {
+  return vec ? launch_short<T, TO, 16 / sizeof(TO)>(src, n, dy, stride, d, scale, accumulate, dw, grid, share, err, st)
+             : launch_short<T, TO, 1>(src, n, dy, stride, d, scale, accumulate, dw, grid, share, err, st);
+}
+
 constexpr int64_t kMaxTokens = 0x7fffffff;  // positions and keys are 32 bits
 constexpr int kMaxWidth = 65536;
 
@@ -839,13 +982,22 @@ extern "C" int opus_embedding_grad(const void* grad_out, int grad_dtype, int64_t
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const KeySource src{tokens, nullptr, token_bits == 64, vocab, padding_idx};
   const int64_t zero_bytes = accumulate ? 0 : vocab * d * dtype_bytes(out_dtype);
-  rc = p.cluster ? launch_cluster_sort(p, src, n, ws, grad_weight, zero_bytes, err, st)
-                 : launch_global_sort(p, src, n, ws, grad_weight, zero_bytes, err, st);
-  if (rc) return rc;
   const bool f32_out = out_dtype == OPUS_DTYPE_F32;
   const int V = 16 / (f32_out ? 4 : dtype_bytes(grad_dtype));
   const bool vec = d % V == 0 && row_stride % V == 0 && aligned(grad_out, V * dtype_bytes(grad_dtype)) &&
                    aligned(grad_weight, V * dtype_bytes(out_dtype));
+  const int64_t grid = static_cast<int64_t>(sm_count()) * kShortBlocksPerSm, share = (vocab + grid - 1) / grid;
+  const int64_t slabs = (d + 32 * (vec ? V : 1) - 1) / (32 * (vec ? V : 1));
+  if (n <= kShortList && (n <= kShortSerial || (n + 63) / 64 * slabs <= kShortWork) && share <= kShortFlags * 32) {
+    const auto run = grad_dtype == OPUS_DTYPE_F32   ? launch_short_by_width<float, float>
+                     : grad_dtype == OPUS_DTYPE_F16 ? (f32_out ? launch_short_by_width<__half, float> : launch_short_by_width<__half, __half>)
+                     : f32_out                      ? launch_short_by_width<__nv_bfloat16, float>
+                                                    : launch_short_by_width<__nv_bfloat16, __nv_bfloat16>;
+    return run(vec, src, n, grad_out, row_stride, d, scale, accumulate != 0, grad_weight, grid, share, err, st);
+  }
+  rc = p.cluster ? launch_cluster_sort(p, src, n, ws, grad_weight, zero_bytes, err, st)
+                 : launch_global_sort(p, src, n, ws, grad_weight, zero_bytes, err, st);
+  if (rc) return rc;
   if (grad_dtype == OPUS_DTYPE_F32)
     return launch_sums_by_width<float, float>(vec, p, n, vocab, grad_out, row_stride, d, scale, accumulate,
                                               grad_weight, ws, st);

@@ -157,6 +157,23 @@ def test_embedding_grad_sort_sizes(n, V, d):
     ops.check_device_error()
 
 
+@pytest.mark.parametrize("n,V,d,step", [(2, 3, 1601, 1), (32, 50304, 4099, 1), (32, 40, 2048, 1), (33, 9, 1024, 1),
+                                        (33, 9, 1032, 1), (64, 1, 4096, 1), (65, 2, 512, 1), (512, 30, 512, 7),
+                                        (513, 30, 512, 7), (1000, 2, 64, 1), (2048, 1, 128, 1), (2048, 700, 31, 3),
+                                        (2048, 1000003, 8, 977), (256, 19398657, 1, 65537)])
+def test_embedding_grad_short_lists(n, V, d, step):
+    """Lists at the bounds of the single launch: runs of one to all positions, shares of the table with and without names."""
+    g = gen(n + d)
+    t = (torch.arange(n, device=DEV) // 3 * step) % V  # runs of three, and of more where the table is short
+    t = torch.where(torch.rand(n, device=DEV, generator=g) < 0.3, t[torch.randint(0, n, (n,), device=DEV, generator=g)], t)
+    for dtype in (torch.bfloat16, torch.float32):
+        dy = randn(g, n, d, dtype=dtype)
+        a = check_embedding_grad(dy, t, V, scale=0.5)
+        assert torch.equal(a, ops.embedding_grad(dy, t, V, scale=0.5))
+        check_embedding_grad(dy, t.int(), V, padding_idx=int(t[0]), out_dtype=torch.float32)
+        check_embedding_grad(dy, t, V, padding_idx=-1, out=randn(g, V, d, dtype=dtype))
+
+
 @pytest.mark.parametrize("pattern", ["one", "each", "pairs", "descending", "padding", "blocks"])
 def test_embedding_grad_patterns(pattern):
     n, V, d = 6000, 7000, 72
