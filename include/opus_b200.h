@@ -12,8 +12,9 @@
  *     asynchronous with respect to the host; results are valid after the
  *     stream is synchronised.
  *   - Device-side failures (a bounded wait that expired) are recorded in a
- *     per-device error word; opus_device_error() synchronises the device and
- *     returns and clears it.
+ *     per-device error word, tokens outside an embedding's rows in a second
+ *     one; opus_device_error() synchronises the device and returns and clears
+ *     them, opus_kernel_error() the first alone.
  *   - Matrices are row-major.  A layer weight is [d_out, d_in]; its per-sample
  *     gradient is G_b = sum_t dLdZ[b,t,:]^T a[b,t,:], flattened row-major,
  *     which is the element order of the CountSketch tables.
@@ -55,8 +56,15 @@ OPUS_API int opus_abi_version(void);
 OPUS_API const char* opus_last_error(void);
 
 /* Synchronise the current device, store its device error word in *code
- * (0 = none) and clear it.  Returns OPUS_ERR_DEVICE when *code != 0. */
+ * (0 = none) and clear it.  Returns OPUS_ERR_DEVICE when *code != 0.
+ * Tokens outside an embedding's rows have a word of their own (0x202), so
+ * that neither hides the other; it is reported, and cleared, when the
+ * first is 0. */
 OPUS_API int opus_device_error(int* code);
+
+/* The same without the word for tokens, which keeps its value: for code that
+ * checks its own kernels behind a model's. */
+OPUS_API int opus_kernel_error(int* code);
 
 /*
  * Self-test of the bounded waits (no reference counterpart).  Every pipelined
@@ -351,8 +359,8 @@ OPUS_API int opus_muon_S(const void* m, int m_dtype, int d_out, int d_in, void* 
  * Embedding lookup with scaling: out[i] = scale * weight[tokens[i]], n rows of
  * d elements of weight's type.  weight is [vocab, d] with rows row_stride
  * elements apart; tokens are int32 or int64 (token_bits 32 or 64).  A token
- * outside [0, vocab) gives a row of zeros and records 0x202 in the device
- * error word.  n and vocab up to 2^31 - 1, d up to 65536.
+ * outside [0, vocab) gives a row of zeros and records 0x202 in the device's
+ * error word for tokens.  n and vocab up to 2^31 - 1, d up to 65536.
  */
 OPUS_API int opus_embedding(const void* tokens, int token_bits, int64_t n, const void* weight, int dtype,
                             int64_t vocab, int64_t row_stride, int d, float scale, void* out, void* stream);

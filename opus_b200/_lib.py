@@ -51,6 +51,7 @@ SIGNATURES: dict[str, tuple] = {
     "opus_abi_version": (_c_int, []),
     "opus_last_error": (ctypes.c_char_p, []),
     "opus_device_error": (_c_int, [ctypes.POINTER(_c_int)]),
+    "opus_kernel_error": (_c_int, [ctypes.POINTER(_c_int)]),
     "opus_selftest_stalled_wait": (_c_int, [_c_p]),
     "opus_pack_hash_sign": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p]),
     "opus_bucket_max_load": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p]),
@@ -100,7 +101,7 @@ _timer = None  # the active KernelTimer, if any
 _tensor_list = None
 
 # entry points that launch no kernel of their own or only query state
-_UNTIMED = {"opus_abi_version", "opus_last_error", "opus_device_error", "opus_sketch_table_entries",
+_UNTIMED = {"opus_abi_version", "opus_last_error", "opus_device_error", "opus_kernel_error", "opus_sketch_table_entries",
             "opus_muon_S_workspace_bytes", "opus_kernel_launches", "opus_embedding_grad_workspace_bytes",
             "opus_residual_norm_grad_workspace_bytes", "opus_grad_norm_workspace_bytes"}
 
@@ -220,10 +221,11 @@ def check(rc: int, what: str) -> None:
     raise RuntimeError(msg)
 
 
-def device_error() -> int:
-    """Synchronise the current device and return (and clear) its error word."""
+def device_error(tokens: bool = True) -> int:
+    """Synchronise the current device and return (and clear) its error word, or its word for tokens (if asked for)."""
+    name = "opus_device_error" if tokens else "opus_kernel_error"
     code = _c_int(0)
-    rc = load().opus_device_error(ctypes.byref(code))
+    rc = getattr(load(), name)(ctypes.byref(code))
     if rc not in (OPUS_OK, OPUS_ERR_DEVICE):
-        check(rc, "opus_device_error")
+        check(rc, name)
     return int(code.value)

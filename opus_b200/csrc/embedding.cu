@@ -17,7 +17,7 @@
 // with three launches a pass.
 //
 // Tokens outside [0, V) give a row of zeros, add to no gradient, and are
-// recorded in the device error word.  Tokens equal to padding_idx add to no
+// recorded in the device's error word for tokens.  Tokens equal to padding_idx add to no
 // gradient.
 //
 // Bound: HBM bandwidth.  The lookup is a stream of writes: 147456 rows of 1600
@@ -934,7 +934,7 @@ extern "C" int opus_embedding(const void* tokens, int token_bits, int64_t n, con
   if (!tokens || !weight || !out) return set_error(OPUS_ERR_INVALID, "embedding: NULL pointer");
   if (!aligned(tokens, token_bits / 8) || !aligned(weight, dtype_bytes(dtype)) || !aligned(out, dtype_bytes(dtype)))
     return set_error(OPUS_ERR_INVALID, "embedding: a pointer is not aligned to its elements");
-  int* err = device_error_word();
+  int* err = token_error_word();
   if (err == nullptr) return set_error(OPUS_ERR_CUDA, "device error word unavailable");
   const int V = 16 / dtype_bytes(dtype);
   const bool vec = d % V == 0 && row_stride % V == 0 && aligned(weight, 16) && aligned(out, 16);
@@ -977,7 +977,7 @@ extern "C" int opus_embedding_grad(const void* grad_out, int grad_dtype, int64_t
     return set_error(OPUS_ERR_INVALID, "embedding_grad: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
                      (long long)p.bytes);
   if (!aligned(workspace, 256)) return set_error(OPUS_ERR_INVALID, "embedding_grad: workspace must be 256-byte aligned");
-  int* err = device_error_word();
+  int* err = token_error_word();
   if (err == nullptr) return set_error(OPUS_ERR_CUDA, "device error word unavailable");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const KeySource src{tokens, nullptr, token_bits == 64, vocab, padding_idx};

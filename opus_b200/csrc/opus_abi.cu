@@ -1,6 +1,6 @@
 // Library-wide state of libopus_b200.so: error reporting, the per-device
-// error word that bounded device waits write into, device properties and
-// TMA descriptor encoding.
+// error words that bounded device waits and embeddings write into, device
+// properties and TMA descriptor encoding.
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -66,6 +66,11 @@ int* device_error_word() {
     g_dev_err[dev] = p;
   }
   return g_dev_err[dev];
+}
+
+int* token_error_word() {
+  int* p = device_error_word();
+  return p == nullptr ? nullptr : p + 1;
 }
 
 int sm_count() {
@@ -150,6 +155,24 @@ __global__ void stalled_wait_kernel(int* err) {
   }
 }
 
+// Reports and clears the first of the current device's first `words` error words that is set.
+int take_error(const char* what, int words, int* code) {
+  if (code == nullptr) return set_error(OPUS_ERR_INVALID, "%s: code is NULL", what);
+  *code = 0;
+  int* w = device_error_word();
+  if (w == nullptr) return set_error(OPUS_ERR_CUDA, "device error word unavailable");
+  OPUS_CUDA_TRY(cudaDeviceSynchronize());
+  int v[2] = {0, 0};
+  OPUS_CUDA_TRY(cudaMemcpy(v, w, words * sizeof(int), cudaMemcpyDeviceToHost));
+  for (int i = 0; i < words; ++i) {
+    if (v[i] == 0) continue;
+    OPUS_CUDA_TRY(cudaMemset(w + i, 0, sizeof(int)));
+    *code = v[i];
+    return set_error(OPUS_ERR_DEVICE, "device error word set: 0x%x", v[i]);
+  }
+  return OPUS_OK;
+}
+
 }  // namespace
 }  // namespace opus
 
@@ -170,20 +193,8 @@ int64_t opus_kernel_launches(void) { return opus::g_launches.load(std::memory_or
 
 const char* opus_last_error(void) { return opus::g_last_error; }
 
-int opus_device_error(int* code) {
-  if (code == nullptr) return opus::set_error(OPUS_ERR_INVALID, "opus_device_error: code is NULL");
-  *code = 0;
-  int* w = opus::device_error_word();
-  if (w == nullptr) return opus::set_error(OPUS_ERR_CUDA, "device error word unavailable");
-  OPUS_CUDA_TRY(cudaDeviceSynchronize());
-  int v = 0;
-  OPUS_CUDA_TRY(cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost));
-  if (v != 0) {
-    OPUS_CUDA_TRY(cudaMemset(w, 0, sizeof(int)));
-    *code = v;
-    return opus::set_error(OPUS_ERR_DEVICE, "device error word set: 0x%x", v);
-  }
-  return OPUS_OK;
-}
+int opus_device_error(int* code) { return opus::take_error("opus_device_error", 2, code); }
+
+int opus_kernel_error(int* code) { return opus::take_error("opus_kernel_error", 1, code); }
 
 }  // extern "C"

@@ -23,6 +23,7 @@ namespace opus {
 int set_error(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
 int* device_error_word();       // per-device int in global memory (allocated once)
+int* token_error_word();        // another, of tokens outside an embedding's rows
 int sm_count();                 // SMs of the current device
 int max_smem_optin();           // max dynamic shared memory per block (opt-in)
 void note_launch();             // count one kernel launch (opus_kernel_launches)
@@ -53,7 +54,7 @@ cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t sh
   return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
-// Device-side error codes (written to the device error word).
+// Device-side error codes (written to the device error word; kDevBadToken to the one for tokens).
 enum DeviceError : int {
   kDevOk = 0,
   kDevTimeoutProducer = 0x101,

@@ -38,9 +38,14 @@ def _contig(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def check_device_error(what: str = "opus kernel") -> None:
-    """Synchronise and raise if a kernel recorded a device-side error."""
-    code = _lib.device_error()
+def check_device_error(what: str = "opus kernel", tokens: bool = True) -> None:
+    """Synchronise and raise if a kernel recorded a device-side error.
+
+    tokens=False looks past tokens outside an embedding's rows, which stay
+    recorded: the selection path checks its own kernels that way, behind
+    those of the model that it scores.
+    """
+    code = _lib.device_error(tokens)
     if code == _ERR_BAD_PROBS:
         raise ValueError(f"{what}: probabilities do not sum to 1")
     if code == _ERR_BAD_TOKEN:
@@ -63,7 +68,7 @@ def pack_hash_sign(hash_: torch.Tensor, sign: torch.Tensor, k: int, validate: bo
     _lib.check(_lib.load().opus_pack_hash_sign(_ptr(h), _ptr(s), h.numel(), int(k), _ptr(out), _stream(h)),
                "opus_pack_hash_sign")
     if validate:
-        check_device_error("opus_pack_hash_sign (bucket outside [0,k) or sign not +-1)")
+        check_device_error("opus_pack_hash_sign (bucket outside [0,k) or sign not +-1)", tokens=False)
     return out
 
 

@@ -1039,7 +1039,7 @@ def stochastic_greedy_selection(scores, interaction_matrix, K, temperature=1.0):
         raise ValueError("zero-size array to reduction operation maximum which has no identity")
     u = torch.from_numpy(np.random.random_sample(K).astype(np.float64))
     idx = ops.boltzmann_select(s, m, K, float(temperature), u)
-    ops.check_device_error("stochastic_greedy_selection")
+    ops.check_device_error("stochastic_greedy_selection", tokens=False)
     return [np.int64(i) for i in idx.cpu().numpy()]
 
 
@@ -1051,7 +1051,7 @@ def _select_on_device(scores, sim, K, method, temperature):
             raise ValueError("zero-size array to reduction operation maximum which has no identity")
         u = torch.from_numpy(np.random.random_sample(K).astype(np.float64))
         idx = ops.boltzmann_select(scores, sim, K, float(temperature), u)
-        ops.check_device_error("stochastic_greedy_selection")
+        ops.check_device_error("stochastic_greedy_selection", tokens=False)
         return idx
     raise ValueError(f"Unknown selection method: {method}")
 

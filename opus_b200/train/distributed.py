@@ -215,7 +215,7 @@ def select_global(score: torch.Tensor, sim: torch.Tensor, n_select: int, method:
         if uniforms is None:
             uniforms = shared_uniforms(int(n_select), scores.device, group)
         idx = ops.boltzmann_select(scores, blocks, int(n_select), float(temperature), uniforms)
-        ops.check_device_error("global stochastic_greedy_selection")
+        ops.check_device_error("global stochastic_greedy_selection", tokens=False)
     else:
         raise ValueError(f"Unknown selection method: {method}")
     return idx, local_picks(idx, rank, score.numel())
