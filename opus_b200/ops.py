@@ -17,6 +17,8 @@ from . import _lib
 _ERR_BAD_PROBS = 0x301
 _ERR_BAD_TOKEN = 0x202
 
+_devices: set[int] = set()  # that training-step operators ran on
+
 
 def _stream(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
@@ -41,11 +43,18 @@ def _contig(t: torch.Tensor) -> torch.Tensor:
 def check_device_error(what: str = "opus kernel", tokens: bool = True) -> None:
     """Synchronise and raise if a kernel recorded a device-side error.
 
-    tokens=False looks past tokens outside an embedding's rows, which stay
+    Looks at the current device, and at those that training-step operators
+    ran on.  tokens=False looks past tokens outside an embedding's rows, which stay
     recorded: the selection path checks its own kernels that way, behind
     those of the model that it scores.
     """
     code = _lib.device_error(tokens)
+    if not code and _devices - {torch.cuda.current_device()}:
+        for index in sorted(_devices):
+            with torch.cuda.device(index):
+                code = _lib.device_error(tokens)
+            if code:
+                break  # the others keep theirs for the next check
     if code == _ERR_BAD_PROBS:
         raise ValueError(f"{what}: probabilities do not sum to 1")
     if code == _ERR_BAD_TOKEN:
@@ -654,6 +663,7 @@ def _device_index(ref: torch.Tensor, name: str, *others: torch.Tensor | None) ->
 def _call(name: str, index: int, *args) -> None:
     """Call an entry point on device `index`, made current, and its current stream; addresses are plain integers."""
     fn = getattr(_lib.load(), name)
+    _devices.add(index)
     if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
