@@ -200,7 +200,7 @@ def tensor_list():
         try:
             from . import _tensor_list as module
         except ImportError as e:
-            raise ImportError("opus_b200/_tensor_list.so is not built for this Python and torch; run `python -m "
+            raise ImportError("the module opus_b200._tensor_list is not built for this Python and torch; run `python -m "
                               "opus_b200.csrc.build`") from e
         _tensor_list = module
     return _tensor_list

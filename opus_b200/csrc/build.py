@@ -6,7 +6,9 @@ Each .cu file is compiled to an object under opus_b200/_build/ (in parallel,
 skipped when up to date) and linked into opus_b200/libopus_b200.so with the
 CUDA runtime linked statically, so the library has no dependency on the
 Python environment.  tensor_list.cpp becomes the extension module
-opus_b200/_tensor_list.so, against this Python's and torch's headers.
+opus_b200/_tensor_list.<this Python's tag>.so, against this Python's and
+torch's headers; the library is built without it where it cannot be (no torch,
+Python headers or C++ compiler), with a warning.
 """
 from __future__ import annotations
 
@@ -18,6 +20,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -25,7 +28,7 @@ PKG = CSRC.parent
 ROOT = PKG.parent
 BUILD = PKG / "_build"
 LIB = PKG / "libopus_b200.so"
-MODULE = PKG / "_tensor_list.so"
+MODULE = PKG / ("_tensor_list" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -75,11 +78,11 @@ def _compile(src: Path, verbose: bool, extra: list[str]) -> Path:
 
 
 def build_module(verbose: bool = False, force: bool = False) -> Path:
-    """The extension module that walks lists of torch tensors."""
+    """The extension module that walks lists of torch tensors; RuntimeError where it cannot be built."""
     src = CSRC / "tensor_list.cpp"
     spec = importlib.util.find_spec("torch")
     if spec is None or spec.origin is None:
-        raise RuntimeError("torch not found: cannot build _tensor_list.so")
+        raise RuntimeError(f"torch not found: cannot build {MODULE.name}")
     torch_dir = Path(spec.origin).resolve().parent
     cuda_include = Path(nvcc()).resolve().parent.parent / "include"
     if not force and not _stale(MODULE, src, [ROOT / "include" / "opus_b200.h", torch_dir / "version.py"]):
@@ -91,7 +94,10 @@ def build_module(verbose: bool = False, force: bool = False) -> Path:
            str(src), f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"no C++ compiler for {src.name}: {e}") from e
     if res.returncode != 0:
         raise RuntimeError(f"c++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, MODULE)
@@ -107,7 +113,6 @@ def build(verbose: bool = False, force: bool = False, extra: list[str] | None = 
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
         module = ex.submit(build_module, verbose, force)
         list(ex.map(lambda s: _compile(s, verbose, extra), todo))
-        module.result()
     objs = [BUILD / (s.stem + ".o") for s in srcs]
     if todo or not LIB.exists() or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs):
         tmp = LIB.with_suffix(".so.tmp")
@@ -118,6 +123,11 @@ def build(verbose: bool = False, force: bool = False, extra: list[str] | None = 
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    if module.exception() is not None:
+        if not isinstance(module.exception(), RuntimeError):
+            raise module.exception()
+        warnings.warn(f"{LIB.name} is built, {MODULE.name} is not (the operators on lists of tensors need it): "
+                      f"{module.exception()}", RuntimeWarning, stacklevel=2)
     return LIB
 
 

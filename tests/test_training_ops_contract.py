@@ -1,11 +1,14 @@
 """What the training-step operators promise beyond their values, as far as it shows without a GPU."""
 import contextlib
+import importlib.util
+import sysconfig
 import types
 
 import pytest
 import torch
 
 from opus_b200 import _lib, ops
+from opus_b200.csrc import build as nvbuild
 
 
 # ============================================================================ errors recorded on the device
@@ -56,3 +59,36 @@ def test_errors_of_another_device_are_reported(monkeypatch):
     with pytest.raises(IndexError):  # not lost to the other's
         ops.check_device_error()
     assert d.words == {0: 0, 1: 0} and d.current == 0
+
+
+# ============================================================================ build
+@pytest.fixture
+def nvcc_alone(tmp_path, monkeypatch):
+    """The build in a folder of its own, with a compiler that only makes its output file."""
+    fake = tmp_path / "nvcc"
+    fake.write_text('#!/bin/sh\nwhile [ $# -gt 0 ]; do [ "$1" = -o ] && : > "$2"; shift; done\n')
+    fake.chmod(0o755)
+    monkeypatch.setenv("NVCC", str(fake))
+    monkeypatch.setattr(nvbuild, "BUILD", tmp_path / "_build")
+    monkeypatch.setattr(nvbuild, "LIB", tmp_path / "libopus_b200.so")
+    monkeypatch.setattr(nvbuild, "MODULE", tmp_path / nvbuild.MODULE.name)
+    return tmp_path
+
+
+@pytest.mark.parametrize("missing", ["torch", "compiler", "headers"])
+def test_library_is_built_where_the_module_cannot_be(nvcc_alone, monkeypatch, missing):
+    if missing == "torch":
+        find = importlib.util.find_spec
+        monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else find(name, *a))
+    elif missing == "compiler":
+        monkeypatch.setenv("CXX", str(nvcc_alone / "no-such-compiler"))
+    else:
+        monkeypatch.setenv("CXX", "false")  # ends with an error, as a compiler without Python.h does
+    with pytest.warns(RuntimeWarning, match="_tensor_list"):
+        assert nvbuild.build() == nvcc_alone / "libopus_b200.so"
+    assert (nvcc_alone / "libopus_b200.so").exists() and not nvbuild.MODULE.exists()
+
+
+def test_module_is_named_by_interpreter():
+    assert nvbuild.MODULE.name == "_tensor_list" + sysconfig.get_config_var("EXT_SUFFIX")
+    assert _lib.tensor_list().__file__ == str(nvbuild.MODULE)
