@@ -47,6 +47,16 @@ class ScaledEmbedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale = float(scale)
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: int | None = None,
+                        scale: float = 1.0) -> "ScaledEmbedding":
+        """A layer on the rows of embeddings (as they are, not a copy), which do not train while freeze is true."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"embeddings must be [V, d], got {tuple(embeddings.shape)}")
+        layer = cls(*embeddings.shape, padding_idx=padding_idx, scale=scale, device="meta", dtype=embeddings.dtype)
+        layer.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return layer
+
     def forward(self, input: torch.Tensor) -> torch.Tensor:  # noqa: A002 - nn.Embedding's argument name
         return scaled_embedding(input, self.weight, self.scale, self.padding_idx)
 

@@ -9,6 +9,7 @@ import torch
 
 from opus_b200 import _lib, ops
 from opus_b200.csrc import build as nvbuild
+from opus_b200.layers import ScaledEmbedding
 
 
 # ============================================================================ errors recorded on the device
@@ -92,3 +93,20 @@ def test_library_is_built_where_the_module_cannot_be(nvcc_alone, monkeypatch, mi
 def test_module_is_named_by_interpreter():
     assert nvbuild.MODULE.name == "_tensor_list" + sysconfig.get_config_var("EXT_SUFFIX")
     assert _lib.tensor_list().__file__ == str(nvbuild.MODULE)
+
+
+# ============================================================================ layers
+def test_scaled_embedding_from_pretrained():
+    w = torch.randn(6, 4, dtype=torch.bfloat16)
+    layer = ScaledEmbedding.from_pretrained(w, padding_idx=-1, scale=2.0)
+    assert type(layer) is ScaledEmbedding and layer.scale == 2.0 and layer.padding_idx == 5
+    assert layer.weight.data_ptr() == w.data_ptr() and layer.weight.dtype == w.dtype and not layer.weight.requires_grad
+    assert (layer.num_embeddings, layer.embedding_dim) == (6, 4) and list(layer.state_dict()) == ["weight"]
+    assert ScaledEmbedding.from_pretrained(w, freeze=False).weight.requires_grad
+    for like in (dict(max_norm=1.0), dict(sparse=True), dict(scale_grad_by_freq=True)):
+        with pytest.raises(TypeError, match=next(iter(like))):  # not offered, as by the constructor
+            ScaledEmbedding.from_pretrained(w, **like)
+    with pytest.raises(ValueError, match="embeddings"):
+        ScaledEmbedding.from_pretrained(w[0])
+    with pytest.raises(AssertionError):  # nn.Embedding's check
+        ScaledEmbedding.from_pretrained(w, padding_idx=6)
