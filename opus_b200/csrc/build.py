@@ -54,7 +54,7 @@ def sources() -> list[Path]:
 
 
 def headers() -> list[Path]:
-    return sorted(CSRC.glob("*.cuh")) + sorted((ROOT / "include").glob("*.h"))
+    return sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted((ROOT / "include").glob("*.h"))
 
 
 def _stale(obj: Path, src: Path, deps: list[Path]) -> bool:

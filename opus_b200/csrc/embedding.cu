@@ -30,6 +30,7 @@
 // memset of dW alone takes 160.  Lists between those and the short ones (below)
 // are bound by the chain of three launches: 19 to 25 us.
 #include "elements.cuh"
+#include "per_device.h"
 
 namespace opus {
 namespace {
@@ -651,13 +652,13 @@ int launch_sums_by_width(bool wide, const Plan& p, int64_t n, int64_t vocab,
 // Clusters of 2^k sorting blocks that the device holds at once (a cluster lies in one group of its
 // multiprocessors): one that had to wait for others would begin to zero when they have ended.
 int resident_clusters(const cudaLaunchConfig_t& cfg, int k) {
-  static std::atomic<int> known[5];
-  int n = known[k].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaOccupancyMaxActiveClusters(&n, cluster_sort_kernel, &cfg) != cudaSuccess || n < 1) n = 1;
-    known[k].store(n, std::memory_order_relaxed);
-  }
-  return n;
+  static PerDevice<5> known;
+  int device = -1;
+  if (cudaGetDevice(&device) != cudaSuccess) device = -1;
+  return known.get(device, k, 1, [&cfg] {
+    int n = 0;
+    return cudaOccupancyMaxActiveClusters(&n, cluster_sort_kernel, &cfg) == cudaSuccess ? n : 0;
+  });
 }
 
 // zero_bytes of zero (0: none) are zeroed by the blocks that do not sort.

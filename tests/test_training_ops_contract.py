@@ -1,6 +1,8 @@
 """What the training-step operators promise beyond their values, as far as it shows without a GPU."""
 import contextlib
 import importlib.util
+import shutil
+import subprocess
 import sysconfig
 import types
 
@@ -110,3 +112,28 @@ def test_scaled_embedding_from_pretrained():
         ScaledEmbedding.from_pretrained(w[0])
     with pytest.raises(AssertionError):  # nn.Embedding's check
         ScaledEmbedding.from_pretrained(w, padding_idx=6)
+
+
+# ============================================================================ answers kept by device
+PER_DEVICE = r"""
+#include <cstdio>
+#include "per_device.h"
+int main() {
+  static opus::PerDevice<5> known;
+  int asked = 0;
+  auto answer = [&asked](int n) { return [&asked, n] { ++asked; return n; }; };
+  int got[] = {known.get(0, 4, 1, answer(9)), known.get(1, 4, 1, answer(7)), known.get(0, 4, 1, answer(3)),
+               known.get(1, 4, 1, answer(3)), known.get(0, 3, 1, answer(0)), known.get(0, 3, 1, answer(6)),
+               known.get(0, 3, 1, answer(2)), known.get(-1, 0, 1, answer(5)), known.get(64, 0, 1, answer(4))};
+  for (int v : got) std::printf("%d ", v);
+  std::printf("%d", asked);
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs a C++ compiler")
+def test_answers_are_kept_by_device_and_failures_are_not(tmp_path):
+    (tmp_path / "t.cpp").write_text(PER_DEVICE)
+    subprocess.run(["g++", "-std=c++17", f"-I{nvbuild.CSRC}", str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")], check=True)
+    out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout
+    assert out.split() == ["9", "7", "9", "7", "1", "6", "6", "5", "4", "6"]
