@@ -360,7 +360,8 @@ OPUS_API int opus_muon_S(const void* m, int m_dtype, int d_out, int d_in, void* 
  * d elements of weight's type.  weight is [vocab, d] with rows row_stride
  * elements apart; tokens are int32 or int64 (token_bits 32 or 64).  A token
  * outside [0, vocab) gives a row of zeros and records 0x202 in the device's
- * error word for tokens.  n and vocab up to 2^31 - 1, d up to 65536.
+ * error word for tokens.  n and vocab up to 2^31 - 1, d up to 65536.  An out
+ * that overlaps the rows of weight or the tokens is refused (OPUS_ERR_INVALID).
  */
 OPUS_API int opus_embedding(const void* tokens, int token_bits, int64_t n, const void* weight, int dtype,
                             int64_t vocab, int64_t row_stride, int d, float scale, void* out, void* stream);
@@ -373,7 +374,8 @@ OPUS_API int opus_embedding(const void* tokens, int token_bits, int64_t n, const
  * accumulate every row is written, zeros where no token names it; with it only
  * rows that a token names are touched.  Tokens equal to padding_idx (-1: none)
  * and tokens outside [0, vocab) (recorded as above) add nothing.  workspace:
- * opus_embedding_grad_workspace_bytes of device memory, 256-byte aligned.
+ * opus_embedding_grad_workspace_bytes of device memory, 256-byte aligned.  A
+ * grad_weight that overlaps grad_out's rows or the tokens is refused.
  */
 OPUS_API int64_t opus_embedding_grad_workspace_bytes(int64_t n, int64_t vocab, int d);
 OPUS_API int opus_embedding_grad(const void* grad_out, int grad_dtype, int64_t row_stride, const void* tokens,

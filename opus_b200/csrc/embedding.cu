@@ -29,6 +29,8 @@
 // 16 to join); 16384 x 2048 bf16 of a 151936-row table in 121 to 137 us, where a
 // memset of dW alone takes 160.  Lists between those and the short ones (below)
 // are bound by the chain of three launches: 19 to 25 us.
+#include <algorithm>
+
 #include "elements.cuh"
 #include "per_device.h"
 
@@ -920,6 +922,15 @@ int check_sizes(const char* what, int64_t n, int64_t vocab, int d, int token_bit
 
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+// Whether the `bytes` bytes at p share one with `rows` rows of d elements of `size` bytes, row_stride elements apart
+// from q on.
+bool overlaps(const void* p, int64_t bytes, const void* q, int64_t rows, int64_t d, int64_t row_stride, int size) {
+  const int64_t from = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(q));
+  const int64_t run = d * size, stride = std::min(row_stride, int64_t{1} << 56) * size;  // no address is that far away
+  const int64_t row = from < run ? 0 : (from - run) / stride + 1;  // the first that ends behind p
+  return row < rows && row * stride < from + bytes;
+}
+
 }  // namespace
 }  // namespace opus
 
@@ -935,6 +946,10 @@ extern "C" int opus_embedding(const void* tokens, int token_bits, int64_t n, con
   if (!tokens || !weight || !out) return set_error(OPUS_ERR_INVALID, "embedding: NULL pointer");
   if (!aligned(tokens, token_bits / 8) || !aligned(weight, dtype_bytes(dtype)) || !aligned(out, dtype_bytes(dtype)))
     return set_error(OPUS_ERR_INVALID, "embedding: a pointer is not aligned to its elements");
+  const int size = dtype_bytes(dtype);
+  if (overlaps(out, n * d * size, weight, vocab, d, row_stride, size) ||
+      overlaps(out, n * d * size, tokens, 1, n, n, token_bits / 8))
+    return set_error(OPUS_ERR_INVALID, "embedding: out overlaps what is read");
   int* err = token_error_word();
   if (err == nullptr) return set_error(OPUS_ERR_CUDA, "device error word unavailable");
   const int V = 16 / dtype_bytes(dtype);
@@ -978,11 +993,15 @@ extern "C" int opus_embedding_grad(const void* grad_out, int grad_dtype, int64_t
     return set_error(OPUS_ERR_INVALID, "embedding_grad: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
                      (long long)p.bytes);
   if (!aligned(workspace, 256)) return set_error(OPUS_ERR_INVALID, "embedding_grad: workspace must be 256-byte aligned");
+  const int64_t whole = vocab * d * dtype_bytes(out_dtype);
+  if (overlaps(grad_weight, whole, grad_out, n, d, row_stride, dtype_bytes(grad_dtype)) ||
+      overlaps(grad_weight, whole, tokens, 1, n, n, token_bits / 8))
+    return set_error(OPUS_ERR_INVALID, "embedding_grad: grad_weight overlaps what is read");
   int* err = token_error_word();
   if (err == nullptr) return set_error(OPUS_ERR_CUDA, "device error word unavailable");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const KeySource src{tokens, nullptr, token_bits == 64, vocab, padding_idx};
-  const int64_t zero_bytes = accumulate ? 0 : vocab * d * dtype_bytes(out_dtype);
+  const int64_t zero_bytes = accumulate ? 0 : whole;
   const bool f32_out = out_dtype == OPUS_DTYPE_F32;
   const int V = 16 / (f32_out ? 4 : dtype_bytes(grad_dtype));
   const bool vec = d % V == 0 && row_stride % V == 0 && aligned(grad_out, V * dtype_bytes(grad_dtype)) &&

@@ -705,7 +705,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
 
     weight [V, d] in bf16, f16 or f32 (rows may be apart: a column slice of a
     wider table is read in place).  A token outside [0, V) gives a row of
-    zeros, and the next check_device_error() raises IndexError.
+    zeros, and the next check_device_error() raises IndexError.  An out that
+    shares memory with weight's rows or the tokens is refused.
     """
     tokens, bits = _tokens(tokens)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
@@ -734,7 +735,8 @@ def embedding_grad(grad_out: torch.Tensor, tokens: torch.Tensor, num_embeddings:
     f32 over the positions in order: every call gives the same bits.  Rows of
     padding_idx get nothing.  accumulate=True adds into out and touches only
     rows that a token names; without it the rows of other tokens are zeros.
-    Tokens out of range add nothing and are reported as by embedding().
+    Tokens out of range add nothing and are reported as by embedding().  An
+    out that shares memory with grad_out or the tokens is refused.
     """
     tokens, bits = _tokens(tokens)
     V = int(num_embeddings)

@@ -45,3 +45,23 @@ def test_bad_token_does_not_hide_an_error_of_the_selection_path():
         with pytest.raises(IndexError, match="token"):
             ops.check_device_error()
         ops.check_device_error()
+
+
+# ============================================================================ outputs that overlap inputs
+def test_embedding_out_may_lie_between_what_is_read_but_not_in_it():
+    table = torch.randint(-9, 10, (12, 16), device=DEV).float()  # sums are exact
+    before = table.clone()
+    t = torch.tensor([3, 0, 11], device=DEV)
+    for bad in (dict(weight=table, out=table[:3]), dict(weight=table[:, :8], out=table.view(-1)[8:32].view(3, 8)),
+                dict(weight=table[4:], out=table[2:5])):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.embedding(t % bad["weight"].shape[0], **bad)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.embedding_grad(table, torch.arange(12, device=DEV), 3, out=table[9:])
+    assert torch.equal(table, before)
+    # in the gap of one row of weight, and behind its rows
+    assert torch.equal(ops.embedding(t[:1], table[:, :8], out=table[5:6, 8:]), before[3:4, :8])
+    assert torch.equal(ops.embedding(t[:1], table[:11], out=table[11:]), table[3:4])
+    assert torch.equal(table[:5], before[:5]) and torch.equal(table[6:11], before[6:11])
+    got = ops.embedding_grad(table[:4], t[:1].expand(4), 8, out=table[4:])
+    assert torch.equal(got[3], table[:4].sum(0)) and not bool(got[:3].any()) and not bool(got[4:].any())

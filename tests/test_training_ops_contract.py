@@ -1,5 +1,6 @@
 """What the training-step operators promise beyond their values, as far as it shows without a GPU."""
 import contextlib
+import ctypes
 import importlib.util
 import shutil
 import subprocess
@@ -137,3 +138,30 @@ def test_answers_are_kept_by_device_and_failures_are_not(tmp_path):
     subprocess.run(["g++", "-std=c++17", f"-I{nvbuild.CSRC}", str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")], check=True)
     out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout
     assert out.split() == ["9", "7", "9", "7", "1", "6", "6", "5", "4", "6"]
+
+
+# ============================================================================ outputs that overlap inputs
+def embedding_rc(tokens, n, weight, vocab, stride, out, d=8, dtype=_lib.DTYPE_F32, bits=64):
+    """opus_embedding at addresses that are never followed: every call is refused before the device is touched."""
+    rc = _lib.load().opus_embedding(tokens, bits, n, weight, dtype, vocab, stride, d, 1.0, out, None)
+    return rc, _lib.last_error()
+
+
+@pytest.mark.parametrize("n,vocab,stride,out", [
+    (4, 10, 8, 4096), (4, 10, 8, 4096 + 9 * 32), (4, 10, 8, 4096 + 9 * 32 + 28), (4, 10, 8, 4096 - 100),
+    (1, 10, 16, 4096 + 3 * 64), (1, 10, 16, 4096 + 3 * 64 + 28), (1, 10, 16, 4096 + 2 * 64 + 36), (2, 10, 16, 4096 + 32),
+    (1, 1, 1 << 62, 4096 + 28), (1, 2, 1 << 62, 4096), (4, 10, 8, 65536 + 28), (4, 10, 8, 65536 - 124)])
+def test_embedding_refuses_an_out_that_overlaps(n, vocab, stride, out):
+    """weight of f32 rows of 32 bytes at 4096, tokens of 8 bytes at 65536."""
+    rc, message = embedding_rc(65536, n, 4096, vocab, stride, out)
+    assert rc == _lib.OPUS_ERR_INVALID and "overlaps" in message
+
+
+@pytest.mark.parametrize("n,vocab,stride,out,dtype", [
+    (10, 4, 8, 4096, 1), (10, 4, 8, 4096 + 9 * 32 + 28, 1), (10, 4, 8, 4096 - 124, 1), (3, 1, 16, 4096 + 2 * 64, 1),
+    (3, 1, 16, 4096 + 36, 1), (4, 10, 8, 65536 + 28, 1), (4, 10, 8, 65536 - 316, 1), (10, 4, 8, 4096 + 9 * 16 + 12, 0)])
+def test_embedding_grad_refuses_an_out_that_overlaps(n, vocab, stride, out, dtype):
+    """grad_out at 4096, tokens at 65536, an f32 grad_weight."""
+    rc = _lib.load().opus_embedding_grad(4096, dtype, stride, 65536, 64, n, vocab, 8, 1.0, -1, out, _lib.DTYPE_F32, 1,
+                                         1 << 20, 1 << 30, None)
+    assert rc == _lib.OPUS_ERR_INVALID and "overlaps" in _lib.last_error()
