@@ -453,7 +453,8 @@ OPUS_API int opus_residual_norm_grad(const opus_residual_norm_args* args, void* 
  * torch.nn.utils.clip_grad_norm_; a NaN norm gives NaN, an infinite one zeros
  * (and NaN where the element is infinite).  outs[j] is grads[j] (in place), or of any
  * of the types in other memory; a list that would write an element twice, or
- * write one that it reads elsewhere, is refused (OPUS_ERR_INVALID).
+ * write one that it reads elsewhere (the norm among them), is refused
+ * (OPUS_ERR_INVALID).
  * opus_scale_grads: the second half for a *norm that the caller has.
  * workspace: opus_grad_norm_workspace_bytes(count), 8-byte aligned.
  */

@@ -275,15 +275,18 @@ int check_lists(const char* what, const Lists& l, bool outs) {
   return OPUS_OK;
 }
 
-// Refuses a list that writes an element twice or writes what it reads elsewhere (outs[j] == grads[j] aside).
-int check_overlap(const char* what, const Lists& l) {
+// Refuses a list that writes an element twice or writes what it reads elsewhere (outs[j] == grads[j] aside); the norm,
+// which every block reads, counts among what is read, or among what is written.
+int check_overlap(const char* what, const Lists& l, const float* norm, bool norm_written) {
   struct Range {
     uintptr_t start, end;
     bool written;
   };
   try {
     std::vector<Range> r;
-    r.reserve(2 * static_cast<size_t>(l.count));
+    r.reserve(2 * static_cast<size_t>(l.count) + 1);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(norm);
+    if (norm != nullptr) r.push_back({at, at + sizeof(float), norm_written});
     for (int i = 0; i < l.count; ++i) {
       if (l.n[i] == 0) continue;
       const uintptr_t in = reinterpret_cast<uintptr_t>(l.in[i]), out = reinterpret_cast<uintptr_t>(l.out[i]);
@@ -296,7 +299,7 @@ int check_overlap(const char* what, const Lists& l) {
     for (const Range& x : r) {
       if (x.start < written || (x.written && x.start < read))
         return set_error(OPUS_ERR_INVALID, "%s: an element would be written twice, or written and read elsewhere "
-                         "(a tensor listed twice, overlapping views, or outputs that overlap the inputs)", what);
+                         "(a tensor listed twice, overlapping views, or outputs or a norm that overlap the inputs)", what);
       uintptr_t& reach = x.written ? written : read;
       reach = x.end > reach ? x.end : reach;
     }
@@ -446,7 +449,7 @@ extern "C" int opus_scale_grads(const void* const* grads, const int* dtypes, voi
                                 const int64_t* numels, int count, float max_norm, const float* norm, void* stream) {
   const Lists l{grads, outs, numels, dtypes, out_dtypes, count};
   int rc = check_lists("scale_grads", l, true);
-  if (rc == OPUS_OK) rc = check_overlap("scale_grads", l);
+  if (rc == OPUS_OK) rc = check_overlap("scale_grads", l, norm, false);
   if (rc) return rc;
   if (!norm) return set_error(OPUS_ERR_INVALID, "scale_grads: NULL pointer");
   return launch_scale(l, 2, nullptr, 0, max_norm, const_cast<float*>(norm), reinterpret_cast<cudaStream_t>(stream));
@@ -457,7 +460,7 @@ extern "C" int opus_clip_grads(const void* const* grads, const int* dtypes, void
                                int64_t workspace_bytes, float* norm, void* stream) {
   const Lists l{grads, outs, numels, dtypes, out_dtypes, count};
   int rc = check_lists("clip_grads", l, true);
-  if (rc == OPUS_OK) rc = check_overlap("clip_grads", l);
+  if (rc == OPUS_OK) rc = check_overlap("clip_grads", l, norm, true);
   if (rc) return rc;
   rc = check_norm_args("clip_grads", norm_kind, workspace, workspace_bytes, count, norm);
   if (rc) return rc;

@@ -1046,7 +1046,8 @@ def scale_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, n
                 out: Sequence[torch.Tensor] | None = None) -> None:
     """The second half of clip_grads, for a norm that is known: joined over ranks that hold shards, say.
 
-    norm: a float32 scalar on the gradients' device.
+    norm: a float32 scalar on the gradients' device, in none of the tensors
+    that are written.
     """
     g, o, back = _clip_targets(grads, out, "scale_grads")
     if norm.numel() != 1 or norm.dtype != torch.float32:

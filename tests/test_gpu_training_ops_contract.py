@@ -65,3 +65,17 @@ def test_embedding_out_may_lie_between_what_is_read_but_not_in_it():
     assert torch.equal(table[:5], before[:5]) and torch.equal(table[6:11], before[6:11])
     got = ops.embedding_grad(table[:4], t[:1].expand(4), 8, out=table[4:])
     assert torch.equal(got[3], table[:4].sum(0)) and not bool(got[:3].any()) and not bool(got[4:].any())
+
+
+def test_scale_grads_with_a_norm_among_the_gradients():
+    flat = torch.full((9,), 2.0, device=DEV)
+    for bad in ([flat], [flat[:5], flat[5:]]):
+        with pytest.raises(ValueError, match="norm"):
+            ops.scale_grads(bad, 1.0, flat[5])
+    assert bool((flat == 2).all())
+    ops.scale_grads([flat[:5], flat[6:]], 1.0, flat[5])  # beside them
+    c = float(np.float32(1.0) / (np.float32(2.0) + np.float32(1e-6)))
+    assert flat.tolist() == [float(np.float32(2.0) * np.float32(c))] * 5 + [2.0] + [float(np.float32(2.0) * np.float32(c))] * 3
+    out = torch.zeros(9, device=DEV)
+    ops.scale_grads([flat], 1.0, flat[5], out=[out])  # nothing that is read is written
+    assert float(out[5]) == float(np.float32(2.0) * np.float32(c))

@@ -165,3 +165,16 @@ def test_embedding_grad_refuses_an_out_that_overlaps(n, vocab, stride, out, dtyp
     rc = _lib.load().opus_embedding_grad(4096, dtype, stride, 65536, 64, n, vocab, 8, 1.0, -1, out, _lib.DTYPE_F32, 1,
                                          1 << 20, 1 << 30, None)
     assert rc == _lib.OPUS_ERR_INVALID and "overlaps" in _lib.last_error()
+
+
+def test_clip_refuses_a_norm_among_the_gradients():
+    """scale_grads: every block reads the norm, and one might scale it first.  Addresses are never followed."""
+    lib = _lib.load()
+    grads, out, n, ty = (ctypes.c_void_p * 1)(4096), (ctypes.c_void_p * 1)(8192), (ctypes.c_int64 * 1)(6), (ctypes.c_int * 1)(1)
+    ws = ctypes.c_void_p(256)
+    for to, norm in ((grads, 4096), (grads, 4116), (out, 8192 + 20)):
+        assert lib.opus_scale_grads(grads, ty, to, ty, n, 1, 1.0, norm, None) == _lib.OPUS_ERR_INVALID
+        assert "norm" in _lib.last_error()
+    for to, norm in ((grads, 4096), (out, 4116), (out, 8192)):
+        assert lib.opus_clip_grads(grads, ty, to, ty, n, 1, 2, 1.0, ws, 1 << 24, norm, None) == _lib.OPUS_ERR_INVALID
+        assert "norm" in _lib.last_error()
