@@ -16,9 +16,10 @@ from .. import ops
 class _ScaledEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding_idx):
+        out = ops.embedding(tokens, weight, scale=scale)
         ctx.save_for_backward(tokens)
         ctx.vocab, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
-        return ops.embedding(tokens, weight, scale=scale)
+        return out
 
     @staticmethod
     @once_differentiable

@@ -642,7 +642,13 @@ def greedy_select(scores: torch.Tensor, sim: torch.Tensor, n_select: int) -> tor
 _TYPE_CODES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16}
 
 
+def _tensor(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+
+
 def _type_code(t: torch.Tensor, name: str) -> int:
+    _tensor(t, name)
     code = _TYPE_CODES.get(t.dtype)
     if code is None:
         raise ValueError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
@@ -692,8 +698,7 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 # ---------------------------------------------------- training step: embedding
 def _tokens(tokens: torch.Tensor) -> tuple[torch.Tensor, int]:
-    if not isinstance(tokens, torch.Tensor):
-        raise TypeError("tokens must be a torch.Tensor")
+    _tensor(tokens, "tokens")
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
     return _contig(tokens), 64 if tokens.dtype == torch.int64 else 32
@@ -709,11 +714,13 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     shares memory with weight's rows or the tokens is refused.
     """
     tokens, bits = _tokens(tokens)
+    code = _type_code(weight, "weight")
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight must be [V, d], got {tuple(weight.shape)}")
-    code = _type_code(weight, "weight")
     V, d = weight.shape
     shape = (*tokens.shape, d)
+    if out is not None:
+        _tensor(out, "out")
     if out is not None and (out.shape != shape or out.dtype != weight.dtype or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {weight.dtype} tensor of shape {shape}")
     index = _device_index(weight, "weight", tokens, out)
@@ -742,9 +749,9 @@ def embedding_grad(grad_out: torch.Tensor, tokens: torch.Tensor, num_embeddings:
     V = int(num_embeddings)
     if V < 1:
         raise ValueError("num_embeddings must be positive")
+    code = _type_code(grad_out, "grad_out")
     if grad_out.dim() < 1 or grad_out.shape[:-1] != tokens.shape or grad_out.shape[-1] < 1:
         raise ValueError(f"grad_out must be [*{tuple(tokens.shape)}, d], got {tuple(grad_out.shape)}")
-    code = _type_code(grad_out, "grad_out")
     d = grad_out.shape[-1]
     if padding_idx is not None:
         if not -V <= padding_idx < V:
@@ -753,6 +760,7 @@ def embedding_grad(grad_out: torch.Tensor, tokens: torch.Tensor, num_embeddings:
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if out is not None:
+        _tensor(out, "out")
         if out_dtype is not None and out_dtype != out.dtype:
             raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
         if out.shape != (V, d) or not out.is_contiguous():
@@ -847,6 +855,9 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, weight: tor
     stats is what residual_norm_grad needs of the forward.
     """
     post = (post_weight is not None or post_bias is not None) if post is None else bool(post)
+    _tensor(x, "x")
+    if y is not None:
+        _tensor(y, "y")
     n_dtype = x.dtype if y is None else y.dtype
     if out_dtype is not None and out_dtype != n_dtype:
         if y is not None:
@@ -886,6 +897,9 @@ def residual_norm_grad(grad_n: torch.Tensor | None, grad_h: torch.Tensor | None,
     post = (post_weight is not None or post_bias is not None) if post is None else bool(post)
     if grad_n is None and grad_h is None:
         raise ValueError("grad_n or grad_h must be given")
+    for name, t in (("h", h), ("stats", stats), ("y", y), ("grad_n", grad_n), ("grad_h", grad_h)):
+        if t is not None or name in ("h", "stats"):
+            _tensor(t, name)
     n_dtype = y.dtype if y is not None else grad_n.dtype if grad_n is not None else h.dtype
     params = (weight, bias, post_weight, post_bias, gate)
     a, kept = _norm_args(h, y, n_dtype, params, post, kind, 0.0, float(residual_scale))
@@ -1050,6 +1064,7 @@ def scale_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, n
     that are written.
     """
     g, o, back = _clip_targets(grads, out, "scale_grads")
+    _tensor(norm, "norm")
     if norm.numel() != 1 or norm.dtype != torch.float32:
         raise ValueError(f"norm must be a float32 scalar, got {norm.dtype} {tuple(norm.shape)}")
     if not g.count:

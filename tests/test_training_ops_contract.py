@@ -12,7 +12,7 @@ import torch
 
 from opus_b200 import _lib, ops
 from opus_b200.csrc import build as nvbuild
-from opus_b200.layers import ScaledEmbedding
+from opus_b200.layers import ScaledEmbedding, scaled_embedding
 
 
 # ============================================================================ errors recorded on the device
@@ -178,3 +178,21 @@ def test_clip_refuses_a_norm_among_the_gradients():
     for to, norm in ((grads, 4096), (out, 4116), (out, 8192)):
         assert lib.opus_clip_grads(grads, ty, to, ty, n, 1, 2, 1.0, ws, 1 << 24, norm, None) == _lib.OPUS_ERR_INVALID
         assert "norm" in _lib.last_error()
+
+
+# ============================================================================ arguments that are no tensors
+def test_arguments_that_are_no_tensors_are_named():
+    x, t, stats = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 4)
+    for name, call in (("weight", lambda: ops.embedding(t, [[1.0]])), ("out", lambda: ops.embedding(t, x, out=[x])),
+                       ("weight", lambda: scaled_embedding(t, [[1.0]])),
+                       ("grad_out", lambda: ops.embedding_grad([1.0], t, 3)), ("out", lambda: ops.embedding_grad(x, t, 3, out=[x])),
+                       ("x", lambda: ops.residual_norm([1.0])), ("y", lambda: ops.residual_norm(x, [1.0])),
+                       ("weight", lambda: ops.residual_norm(x, weight=[1.0] * 8)), ("gate", lambda: ops.residual_norm(x, x, gate=1.0)),
+                       ("grad_n", lambda: ops.residual_norm_grad([1.0], None, x, stats)),
+                       ("grad_h", lambda: ops.residual_norm_grad(None, 1.0, x, stats)),
+                       ("h", lambda: ops.residual_norm_grad(x, None, None, stats)),
+                       ("stats", lambda: ops.residual_norm_grad(x, None, x, None)),
+                       ("y", lambda: ops.residual_norm_grad(x, None, x, stats, 1.0)),
+                       ("norm", lambda: ops.scale_grads([x], 1.0, 3.0))):
+        with pytest.raises(TypeError, match=rf"^{name} must be a torch.Tensor"):
+            call()
