@@ -10,10 +10,11 @@
 // Bound: HBM bandwidth; x and y are read once, h and n written once, nothing
 // else but 16 bytes of statistics a row.  65536 x 2048 bf16: 185 us, 5.8 TB/s;
 // 32768 x 2048 f32 185 us, 5.8 TB/s.  With norms on both sides and a gate 181 us,
-// 5.9 TB/s (f32 186): the gate that all rows share is folded into post_weight and
+// 5.9 TB/s: the gate that all rows share is folded into post_weight and
 // post_bias once a block, and biases that are not there are not read.  Reading
 // all five arrays from shared memory for every row took 213 us, its warps
-// waiting for that memory most.
+// waiting for that memory most.  f32: 175 us, 6.1 TB/s, with the gate apart
+// (gate_apart).
 #pragma once
 
 #include "residual_norm.cuh"
@@ -29,8 +30,8 @@ enum Form : int { kAlone, kJoin, kFull };  // no y; y; y with a norm or a gate
 // both norms and a gate).
 enum Split : int { kBlock, kLargeBlock, kCluster };
 
-// Bias: with a bias or post_bias.
-template <typename TX, typename TY, int V, int NV, int F, bool Bias, int By>
+// Bias: with a bias or post_bias.  Apart: one gate for all rows, in an array of its own (ones where there is none).
+template <typename TX, typename TY, int V, int NV, int F, bool Bias, int By, bool Apart>
 __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormThreads,
                                   By == kLargeBlock ? 1 : F == kFull || V < 8 ? 2 : 3)
     residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
@@ -60,13 +61,15 @@ __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormTh
   float* place = shared + group_floats(s.group, s.groups, Wide ? s.ranks : 1);
   Param<NV, V> w(a.weight, a.weight_dtype, 1.f, base), b(a.bias, a.bias_dtype, 0.f, base);
   Param<NV, V> pw(a.post_weight, a.post_weight_dtype, 1.f, base), pb(a.post_bias, a.post_bias_dtype, 0.f, base);
+  Param<NV, V> q(a.gate, a.gate_dtype, 1.f, base);
   w.fill(&place, s);
   if constexpr (Bias) b.fill(&place, s);
-  const bool one_gate = s.seq == s.rows;  // it is folded into the norm's weight and bias
+  const bool one_gate = s.seq == s.rows;  // it is folded into the norm's weight and bias, or apart
   if constexpr (F == kFull) {
-    const void* gate = one_gate ? a.gate : nullptr;
+    const void* gate = one_gate && !Apart ? a.gate : nullptr;
     pw.fill(&place, s, gate, a.gate_dtype);
     if constexpr (Bias) pb.fill(&place, s, gate, a.gate_dtype);
+    if constexpr (Apart) q.fill(&place, s);
   }
   __syncthreads();
   int64_t until = 0, gate_at = 0;  // the first row of the next sample, this sample's gate
@@ -94,6 +97,11 @@ __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormTh
 #pragma unroll
         for (int k = 0; k < NV; ++k) vfma<kPairs>(u[k], p[k], o[k]);
       } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
+      }
+      if (Apart && one_gate) {
+        q.row(c, p);
 #pragma unroll
         for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
       }
@@ -136,16 +144,30 @@ __global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormTh
   sum.leave();
 }
 
-template <typename TX, typename TY, int V, int NV, int F, bool Bias, int By>
+template <typename TX, typename TY, int V, int NV, int F, bool Bias, int By, bool Apart = false>
 int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t st) {
-  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Bias, By>;
-  const int arrays = (F == kFull ? 2 : 1) * (Bias ? 2 : 1);
+  constexpr auto kernel = residual_norm_kernel<TX, TY, V, NV, F, Bias, By, Apart>;
+  const int arrays = (F == kFull ? 2 : 1) * (Bias ? 2 : 1) + (Apart ? 1 : 0);
   NormLaunch launch;
   const int rc = launch.plan<kernel>(&s, group_floats(s.group, s.groups, s.ranks) + arrays * Param<NV, V>::size(s.group), 32, st);
   if (rc) return rc;
   OPUS_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, kernel, s, a));
   note_launch();
   return OPUS_OK;
+}
+
+// Whether one gate of f32 rows is kept apart.  Folding it takes a read of shared memory and a multiplication from each
+// element, and yet HBM is left less well used where all of a multiprocessor's 16 warps work: the kernel then waits for
+// HBM alone, which moves 6.1 to 6.3 TB/s while the read lies between a row's two sums and 5.5 to 5.8 without it.  512 MB
+// in and out, folded and apart, without biases: RMS norms of 2048 columns 188 and 174 us, 4096 196 and 176, 1792 187 and
+// 172, 768 185 and 176; layer norms of 2048 199 and 172, with biases too; 1024 196 and 175.  Rows that leave warps or
+// lanes idle, or lie in one warp, are bound by what they issue: 1280 columns 175 and 192, 640 177 and 195, 5120 180 and
+// 216, 512 185 and 191; layer norms or biases also where a row takes the block: 3712 columns 179 and 199.  (Rows
+// of five warps would gain apart, 2560 columns 192 and 176, those of six and seven would not.)
+bool gate_apart(const NormShape& s, int slots, bool bias) {
+  if (s.group <= 32 || s.group * s.groups != kNormThreads) return false;
+  if (!s.layer && !bias) return 4 * s.d >= 3 * s.group * slots;
+  return s.groups > 1 && 8 * s.d >= 7 * s.group * slots;
 }
 
 template <typename TX, typename TY, int V, int F, bool Bias>
@@ -169,6 +191,9 @@ int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   }
   if constexpr (V < 8) {
     if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, Bias, kBlock>(s, a, st);
+  }
+  if constexpr (V == 4 && sizeof(TY) == 4 && kBoth) {
+    if (gate_apart(s, V * kMost, Bias)) return launch_forward<TX, TY, V, kMost, F, Bias, kBlock, true>(s, a, st);
   }
   return launch_forward<TX, TY, V, kMost, F, Bias, kBlock>(s, a, st);
 }

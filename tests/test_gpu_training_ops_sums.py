@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from opus_b200 import ops
-from test_gpu_training_ops import U, gen, half_step, norm_case, stats64, wide_mag, within
+from test_gpu_training_ops import U, check_norm, gen, half_step, norm_case, stats64, wide_mag, within
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -106,7 +106,22 @@ def test_embedding_grad_of_no_tokens_zeroes_the_table():
     out.check()
 
 
-# ============================================================================ residual norm, backward
+# ============================================================================ residual norm
+@pytest.mark.parametrize("gate", [None, "channel", "sample"])
+@pytest.mark.parametrize("kind,bias", [("rms", False), ("rms", True), ("layer", False), ("layer", True)])
+@pytest.mark.parametrize("d", [512, 764, 768, 896, 1024, 1532, 1600, 1792, 2044, 2048, 2560, 3712, 4096, 4100])
+def test_residual_norm_where_a_gate_is_kept_apart(d, kind, bias, gate):
+    """f32 rows on both sides of the rule that folds a gate into the norm's weight, and more rows than run at once."""
+    for x_dtype in (torch.float32, torch.bfloat16):
+        check_norm(*norm_case(d, (3, 5), d, x_dtype, post=True, gate=gate, bias=bias), kind=kind, post=True, r=0.5)
+    c, p, _, _ = norm_case(d, (4, 500), d, post=True, gate=gate, bias=bias)
+    n, h, stats = ops.residual_norm(c["x"], c["y"], **p, kind=kind)
+    for rows in (slice(0, 3), slice(497, 500)):  # a row's values do not depend on the rows beside it
+        part = ops.residual_norm(c["x"][:, rows], c["y"][:, rows], **p, kind=kind)
+        assert torch.equal(part[0], n[:, rows]) and torch.equal(part[1], h[:, rows])
+
+
+# ---------------------------------------------------------------------------- backward
 EXACT = [((140000, 1), 8), ((70000,), 24), ((8, 16384), 64), ((1, 100000), 136), ((3, 8192), 1600), ((20, 700), 771),
          ((4, 4096), 4096), ((50, 60), 8192), ((7, 300), 5001), ((2, 600), 16384)]
 
