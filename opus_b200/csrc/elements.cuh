@@ -222,12 +222,7 @@ __device__ __forceinline__ void vdot(float (&s)[2], const float (&a)[V], const f
   }
 }
 
-// One element of an array whose type is known at run time (parameters: read once per block or row).
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
-  if (dtype == OPUS_DTYPE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == OPUS_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
+// One element into an array whose type is known at run time (the parameters' gradients).
 __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
   if (dtype == OPUS_DTYPE_F32) static_cast<float*>(p)[i] = v;
   else if (dtype == OPUS_DTYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);

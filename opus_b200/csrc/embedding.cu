@@ -21,7 +21,7 @@
 // gradient.
 //
 // Bound: HBM bandwidth.  The lookup is a stream of writes: 147456 rows of 1600
-// bf16 elements in 96 to 105 us, 4.5 to 4.9 TB/s written (a memset on the same
+// bf16 elements in 95 to 97 us, 4.9 TB/s written (a memset on the same
 // device writes 3.9, a copy moves 6.5).  The gradient reads dY once, whole rows in sorted
 // order, and writes dW, the named rows twice (zeros, then sums: the zeroing
 // hides behind the sort, which leaves HBM idle): 81920 x 768 f32 tokens of a

@@ -20,12 +20,14 @@ namespace opus {
 
 constexpr int kNormMaxWidth = 16384;
 
-// A block is 256 threads at most, with up to 16 elements a thread.  Vectors of one element need more registers each
+// A block has up to 256 threads of up to 16 elements each (the forward's large blocks 512, one form of the backward
+// 384).  Vectors of one element need more registers each
 // (an address, a predicate): with a norm of y or a gate they are 8 at most.  Registers that spill cost more than
 // anything else here: 50000 x 771 f32 with both norms took 335 us forward with 16 elements a thread and 820 bytes
 // spilled, 155 us with 8; without them 128 us with 8, 107 with 16.  Rows wider than a block are split among the
 // blocks of a cluster, which have the same registers each and share the row's sums.
 constexpr int kNormThreads = 256;
+constexpr int kNormMostThreads = 512;
 constexpr int narrow_vectors(int V, bool full) { return V == 1 && full ? 8 : 16 / V; }
 constexpr int norm_narrow(int V, bool full) { return kNormThreads * narrow_vectors(V, full) * V; }
 // the smaller choice for shorter rows (vectors of 8: one vector)
@@ -86,7 +88,8 @@ struct GroupSum {
     span = s.groups * slots;
     const int g = static_cast<int>(threadIdx.x) / s.group;
     buf = shared + g * slots;
-    barrier = 1 + g;  // named barriers 1 to 15: a block has at most 4 groups of more than a warp
+    static_assert(kNormMostThreads / 64 < 16, "a named barrier, 1 to 15, for each group of more than a warp");
+    barrier = 1 + g;
     if (SubWarp && s.group < 32) lanes = ((1u << s.group) - 1) << ((threadIdx.x & 31) / s.group * s.group);
     for (int i = threadIdx.x; i < 4 * span; i += blockDim.x) shared[i] = 0.f;
     if constexpr (Cluster) {

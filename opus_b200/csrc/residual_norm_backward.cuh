@@ -10,10 +10,11 @@
 //
 // One kernel reads each row once, writes dx and dy, and keeps a column's sums
 // over its run of rows in registers (16 columns a thread, up to five sums each); a
-// second kernel joins the runs.  More than 256 threads would have too few
-// registers for that: rows wider than such a block holds (4096 elements, or
-// 2048) are split among the blocks of a cluster, which exchange the row's sums
-// through each other's shared memory.  Every sum has a fixed order.
+// second kernel joins the runs.  Blocks of 512 threads would have too few
+// registers for that (all but one form have 256, that one 384): rows wider than
+// 256 threads hold (4096 elements, or 2048) are split among the blocks of a
+// cluster, which exchange the row's sums through each other's shared memory.
+// Every sum has a fixed order.
 //
 // Bound: HBM bandwidth (h, dn, dh_in and y read once, dx and dy written once).
 // 65536 x 2048 bf16: RMS joints 210 us, 6.4 TB/s; layer norms with biases 227 us,
@@ -54,8 +55,10 @@ constexpr int grad_blocks(int V, int NV, int form, bool bias) {
 
 // Threads of a block: 384 where their registers (168 a thread) fill a multiprocessor that a block of 256 would leave a
 // third of (24576 x 1600 bf16 layer norms 86 us, 98 with 256; 65536 x 2048 227 and 264).
+constexpr int kGradLargeThreads = 384;
+static_assert(kGradLargeThreads <= kNormMostThreads, "groups of a block");
 constexpr int grad_threads(int V, int NV, int form, bool bias, bool wide) {
-  return V == 8 && NV == 2 && form == kGradJoin && bias && !wide ? 384 : kNormThreads;
+  return V == 8 && NV == 2 && form == kGradJoin && bias && !wide ? kGradLargeThreads : kNormThreads;
 }
 
 // parts[block or cluster][array][d]: sums over its rows.  gates[worker + sample][d]: sums over the worker's rows of

@@ -32,7 +32,7 @@ enum Split : int { kBlock, kLargeBlock, kCluster };
 
 // Bias: with a bias or post_bias.  Apart: one gate for all rows, in an array of its own (ones where there is none).
 template <typename TX, typename TY, int V, int NV, int F, bool Bias, int By, bool Apart>
-__global__ void __launch_bounds__(By == kLargeBlock ? 2 * kNormThreads : kNormThreads,
+__global__ void __launch_bounds__(By == kLargeBlock ? kNormMostThreads : kNormThreads,
                                   By == kLargeBlock ? 1 : F == kFull || V < 8 ? 2 : 3)
     residual_norm_kernel(const __grid_constant__ NormShape s, const __grid_constant__ opus_residual_norm_args a) {
   extern __shared__ __align__(16) float shared[];
@@ -176,6 +176,7 @@ int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   constexpr bool kBoth = F == kFull;
   constexpr int kMost = narrow_vectors(V, kBoth), kFewer = fewer_vectors(V, kBoth);
   if constexpr (V > 1) {  // single elements would need 1024 threads of 64 registers
+    static_assert(2 * kNormThreads == kNormMostThreads, "what a large block holds");
     if (a.d > norm_narrow(V, kBoth) && a.d <= 2 * norm_narrow(V, kBoth)) {
       norm_shape(&a, V, kMost, &s);
       return launch_forward<TX, TY, V, kMost, F, Bias, kLargeBlock>(s, a, st);

@@ -1,7 +1,7 @@
 """Gradient clipping by the global norm (the optional clip of the training step, between backward and optimizer).
 
-Same call and result as torch.nn.utils.clip_grad_norm_, on the package's
-kernels: one launch reads every gradient for the norm, one scales them, and
+The call (but for foreach) and the result of torch.nn.utils.clip_grad_norm_, on
+the package's kernels: one launch reads every gradient for the norm, one scales them, and
 gradients within the bound are not written.
 """
 from __future__ import annotations
