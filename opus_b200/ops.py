@@ -648,9 +648,9 @@ def _tensor(t: torch.Tensor, name: str) -> None:
 
 
 def _type_code(t: torch.Tensor, name: str) -> int:
-    _tensor(t, name)
-    code = _TYPE_CODES.get(t.dtype)
+    code = _TYPE_CODES.get(getattr(t, "dtype", None))
     if code is None:
+        _tensor(t, name)
         raise ValueError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
     return code
 
@@ -855,8 +855,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, weight: tor
     stats is what residual_norm_grad needs of the forward.
     """
     post = (post_weight is not None or post_bias is not None) if post is None else bool(post)
-    _tensor(x, "x")
-    if y is not None:
+    if not isinstance(x, torch.Tensor) or not (y is None or isinstance(y, torch.Tensor)):
+        _tensor(x, "x")
         _tensor(y, "y")
     n_dtype = x.dtype if y is None else y.dtype
     if out_dtype is not None and out_dtype != n_dtype:
@@ -897,9 +897,12 @@ def residual_norm_grad(grad_n: torch.Tensor | None, grad_h: torch.Tensor | None,
     post = (post_weight is not None or post_bias is not None) if post is None else bool(post)
     if grad_n is None and grad_h is None:
         raise ValueError("grad_n or grad_h must be given")
-    for name, t in (("h", h), ("stats", stats), ("y", y), ("grad_n", grad_n), ("grad_h", grad_h)):
-        if t is not None or name in ("h", "stats"):
-            _tensor(t, name)
+    T = torch.Tensor
+    if not (isinstance(h, T) and isinstance(stats, T) and (y is None or isinstance(y, T))
+            and (grad_n is None or isinstance(grad_n, T)) and (grad_h is None or isinstance(grad_h, T))):
+        for name, t in (("h", h), ("stats", stats), ("y", y), ("grad_n", grad_n), ("grad_h", grad_h)):
+            if t is not None or name in ("h", "stats"):
+                _tensor(t, name)
     n_dtype = y.dtype if y is not None else grad_n.dtype if grad_n is not None else h.dtype
     params = (weight, bias, post_weight, post_bias, gate)
     a, kept = _norm_args(h, y, n_dtype, params, post, kind, 0.0, float(residual_scale))
