@@ -126,7 +126,7 @@ def build(verbose: bool = False, force: bool = False, extra: list[str] | None = 
     if module.exception() is not None:
         if not isinstance(module.exception(), RuntimeError):
             raise module.exception()
-        warnings.warn(f"{LIB.name} is built, {MODULE.name} is not (the operators on lists of tensors need it): "
+        warnings.warn(f"{LIB.name} is built, {MODULE.name} could not be (operators on lists of tensors need it): "
                       f"{module.exception()}", RuntimeWarning, stacklevel=2)
     return LIB
 

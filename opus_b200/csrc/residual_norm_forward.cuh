@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(By == kLargeBlock ? kNormMostThreads : kNormTh
 #pragma unroll
         for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
       }
-      if (Apart && one_gate) {
+      if (Apart && one_gate) {  // both branches are part of what gate_apart's figures were measured on
         q.row(c, p);
 #pragma unroll
         for (int k = 0; k < NV; ++k) vmul<kPairs>(u[k], p[k]);
@@ -163,9 +163,10 @@ int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t s
 // 172, 768 185 and 176; layer norms of 2048 199 and 172, with biases too; 1024 196 and 175.  Rows that leave warps or
 // lanes idle, or lie in one warp, are bound by what they issue: 1280 columns 175 and 192, 640 177 and 195, 5120 180 and
 // 216, 512 185 and 191; layer norms or biases also where a row takes the block: 3712 columns 179 and 199.  (Rows
-// of five warps would gain apart, 2560 columns 192 and 176, those of six and seven would not.)
+// of five warps would gain apart, 2560 columns 192 and 176, those of six and seven would not.)  A gate
+// for each sample is read from where it is: 2048 columns 172 us, 185 in the kernel for one gate.
 bool gate_apart(const NormShape& s, int slots, bool bias) {
-  if (s.group <= 32 || s.group * s.groups != kNormThreads) return false;
+  if (s.seq != s.rows || s.group <= 32 || s.group * s.groups != kNormThreads) return false;
   if (!s.layer && !bias) return 4 * s.d >= 3 * s.group * slots;
   return s.groups > 1 && 8 * s.d >= 7 * s.group * slots;
 }
