@@ -156,7 +156,7 @@ int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t s
   return OPUS_OK;
 }
 
-// Whether one gate of f32 rows is kept apart.  Folding it takes a read of shared memory and a multiplication from each
+// Whether one gate of f32 streams is kept apart.  Folding it takes a read of shared memory and a multiplication from each
 // element, and yet HBM is left less well used where all of a multiprocessor's 16 warps work: the kernel then waits for
 // HBM alone, which moves 6.1 to 6.3 TB/s while the read lies between a row's two sums and 5.5 to 5.8 without it.  512 MB
 // in and out, folded and apart, without biases: RMS norms of 2048 columns 188 and 174 us, 4096 196 and 176, 1792 187 and
@@ -165,8 +165,13 @@ int launch_forward(NormShape s, const opus_residual_norm_args& a, cudaStream_t s
 // 216, 512 185 and 191; layer norms or biases also where a row takes the block: 3712 columns 179 and 199.  (Rows
 // of five warps would gain apart, 2560 columns 192 and 176, those of six and seven would not.)  A gate
 // for each sample is read from where it is: 2048 columns 172 us, 185 in the kernel for one gate.
-bool gate_apart(const NormShape& s, int slots, bool bias) {
-  if (s.seq != s.rows || s.group <= 32 || s.group * s.groups != kNormThreads) return false;
+// With 16-bit blocks only rows of one or two warps without an idle lane come to wait for HBM: 512 columns 144 and 140 us,
+// layer norms 147 and 133, with biases 151 and 132; 1024 columns 144 and 132, 147 and 137, but 140 and 142 with biases.
+// 960 columns take 141 and 138, layer norms 139 and 146; 768 columns 136 and 152, 2048 139 and 139.
+bool gate_apart(const NormShape& s, int slots, bool bias, bool f32_blocks) {
+  if (s.seq != s.rows || s.group * s.groups != kNormThreads) return false;
+  if (!f32_blocks) return s.d == s.group * slots && s.group <= (bias ? 32 : 64);
+  if (s.group <= 32) return false;
   if (!s.layer && !bias) return 4 * s.d >= 3 * s.group * slots;
   return s.groups > 1 && 8 * s.d >= 7 * s.group * slots;
 }
@@ -194,8 +199,8 @@ int forward_by_width(const opus_residual_norm_args& a, cudaStream_t st) {
   if constexpr (V < 8) {
     if (nv <= kFewer) return launch_forward<TX, TY, V, kFewer, F, Bias, kBlock>(s, a, st);
   }
-  if constexpr (V == 4 && sizeof(TY) == 4 && kBoth) {
-    if (gate_apart(s, V * kMost, Bias)) return launch_forward<TX, TY, V, kMost, F, Bias, kBlock, true>(s, a, st);
+  if constexpr (V == 4 && kBoth) {
+    if (gate_apart(s, V * kMost, Bias, sizeof(TY) == 4)) return launch_forward<TX, TY, V, kMost, F, Bias, kBlock, true>(s, a, st);
   }
   return launch_forward<TX, TY, V, kMost, F, Bias, kBlock>(s, a, st);
 }

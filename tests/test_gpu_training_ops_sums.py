@@ -109,11 +109,12 @@ def test_embedding_grad_of_no_tokens_zeroes_the_table():
 # ============================================================================ residual norm
 @pytest.mark.parametrize("gate", [None, "channel", "sample"])
 @pytest.mark.parametrize("kind,bias", [("rms", False), ("rms", True), ("layer", False), ("layer", True)])
-@pytest.mark.parametrize("d", [512, 764, 768, 896, 1024, 1532, 1600, 1792, 2044, 2048, 2560, 3712, 4096, 4100])
+@pytest.mark.parametrize("d", [512, 516, 764, 768, 896, 1024, 1532, 1600, 1792, 2044, 2048, 2560, 3712, 4096, 4100])
 def test_residual_norm_where_a_gate_is_kept_apart(d, kind, bias, gate):
     """f32 rows on both sides of the rule that folds a gate into the norm's weight, and more rows than run at once."""
-    for x_dtype in (torch.float32, torch.bfloat16):
-        check_norm(*norm_case(d, (3, 5), d, x_dtype, post=True, gate=gate, bias=bias), kind=kind, post=True, r=0.5)
+    for dtype, x_dtype in ((torch.float32, None), (torch.bfloat16, None), (torch.bfloat16, torch.float32),
+                           (torch.float16, torch.float32)):
+        check_norm(*norm_case(d, (3, 5), d, dtype, x_dtype, post=True, gate=gate, bias=bias), kind=kind, post=True, r=0.5)
     c, p, _, _ = norm_case(d, (4, 500), d, post=True, gate=gate, bias=bias)
     n, h, stats = ops.residual_norm(c["x"], c["y"], **p, kind=kind)
     for rows in (slice(0, 3), slice(497, 500)):  # a row's values do not depend on the rows beside it
